@@ -70,6 +70,29 @@ SIGNATURES: dict[str, tuple] = {
         _c_int,
         [_vp, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _vp, _c_i64, _vp, _vp, _vp, _vp, _c_int, _vp, _vp, _c_size, _vp],
     ),
+    "aklr_rotary_embedding": (
+        _c_int,
+        [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp,
+         _c_int, _vp, _c_i64, _c_i64, _c_i64, _c_int, ctypes.c_float, _c_int, _vp],
+    ),
+    "aklr_kv_cache_write_fp8": (
+        _c_int,
+        [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_int,
+         _vp, _c_i64, _c_int, ctypes.c_float, _vp, _c_int, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64,
+         _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _vp],
+    ),
+    "aklr_kv_cache_read_fp8": (
+        _c_int,
+        [_vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp,
+         _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _vp],
+    ),
+    "aklr_tree_attention_fp8_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64]),
+    "aklr_tree_attention_fp8": (
+        _c_int,
+        [_vp, _c_i64, _c_i64, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _vp,
+         _c_i64, _c_i64, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float, _c_int,
+         _vp, _c_size, _vp],
+    ),
     "aklr_probe_hbm_read": (_c_int, [_vp, _c_i64, _vp, _c_int, _c_int, _vp]),
 }
 
@@ -80,6 +103,7 @@ AKLR_ERR_SCRATCH_LIMIT = 5
 NOALLOC_SCRATCH_BYTES = 48 << 20  # AKLR_NOALLOC_SCRATCH_BYTES
 FP8_E4M3FN, FP8_E5M2 = 0, 1
 OUT_BF16, OUT_F16 = 0, 1
+F32 = 2  # AKLR_F32
 B_ROW_MAJOR, B_PRESHUFFLE_16x16 = 0, 1
 SCALES_ROW_MAJOR, SCALES_SHUFFLED = 0, 1
 ABI_VERSION = 1

@@ -45,6 +45,7 @@ enum {
 /* Element types. */
 enum { AKLR_FP8_E4M3FN = 0, AKLR_FP8_E5M2 = 1 };
 enum { AKLR_OUT_BF16 = 0, AKLR_OUT_F16 = 1 };
+enum { AKLR_F32 = 2 }; /* beside them, where an operator also takes fp32 */
 
 /* Weight (b) layouts. PRESHUFFLE_16x16 is aiter shuffle_weight(layout=(16,16)): rows split in
  * tiles of 16, columns in tiles of 32 bytes; tile-major, each tile stored as two 256-byte halves
@@ -260,6 +261,83 @@ int aklr_moe_fp8_experts(const void* hidden, int64_t tokens, int64_t model_dim, 
                          const int32_t* ids, const float* weights, int64_t slots, const void* w1, const float* w1_scale,
                          const void* w2, const float* w2_scale, int w_layout, void* out, void* workspace,
                          size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * Rotary positions. Pair i of the first rotary_dim values of every head, (x[2i], x[2i+1]) when interleaved, else
+ * (x[i], x[i + rotary_dim/2]), turns by the angle positions[t] * frequencies[i] (radians, in 64 bits):
+ * (a, b) -> (a cos - b sin, b cos + a sin) * magnitude, in fp32, rounded once. The other values are copied. No
+ * counterpart in the reference's scope here; it stands between the projections and the cache.
+ * q, k and their outputs: [tokens, heads, head_dim] of dtype (AKLR_OUT_BF16, AKLR_OUT_F16, AKLR_F32), the last
+ * dimension contiguous, token and head strides in elements; pointers and strides multiples of 16 bytes. An output is
+ * its own input (same pointer and strides) or apart from both. k_heads may be 0. positions: int32 or int64 [tokens],
+ * any sign. frequencies: fp64 [rotary_dim / 2]. head_dim and rotary_dim multiples of 16, head_dim <= 1024.
+ */
+int aklr_rotary_embedding(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out,
+                          int64_t q_out_token_stride, int64_t q_out_head_stride, int64_t q_heads, const void* k,
+                          int64_t k_token_stride, int64_t k_head_stride, void* k_out, int64_t k_out_token_stride,
+                          int64_t k_out_head_stride, int64_t k_heads, const void* positions, int positions_64,
+                          const double* frequencies, int64_t tokens, int64_t head_dim, int64_t rotary_dim,
+                          int interleaved, float magnitude, int dtype, hipStream_t stream);
+
+/*
+ * Keys and values into a paged FP8 cache, quantized as they are written; with rotary_dim != 0 k is rotated first (in
+ * fp32, with no rounding before the quantization) and, with q_heads != 0, q into q_out, in the same launch.
+ * The cache: codes e4m3fn [pages, kv_heads, page_size, head_dim] and scales fp32 [pages, kv_heads, page_size], for
+ * keys and for values, each page contiguous and pages k_page, v_page, ks_page, vs_page elements apart. Per token and
+ * head the arithmetic of aklr_per_group_quant_fp8 with one group of head_dim values; a vector holding a NaN or an
+ * infinity is stored as zero codes under a NaN scale.
+ * slots: int32 or int64 [tokens], page * page_size + place in the page; a slot outside [0, pages * page_size) skips
+ * its token (q is rotated all the same). The slots of a call are distinct: of two tokens for one slot, what is stored
+ * is not defined. k, v: [tokens, kv_heads, head_dim] as in aklr_rotary_embedding. head_dim 64, 128 or 256; page_size a
+ * multiple of 16 up to 1024; pages * page_size < 2^31.
+ */
+int aklr_kv_cache_write_fp8(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* q_out,
+                            int64_t q_out_token_stride, int64_t q_out_head_stride, int64_t q_heads, const void* k,
+                            int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                            int64_t v_head_stride, const void* positions, int positions_64, const double* frequencies,
+                            int64_t rotary_dim, int interleaved, float magnitude, const void* slots, int slots_64,
+                            void* k_codes, void* v_codes, float* k_scales, float* v_scales, int64_t k_page,
+                            int64_t v_page, int64_t ks_page, int64_t vs_page, int64_t tokens, int64_t kv_heads,
+                            int64_t head_dim, int64_t pages, int64_t page_size, int dtype, hipStream_t stream);
+
+/*
+ * Cached prefixes read back: rows starts[b] .. starts[b + 1] - 1 of k_out and v_out ([total, kv_heads, head_dim]
+ * contiguous, out_dtype) become positions 0, 1, ... of sequence b, code * scale rounded once. Position p lies in page
+ * block_table[b, p / page_size]; a page outside [0, pages), or past the table's columns, gives zeros. Rows outside
+ * every sequence are left as they were.
+ */
+int aklr_kv_cache_read_fp8(const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales,
+                           int64_t k_page, int64_t v_page, int64_t ks_page, int64_t vs_page, const int32_t* block_table,
+                           int64_t table_stride, int64_t table_cols, const int32_t* starts, int64_t batch, int64_t total,
+                           void* k_out, void* v_out, int64_t kv_heads, int64_t head_dim, int64_t pages,
+                           int64_t page_size, int out_dtype, hipStream_t stream);
+
+/*
+ * Attention of query tokens over a paged FP8 cache (aklr_kv_cache_write_fp8's): decode (one token a sequence), trees
+ * of drafted tokens, chunks of a prompt. Query tokens starts[b] .. starts[b + 1] - 1 of q are sequence b's; their own
+ * keys and values are its last T = starts[b + 1] - starts[b] of seq_lens[b] positions in the cache. Every query token
+ * sees the seq_lens[b] - T positions before them, and of the T those j for which mask[token, j] is not 0 (token counts
+ * over q, j < mask_cols; others are not seen), or, with mask NULL, those up to its own. out[token, head] = softmax over
+ * the positions seen of softmax_scale * (q . k), times v; lse (may be NULL): log of the sum of the exponentials. A token
+ * that sees nothing gets zeros and -infinity. What a token does not see does not reach it, NaN included. Query tokens
+ * outside every sequence keep what out and lse hold. Positions past the block table's columns, and pages outside
+ * [0, pages), are seen by none. starts ascend.
+ * q: [total_q, q_heads, head_dim] bf16 or fp16 (dtype), strides in elements, multiples of 8; out: the same dtype,
+ * contiguous; head h attends kv head h / (q_heads / kv_heads). lse: fp32 [total_q, q_heads]. mask: bytes, rows
+ * mask_stride apart. head_dim 64, 128 or 256; page_size a multiple of 16 up to 1024; table_cols * page_size <= 2^30.
+ * Workspace: aklr_tree_attention_fp8_workspace_bytes(..., capacity = table_cols * page_size), any content. Results do
+ * not depend on the order in which workgroups end.
+ */
+size_t aklr_tree_attention_fp8_workspace_bytes(int64_t total_q, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                               int64_t head_dim, int64_t capacity);
+int aklr_tree_attention_fp8(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_codes,
+                            const void* v_codes, const float* k_scales, const float* v_scales, int64_t k_page,
+                            int64_t v_page, int64_t ks_page, int64_t vs_page, const int32_t* block_table,
+                            int64_t table_stride, int64_t table_cols, const int32_t* seq_lens, const int32_t* starts,
+                            const void* mask, int64_t mask_stride, int64_t mask_cols, void* out, float* lse,
+                            int64_t total_q, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                            int64_t pages, int64_t page_size, float softmax_scale, int dtype, void* workspace,
+                            size_t workspace_bytes, hipStream_t stream);
 
 /*
  * Calibration kernel for the decode roofline (no counterpart in the reference): reads `bytes` from
