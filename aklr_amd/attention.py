@@ -76,7 +76,7 @@ def _run_attention(p: _AttentionPlan):
     return (out, lse) if p.return_lse else out
 
 
-@api("tree_attention_fp8@1.0", _run_attention)
+@api("tree_attention_fp8@1.0", _run_attention, native="tree_attention")
 def tree_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, starts, tree_mask=None, *,
                        softmax_scale=None, return_lse=False, out=None):
     cache = (k_cache, v_cache, k_scale, v_scale)

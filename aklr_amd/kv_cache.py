@@ -153,7 +153,7 @@ def _write_plan(k, v, cache, slots):
     return strides
 
 
-@api("kv_cache_write_fp8@1.0", _run_write)
+@api("kv_cache_write_fp8@1.0", _run_write, native="kv_write")
 def kv_cache_write_fp8(k, v, k_cache, v_cache, k_scale, v_scale, slots):
     cache = (k_cache, v_cache, k_scale, v_scale)
     strides = _write_plan(k, v, cache, slots)
@@ -162,7 +162,7 @@ def kv_cache_write_fp8(k, v, k_cache, v_cache, k_scale, v_scale, slots):
     return _WritePlan(None, k, v, None, None, cache, strides, slots, False, 1.0, None, "write")
 
 
-@api("rotary_kv_cache_write_fp8@1.0", _run_write)
+@api("rotary_kv_cache_write_fp8@1.0", _run_write, native="rotary_kv_write")
 def rotary_kv_cache_write_fp8(q, k, v, positions, frequencies, k_cache, v_cache, k_scale, v_scale, slots, *,
                               interleaved=False, magnitude=1.0, out=None):
     cache = (k_cache, v_cache, k_scale, v_scale)
@@ -221,7 +221,7 @@ def _run_read(p: _ReadPlan):
     return outs[0], outs[1]
 
 
-@api("kv_cache_read_fp8@1.0", _run_read)
+@api("kv_cache_read_fp8@1.0", _run_read, native="kv_read")
 def kv_cache_read_fp8(k_cache, v_cache, k_scale, v_scale, block_table, starts, total, *, out_dtype=None, out_k=None,
                       out_v=None):
     cache = (k_cache, v_cache, k_scale, v_scale)

@@ -170,7 +170,7 @@ def _run_rotary(p: _RotaryPlan):
     return out_q, out_k
 
 
-@api("rotary_embedding@1.0", _run_rotary)
+@api("rotary_embedding@1.0", _run_rotary, native="rotary")
 def rotary_embedding(q, k, positions, frequencies, *, interleaved=False, magnitude=1.0, out_q=None, out_k=None):
     given = [q, positions, frequencies] + [t for t in (k, out_q, out_k) if t is not None]
     if not all(isinstance(t, torch.Tensor) for t in given):
