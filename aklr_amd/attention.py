@@ -66,8 +66,8 @@ def _run_attention(p: _AttentionPlan):
             nbytes = L.aklr_tree_attention_fp8_workspace_bytes(tokens, batch, heads, kv_heads, head_dim, cols * page)
             ws = workspace.get(dev, nbytes)
             st = L.aklr_tree_attention_fp8(
-                q.data_ptr(), q.stride(0), q.stride(1), *(t.data_ptr() for t in p.cache), *p.strides,
-                p.block_table.data_ptr(), table_stride(p.block_table), cols, p.seq_lens.data_ptr(), p.starts.data_ptr(),
+                q.data_ptr(), q.stride(0), q.stride(1), *(t.data_ptr() for t in p.cache), p.strides[0],
+                p.strides[2], p.block_table.data_ptr(), table_stride(p.block_table), cols, p.seq_lens.data_ptr(), p.starts.data_ptr(),
                 mask.data_ptr() if mask is not None else None, mask.stride(0) if mask is not None else 0,
                 mask.shape[1] if mask is not None else 0, out.data_ptr(), lse.data_ptr() if lse is not None else None,
                 tokens, batch, heads, kv_heads, head_dim, pages, page, p.scale, _OUT[q.dtype],
@@ -85,7 +85,7 @@ def tree_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_l
     if not all(isinstance(t, torch.Tensor) for t in given) or return_lse not in (True, False):
         return _OOC
     strides = cache_strides(*cache)
-    if strides is None or q.dim() != 3 or q.dtype not in _OUT:
+    if strides is None or strides[0] != strides[1] or strides[2] != strides[3] or q.dim() != 3 or q.dtype not in _OUT:
         return _OOC
     tokens, heads, head_dim = q.shape
     _, kv_heads, page, cache_dim = k_cache.shape
@@ -98,7 +98,7 @@ def tree_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_l
     batch = seq_lens.numel()
     if batch > 65536 or not starts_ok(starts) or starts.numel() != batch + 1 or not table_ok(block_table, batch):
         return _OOC
-    if block_table.shape[1] * page > 2**30:
+    if block_table.shape[1] * page > 2**28:
         return _OOC
     if tree_mask is not None:
         if tree_mask.dtype not in (torch.bool, torch.uint8) or tree_mask.dim() != 2 or tree_mask.shape[0] != tokens:

@@ -324,16 +324,17 @@ int aklr_kv_cache_read_fp8(const void* k_codes, const void* v_codes, const float
  * [0, pages), are seen by none. starts ascend.
  * q: [total_q, q_heads, head_dim] bf16 or fp16 (dtype), strides in elements, multiples of 8; out: the same dtype,
  * contiguous; head h attends kv head h / (q_heads / kv_heads). lse: fp32 [total_q, q_heads]. mask: bytes, rows
- * mask_stride apart. head_dim 64, 128 or 256; page_size a multiple of 16 up to 1024; table_cols * page_size <= 2^30.
+ * mask_stride apart. head_dim 64, 128 or 256; page_size a multiple of 16 up to 1024; table_cols * page_size <= 2^28; pages
+ * of keys and of values lie code_page elements apart, those of their scales scale_page.
  * Workspace: aklr_tree_attention_fp8_workspace_bytes(..., capacity = table_cols * page_size), any content. Results do
  * not depend on the order in which workgroups end.
  */
 size_t aklr_tree_attention_fp8_workspace_bytes(int64_t total_q, int64_t batch, int64_t q_heads, int64_t kv_heads,
                                                int64_t head_dim, int64_t capacity);
 int aklr_tree_attention_fp8(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_codes,
-                            const void* v_codes, const float* k_scales, const float* v_scales, int64_t k_page,
-                            int64_t v_page, int64_t ks_page, int64_t vs_page, const int32_t* block_table,
-                            int64_t table_stride, int64_t table_cols, const int32_t* seq_lens, const int32_t* starts,
+                            const void* v_codes, const float* k_scales, const float* v_scales, int64_t code_page,
+                            int64_t scale_page, const int32_t* block_table, int64_t table_stride,
+                            int64_t table_cols, const int32_t* seq_lens, const int32_t* starts,
                             const void* mask, int64_t mask_stride, int64_t mask_cols, void* out, float* lse,
                             int64_t total_q, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                             int64_t pages, int64_t page_size, float softmax_scale, int dtype, void* workspace,

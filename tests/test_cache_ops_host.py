@@ -248,13 +248,13 @@ def test_entry_points_reject_before_any_launch(native_lib):
         assert read_call(**{"batch": 1, **bad}) == 1, bad
 
     def attend_call(q=p, total=1, batch=1, hq=2, hkv=1, d=64, page=16, cols=1, dtype=0, ws=None, nbytes=0, qs=128, lens=p):
-        return L.aklr_tree_attention_fp8(q, qs, 64, p, p, p, p, hkv * page * d, hkv * page * d, hkv * page, hkv * page, p, cols, cols,
+        return L.aklr_tree_attention_fp8(q, qs, 64, p, p, p, p, hkv * page * d, hkv * page, p, cols, cols,
                                          lens, p, None, 0, 0, p, None, total, batch, hq, hkv, d, 2, page, 1.0, dtype, ws, nbytes, None)
 
     assert attend_call(total=0) == 0 and attend_call(batch=0) == 0
     assert attend_call(dtype=2) == 2
     for bad in ({"q": None}, {"q": p + 8}, {"hq": 3, "hkv": 2}, {"d": 80}, {"page": 12}, {"qs": 100}, {"lens": None},
-                {"cols": (1 << 26) + 1}, {"cols": 1 << 26, "page": 32}):
+                {"cols": (1 << 24) + 1}, {"cols": 1 << 24, "page": 32}):
         assert attend_call(**bad) == 1, bad
     need = L.aklr_tree_attention_fp8_workspace_bytes(1, 1, 2, 1, 64, 16 * 64)
     assert need > 0 and attend_call(cols=64) == 3 and attend_call(cols=64, ws=p, nbytes=need - 1) == 3
