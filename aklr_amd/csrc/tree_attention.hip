@@ -49,7 +49,8 @@ struct AttnArgs {
   uint64_t* word;
   uint32_t page_magic;  // 2^32 / (page / 8), rounded up
   int table_cols, mask_cols, total, batch, hq, hkv, group, page, pages;
-  int target;  // work items a kv head is cut into, beside one for each tile of rows
+  // Work items a kv head is cut into: as many as run at once where its tiles are few, else `target` beside one a tile
+  int slots, target;
   int dim;     // of a head
   int wide;    // page % 32 == 0
   int cap;     // items a kv head can have
@@ -92,14 +93,20 @@ __device__ __forceinline__ Item find(const AttnArgs& a, int index) {
   };
   One s = look(lane);
   int64_t work = (int64_t)s.tiles * s.units;
+  int all_tiles = s.tiles;
   for (int b0 = 64; b0 < a.batch; b0 += 64) {
     const One x = look(b0 + lane);
     work += (int64_t)x.tiles * x.units;
+    all_tiles += x.tiles;
   }
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) work += __shfl_xor(work, d, 64);
+  for (int d = 1; d < 64; d *= 2) {
+    work += __shfl_xor(work, d, 64);
+    all_tiles += __shfl_xor(all_tiles, d, 64);
+  }
   Item r{};
-  r.chunk = uniform((int)fmin((double)work / a.target, (double)(1 << 23)) + 1);
+  const int target = all_tiles > 0 && 2 * all_tiles <= a.slots ? a.slots - all_tiles : a.target;
+  r.chunk = uniform((int)fmin((double)work / target, (double)(1 << 23)) + 1);
   int items_before = 0, tiles_before = 0;  // of the 64 sequences at hand
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     if (b0) s = look(b0 + lane);
@@ -1124,12 +1131,15 @@ __global__ __launch_bounds__(64 * W, D * NQ > 128 ? 1 : 2) void tile_kernel(cons
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int kTarget = 512;  // workgroups a call is cut into beside one for each tile of rows: two for each CU
+// Workgroups a call is cut into. Two run on a CU; where the tiles of rows are at most half of those, all run at once.
+// Where they are more, 768 beside them let short and long ones even out: 64 sequences and 8 kv heads took 142 us with
+// 512, 127 with 768, 136 with 1024 (more partial results), and 144 with 2048.
+constexpr int kSlots = 512, kTarget = 768;
 constexpr int kMostSplits = 254;  // an arrival word counts to 255
 
 struct AttnPlan {
   int rows;     // a workgroup's
-  int64_t target, tiles, cap;
+  int64_t slots, target, tiles, cap;
   size_t words, bytes;
 };
 
@@ -1137,6 +1147,7 @@ bool plan_attention(int64_t total, int64_t batch, int64_t hq, int64_t hkv, int64
   const int64_t group = hq / hkv, rows = (total * group + batch - 1) / batch;  // of a sequence, on the mean
   p->rows = rows > 64 ? 128 : rows > 32 ? 64 : rows > 16 && d < 256 ? 32 : 16;
   p->target = (kTarget + hkv - 1) / hkv < kMostSplits ? (kTarget + hkv - 1) / hkv : kMostSplits;
+  p->slots = (kSlots + hkv - 1) / hkv < kMostSplits ? (kSlots + hkv - 1) / hkv : kMostSplits;
   p->tiles = total * group / p->rows + (batch < total ? batch : total);
   const int64_t units = (capacity + kUnit - 1) / kUnit;
   p->cap = p->tiles + (units > 1 ? p->target : 0);
@@ -1241,6 +1252,7 @@ extern "C" int aklr_tree_attention_fp8(const void* q, int64_t q_token, int64_t q
   a.page = (int)page_size;
   a.pages = (int)pages;
   a.target = (int)p.target;
+  a.slots = (int)p.slots;
   a.cap = (int)p.cap;
   a.words = (int)p.tiles;
   a.scale_log2 = softmax_scale * 1.44269504f;
