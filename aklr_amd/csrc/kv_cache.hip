@@ -11,6 +11,8 @@ AKLR_SCALAR_FP32_BEGIN
 namespace aklr {
 
 constexpr int kThreads = 256;
+constexpr int kManyGroups = 4096, kTokens = 4;
+constexpr int64_t kManyItems = 1 << 20;
 
 // Eight consecutive values of T (bf16 bits, fp16 or fp32) as fp32, and back with one rounding to nearest even.
 template <typename T>
@@ -261,17 +263,21 @@ __global__ __launch_bounds__(kThreads) void vec_kernel(const VecArgs a, const in
 }
 
 // How many tokens a workgroup takes and how many workgroups share them: one item a lane while that leaves the chip
-// room (a call is latency then), else up to four.
+// room (a call is latency then); else whole tokens, up to four, so that the angles of one are a part of the work of all
+// waves and the items come to full rounds of them.
 template <typename T, int D, bool ROT, bool WRITE>
 int launch_vec(VecArgs& a, int head_dim, hipStream_t stream) {
   const int64_t row = (int64_t)((ROT ? a.q.heads : 0) + a.k.heads + (WRITE ? a.v.heads : 0)) * (head_dim / 16);
   if (row == 0 || a.tokens == 0) return AKLR_OK;
   a.per_wg = (int)(row >= kThreads ? 1 : kThreads / row);
-  if (ROT) a.per_wg = (int)(a.per_wg > 2048 / a.rot ? (2048 / a.rot ? 2048 / a.rot : 1) : a.per_wg);
+  const int most = ROT ? (2048 / a.rot ? 2048 / a.rot : 1) : 1 << 20;  // angles a workgroup keeps: 8 KiB
+  if (a.per_wg > most) a.per_wg = most;
+  int64_t gy = (row * a.per_wg + kThreads - 1) / kThreads;
+  if ((a.tokens + a.per_wg - 1) / a.per_wg * gy > kManyGroups) {
+    while (a.per_wg < kTokens && 2 * a.per_wg <= most) a.per_wg *= 2;
+    gy = 1;
+  }
   const int64_t gx = (a.tokens + a.per_wg - 1) / a.per_wg;
-  const int64_t waves = (row * a.per_wg + kThreads - 1) / kThreads;
-  int64_t gy = waves;
-  if (gx * gy > 4096) gy = (waves + 3) / 4;
   if (gx > 0x7FFFFFFF || gy > 65535) return AKLR_ERR_INVALID_ARGUMENT;
   const size_t lds = ROT ? (size_t)a.per_wg * (a.rot / 2) * sizeof(float2) : 0;
   hipLaunchKernelGGL((vec_kernel<T, D, ROT, WRITE>), dim3((unsigned)gx, (unsigned)gy), dim3(kThreads), lds, stream, a,
@@ -281,7 +287,7 @@ int launch_vec(VecArgs& a, int head_dim, hipStream_t stream) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// A packed prefix out of the pages: workgroup x takes 16 consecutive rows, y keys or values. Rows' places are looked
+// A packed prefix out of the pages: workgroup x takes `rows` consecutive rows, y keys or values. Rows' places are looked
 // up once a row (a binary search of the sequence, then the block table), then a lane turns 16 codes into 16 values.
 struct ReadSide {
   const uint8_t* codes;
@@ -290,18 +296,18 @@ struct ReadSide {
   void* out;
 };
 
-constexpr int kReadRows = 16;
+constexpr int kReadRows = 128;
 
 template <int D, bool F16>
 __global__ __launch_bounds__(kThreads) void read_kernel(ReadSide k, ReadSide v, const int32_t* table, int64_t table_row,
                                                         int64_t table_cols, const int32_t* starts, int batch,
-                                                        int64_t total, int heads, int page, int64_t pages) {
+                                                        int64_t total, int heads, int page, int64_t pages, int rows) {
   constexpr int U = D / 16;
   __shared__ int64_t place[kReadRows];  // page, or -1: no such page, or -2: no such row
   __shared__ int offset[kReadRows];
-  const int64_t r0 = (int64_t)blockIdx.x * kReadRows;
+  const int64_t r0 = (int64_t)blockIdx.x * rows;
   const ReadSide& s = blockIdx.y ? v : k;
-  if (threadIdx.x < kReadRows) {
+  if ((int)threadIdx.x < rows) {
     const int64_t r = r0 + threadIdx.x;
     int lo = 0, hi = batch;  // the first sequence that ends behind r
     while (lo < hi) {
@@ -324,7 +330,7 @@ __global__ __launch_bounds__(kThreads) void read_kernel(ReadSide k, ReadSide v, 
   }
   __syncthreads();
   const int row = heads * U;
-  for (int i = threadIdx.x; i < kReadRows * row; i += kThreads) {
+  for (int i = threadIdx.x; i < rows * row; i += kThreads) {
     const int r = i / row, rest = i - r * row, h = rest / U, u = rest % U;
     const int64_t at = place[r];
     if (at == -2) continue;
@@ -477,10 +483,13 @@ extern "C" int aklr_kv_cache_read_fp8(const void* k_codes, const void* v_codes, 
     return AKLR_ERR_INVALID_ARGUMENT;
   const ReadSide k = {static_cast<const uint8_t*>(k_codes), k_scales, k_page, ks_page, k_out};
   const ReadSide v = {static_cast<const uint8_t*>(v_codes), v_scales, v_page, vs_page, v_out};
-  const dim3 grid((unsigned)((total + kReadRows - 1) / kReadRows), 2);
+  const int64_t row = kv_heads * head_dim / 16;
+  const int64_t fit = (kThreads * (total * row > kManyItems ? 2 : 1) + row - 1) / row;
+  const int64_t rows = fit < kReadRows ? fit : kReadRows;
+  const dim3 grid((unsigned)((total + rows - 1) / rows), 2);
   const auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, k, v, block_table, table_stride, table_cols, starts,
-                       (int)batch, total, (int)kv_heads, (int)page_size, pages);
+                       (int)batch, total, (int)kv_heads, (int)page_size, pages, (int)rows);
   };
   const bool f16 = out_dtype == AKLR_OUT_F16;
   if (head_dim == 64)

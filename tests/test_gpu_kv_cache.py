@@ -65,7 +65,8 @@ def new_cache(pages, heads, dim, page, seed=None):
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("t,hq,hk,d,rot", [(1, 1, 1, 16, 16), (3, 5, 2, 64, 64), (16, 128, 1, 64, 64), (33, 4, 4, 128, 64),
-                                           (7, 3, 1, 96, 48), (2, 1, 1, 1024, 1024), (257, 32, 8, 128, 128), (1, 300, 2, 256, 32)])
+                                           (7, 3, 1, 96, 48), (2, 1, 1, 1024, 1024), (257, 32, 8, 128, 128), (1, 300, 2, 256, 32),
+                                           (2051, 32, 8, 128, 64)])
 def test_rotary(t, hq, hk, d, rot, dtype, interleaved):
     say(f"rotary {t} {hq} {hk} {d} {rot} {dtype} {interleaved}")
     q, k = normal((t, hq, d), dtype, 1), normal((t, hk, d), dtype, 2)
@@ -122,7 +123,7 @@ def place(slots, page):
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("t,h,d,page,pages", [(1, 1, 64, 16, 1), (5, 3, 64, 48, 4), (64, 8, 128, 16, 9), (333, 2, 256, 64, 7),
-                                              (257, 1, 128, 1024, 1), (19, 40, 64, 16, 3)])
+                                              (257, 1, 128, 1024, 1), (19, 40, 64, 16, 3), (2051, 40, 64, 16, 129)])
 def test_write_and_read(t, h, d, page, pages, dtype):
     say(f"write {t} {h} {d} {page} {dtype}")
     k, v = normal((t, h, d), dtype, 1) * 3, normal((t, h, d), dtype, 2)
@@ -183,7 +184,8 @@ def test_write_skips_and_marks():
 
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("t,hq,h,d,rot,dtype", [(1, 1, 1, 64, 64, BF16), (8, 64, 8, 128, 128, BF16), (37, 6, 2, 256, 64, F16),
-                                                (300, 4, 4, 64, 32, BF16), (12, 3, 1, 128, 96, F32)])
+                                                (300, 4, 4, 64, 32, BF16), (12, 3, 1, 128, 96, F32),
+                                                (2051, 33, 4, 128, 128, BF16), (4109, 5, 3, 256, 256, F16)])
 def test_rotary_write(t, hq, h, d, rot, dtype, interleaved):
     say(f"rotary write {t} {hq} {h} {d} {rot} {dtype} {interleaved}")
     page, pages = 16, -(-t // 16) + 2
@@ -223,7 +225,7 @@ def test_rotary_write(t, hq, h, d, rot, dtype, interleaved):
     assert again is q and torch.equal(q, got)
 
 
-@pytest.mark.parametrize("d,h,page", [(64, 2, 16), (128, 8, 48), (256, 1, 64)])
+@pytest.mark.parametrize("d,h,page", [(64, 2, 16), (128, 8, 48), (256, 1, 64), (128, 96, 512)])
 def test_read_packs_ragged_prefixes(d, h, page):
     say(f"read {d} {h} {page}")
     pages = 12
