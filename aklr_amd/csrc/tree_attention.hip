@@ -55,6 +55,7 @@ struct AttnArgs {
   int wide;    // page % 32 == 0
   int cap;     // items a kv head can have
   int words;   // tiles of rows a kv head can have: arrival words
+  int joiners;  // workgroups of a kernel of its own that join a tile's partial results; 0: the last of those that wrote them does
   float scale_log2;
 };
 
@@ -72,8 +73,8 @@ struct Item {
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // Item `index` of a kv head: items are the tiles of each sequence's first chunk, of its second, ..., then the next
-// sequence's. Wave-wide: lane i looks at sequence i of each 64.
-template <int R>
+// sequence's. TILE: the first item of tile `index` of a kv head. Wave-wide: lane i looks at sequence i of each 64.
+template <int R, bool TILE = false>
 __device__ __forceinline__ Item find(const AttnArgs& a, int index) {
   const int lane = threadIdx.x & 63;
   const int64_t most = (int64_t)a.table_cols * a.page;
@@ -117,7 +118,7 @@ __device__ __forceinline__ Item find(const AttnArgs& a, int index) {
       const int x = __shfl_up(items, d, 64), y = __shfl_up(tiles, d, 64);
       if (lane >= d) items += x, tiles += y;
     }
-    const uint64_t past = __ballot(items_before + items > index);
+    const uint64_t past = __ballot(TILE ? tiles_before + tiles > index : items_before + items > index);
     if (past) {
       const int at = __builtin_ctzll(past);
       auto take = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
@@ -126,10 +127,11 @@ __device__ __forceinline__ Item find(const AttnArgs& a, int index) {
       r.splits = take(splits);
       r.chunk = (take(s.units) + r.splits - 1) / r.splits;  // of even length
       r.slot = items_before + take(items) - r.tiles * r.splits;
-      r.split = (index - r.slot) / r.tiles;
-      r.tile = index - r.slot - r.split * r.tiles;
+      r.row_tile = tiles_before + take(tiles) - r.tiles;
+      r.split = TILE ? 0 : (index - r.slot) / r.tiles;
+      r.tile = TILE ? index - r.row_tile : index - r.slot - r.split * r.tiles;
       r.slot += r.tile;
-      r.row_tile = tiles_before + take(tiles) - r.tiles + r.tile;
+      r.row_tile += r.tile;
       r.q0 = take(s.q0);
       r.count = take(s.count);
       r.len = take(s.len);
@@ -407,18 +409,18 @@ __device__ __forceinline__ void finish(const AttnArgs& a, const Item& it, int he
   if (a.lse && d == 0) a.lse[at] = total == 0.0f ? -__builtin_inff() : (best + __log2f(total)) * 0.69314718f;
 }
 
-// The workgroup of a tile of rows that arrives last joins its splits. 16 lanes take a row; where there are fewer rows
-// than 16-lane groups, the groups left over take every second, fourth, ... split each, and their sums meet in LDS
+// Joins the splits of a tile's rows from `first` to `left`, by a workgroup. 16 lanes take a row; where there are fewer
+// rows than 16-lane groups, the groups left over take every second, fourth, ... split each, and their sums meet in LDS
 // (`sum`, a row of D + 4 floats for each group). Always in the same order.
 template <int D, int R, bool F16>
-__device__ __forceinline__ void join(const AttnArgs& a, const Item& it, int head, int left, int r0, float* sum) {
+__device__ __forceinline__ void join(const AttnArgs& a, const Item& it, int head, int first, int left, int r0, float* sum) {
   constexpr int DT = D / 16;
   const int all = blockDim.x >> 4;  // 16-lane groups
   const int chunk = (threadIdx.x & 15) * DT;
   int at_once = all;
-  while (at_once > 1 && at_once / 2 >= left) at_once /= 2;
+  while (at_once > 1 && at_once / 2 >= left - first) at_once /= 2;
   const int groups = all / at_once, r = (threadIdx.x >> 4) % at_once, part = (threadIdx.x >> 4) / at_once;
-  for (int base = 0; base < left; base += at_once) {
+  for (int base = first; base < left; base += at_once) {
     const int row = base + r;
     float best = kNone, total = 0.0f, v[DT];
 #pragma unroll
@@ -463,6 +465,18 @@ __device__ __forceinline__ void join(const AttnArgs& a, const Item& it, int head
   }
 }
 
+// Joins all tiles of rows, `joiners` workgroups a tile.
+template <int D, int R, bool F16>
+__global__ __launch_bounds__(kThreads) void join_kernel(const AttnArgs a) {
+  __shared__ float sum[kThreads / 16][D + 4];
+  const int head = blockIdx.x % a.hkv, index = blockIdx.x / a.hkv;
+  const Item it = find<R, true>(a, index / a.joiners);
+  if (!it.ok || it.splits == 1) return;
+  const int r0 = it.tile * R, left = min(R, it.count * a.group - r0), each = (R + a.joiners - 1) / a.joiners;
+  const int first = index % a.joiners * each;
+  join<D, R, F16>(a, it, head, first, min(left, first + each), r0, sum[0]);
+}
+
 // Rows by the 16 * NQ, tokens by the 32 of a wave. S^T = K Q^T puts a row in a lane (column c of the
 // accumulator) and tokens 4g..4g+3 of each 16 in lane group g, which is just what the second product wants of its
 // operand P^T, so the weights never move between lanes: O^T = V^T P^T sums over k in any order as long as both
@@ -487,7 +501,7 @@ __global__ __launch_bounds__(kThreads, D * NQ > 384 ? 1 : 2) void stream_kernel(
   if (!it.ok) return;
   uint64_t* const word = a.word + (int64_t)head * a.words + it.row_tile;
   uint64_t seen = 0;
-  if (threadIdx.x == 0 && it.splits > 1) seen = splitk_peek(word);
+  if (threadIdx.x == 0 && it.splits > 1 && !a.joiners) seen = splitk_peek(word);
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int rows = it.count * a.group, r0 = it.tile * R, ctx = it.len - it.count;
   const int last_t = (min(r0 + R, rows) - 1) / a.group, first_t = r0 / a.group;
@@ -774,9 +788,9 @@ __global__ __launch_bounds__(kThreads, D * NQ > 384 ? 1 : 2) void stream_kernel(
       finish<DT, F16>(a, it, head, row, d, best, total, v);
     }
   }
-  if (it.splits == 1) return;
+  if (it.splits == 1 || a.joiners) return;
   __shared__ unsigned arrived;
-  if (splitk_arrive(word, seen, it.splits, &arrived)) join<D, R, F16>(a, it, head, min(R, rows - r0), r0, &sum[0][0][0]);
+  if (splitk_arrive(word, seen, it.splits, &arrived)) join<D, R, F16>(a, it, head, 0, min(R, rows - r0), r0, &sum[0][0][0]);
 }
 
 template <bool F16>
@@ -803,9 +817,6 @@ __global__ __launch_bounds__(64 * W, D * NQ > 128 ? 1 : 2) void tile_kernel(cons
   const int head = blockIdx.x % a.hkv, index = blockIdx.x / a.hkv;
   const Item it = find<R>(a, index);
   if (!it.ok) return;
-  uint64_t* const word = a.word + (int64_t)head * a.words + it.row_tile;
-  uint64_t seen = 0;
-  if (threadIdx.x == 0 && it.splits > 1) seen = splitk_peek(word);
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), c = lane & 31, hf = lane >> 5;
   const int rows = it.count * a.group, r0 = it.tile * R, rw = r0 + RW * wave, ctx = it.len - it.count;
   const int last_t = (min(r0 + R, rows) - 1) / a.group;
@@ -1127,24 +1138,25 @@ __global__ __launch_bounds__(64 * W, D * NQ > 128 ? 1 : 2) void tile_kernel(cons
       if (it.splits > 1 && hf == 0) store_partial4(to, R * D + 4 * (row - r0), f32x4{m[n], l[n], 0, 0});
     }
   }
-  if (it.splits == 1) return;
-  __syncthreads();
-  __shared__ unsigned arrived;
-  static_assert(sizeof(ring) >= sizeof(float) * 4 * W * (D + 4), "the joined sums fit the ring");
-  if (splitk_arrive(word, seen, it.splits, &arrived))
-    join<D, R, F16>(a, it, head, min(R, rows - r0), r0, reinterpret_cast<float*>(ring));
 }
 
 // ---------------------------------------------------------------------------------------------------------------
 // Workgroups a call is cut into. Two run on a CU; where the tiles of rows are at most half of those, all run at once.
 // Where they are more, 768 beside them let short and long ones even out: 64 sequences and 8 kv heads took 142 us with
 // 512, 127 with 768, 136 with 1024 (more partial results), and 144 with 2048.
-constexpr int kSlots = 512, kTarget = 768;
+//
+// Joining: the last workgroup of a tile does it in the same launch where there is little to join, else a kernel of its
+// own with up to a workgroup for four rows. A launch costs 2 us more (one row of each of 16 sequences of 1000 tokens and
+// 8 kv heads of 4: 14.0 us joined by the last, 16.4 apart), and the last workgroup alone is bound by how long its loads
+// take (one sequence of 16000: 23.8 and 20.8; of 2000 with 16 rows of one kv head 14.3 and 11.8, of 16000 61.8 and 24.1;
+// 64 rows of each of 8 kv heads 165 and 37).
+constexpr int kSlots = 512, kTarget = 768, kJoinGroups = 2048, kApart = 240;
 constexpr int kMostSplits = 254;  // an arrival word counts to 255
 
 struct AttnPlan {
   int rows;     // a workgroup's
   int64_t slots, target, tiles, cap;
+  int64_t joiners;
   size_t words, bytes;
 };
 
@@ -1156,6 +1168,13 @@ bool plan_attention(int64_t total, int64_t batch, int64_t hq, int64_t hkv, int64
   p->tiles = total * group / p->rows + (batch < total ? batch : total);
   const int64_t units = (capacity + kUnit - 1) / kUnit;
   p->cap = p->tiles + (units > 1 ? p->target : 0);
+  const int64_t tiles = batch * ((rows + p->rows - 1) / p->rows);  // at the mean; with the most splits a tile can have
+  const int64_t splits = units < p->slots / tiles ? units : p->slots / tiles;
+  p->joiners = 0;
+  if (units > 1 && (p->rows > 16 || splits * (rows + 8) >= kApart)) {
+    const int64_t most = p->rows / 4, each = kJoinGroups / (p->tiles * hkv);
+    p->joiners = each < 1 ? 1 : each > most ? most : each;
+  }
   if (p->cap * hkv > 0x7FFFFFFF) return false;
   p->words = ((size_t)(p->tiles * hkv) * 8 + 15) / 16 * 16;
   p->bytes = units > 1 ? p->words + (size_t)(p->cap * hkv * p->rows * (d + 4)) * sizeof(float) : 0;
@@ -1164,17 +1183,20 @@ bool plan_attention(int64_t total, int64_t batch, int64_t hq, int64_t hkv, int64
 
 template <int D, bool F16>
 int launch_attention(const AttnArgs& a, const AttnPlan& p, hipStream_t stream) {
-  const dim3 grid((unsigned)(p.cap * a.hkv));
-  if (p.rows == 128)
-    hipLaunchKernelGGL((tile_kernel<D, 1, 4, F16>), grid, dim3(256), 0, stream, a);
-  else if (p.rows == 64)
-    hipLaunchKernelGGL((tile_kernel<D, 1, 2, F16>), grid, dim3(128), 0, stream, a);
-  else if (p.rows == 32)
-    hipLaunchKernelGGL((stream_kernel<D, D == 256 ? 1 : 2, F16>), grid, dim3(kThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL((stream_kernel<D, 1, F16>), grid, dim3(kThreads), 0, stream, a);
-  AKLR_LAUNCH_CHECK();
-  return AKLR_OK;
+  const auto go = [&](auto kernel, auto rows, int threads) {
+    constexpr int R = decltype(rows)::value;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(p.cap * a.hkv)), dim3(threads), 0, stream, a);
+    AKLR_LAUNCH_CHECK();
+    if (!a.joiners) return AKLR_OK;
+    hipLaunchKernelGGL((join_kernel<D, R, F16>), dim3((unsigned)(p.tiles * a.joiners * a.hkv)), dim3(kThreads), 0, stream, a);
+    AKLR_LAUNCH_CHECK();
+    return AKLR_OK;
+  };
+  if (p.rows == 128) return go(tile_kernel<D, 1, 4, F16>, IC<128>{}, 256);
+  if (p.rows == 64) return go(tile_kernel<D, 1, 2, F16>, IC<64>{}, 128);
+  if constexpr (D < 256)
+    if (p.rows == 32) return go(stream_kernel<D, 2, F16>, IC<32>{}, kThreads);
+  return go(stream_kernel<D, 1, F16>, IC<16>{}, kThreads);
 }
 
 bool attention_shape_ok(int64_t total, int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t capacity) {
@@ -1260,6 +1282,7 @@ extern "C" int aklr_tree_attention_fp8(const void* q, int64_t q_token, int64_t q
   a.slots = (int)p.slots;
   a.cap = (int)p.cap;
   a.words = (int)p.tiles;
+  a.joiners = (int)p.joiners;
   a.scale_log2 = softmax_scale * 1.44269504f;
   a.dim = (int)head_dim;
   const auto go = [&](auto d) {
