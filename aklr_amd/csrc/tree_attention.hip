@@ -130,6 +130,7 @@ __device__ __forceinline__ Item find(const AttnArgs& a, int index) {
       r.row_tile = tiles_before + take(tiles) - r.tiles;
       r.split = TILE ? 0 : (index - r.slot) / r.tiles;
       r.tile = TILE ? index - r.row_tile : index - r.slot - r.split * r.tiles;
+      r.tile = r.tiles - 1 - r.tile;  // the last first: under causal masks it sees the most
       r.slot += r.tile;
       r.row_tile += r.tile;
       r.q0 = take(s.q0);
@@ -801,6 +802,48 @@ __device__ __forceinline__ f32x16 mfma16(const u32x4& a, const u32x4& b, const f
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// Codes against a piece of a query, whose values are 2^DOWN times too large.
+template <int DOWN>
+__device__ __forceinline__ f32x16 mfma64(const i32x8& k, const i32x8& q, const f32x16& c) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q, c, 0, 0, 0, 127, 0, 127 - DOWN);
+}
+
+// A row's bf16 query, half of it in each of two lanes 32 apart, as two e4m3 pieces of its values times a power of two that
+// brings the largest to [128, 256). The first keeps 4 of a value's 8 bits, the second, 2^kPiece times what is left, the
+// other 4. A value below 2^-13 of the row's largest loses some of them: at most 2^-22 of the largest. Returns what
+// takes the power back. An infinity makes the row NaN, as it would its scores.
+constexpr int kPiece = 5;
+template <int N>
+__device__ __forceinline__ float in_pieces(const u32x4 (&w)[4 * N], i32x8 (&hi)[N], i32x8 (&lo)[N]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int s = 0; s < 4 * N; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = max(top, max(w[s][i] << 16 & 0x7FFF0000u, w[s][i] & 0x7FFF0000u));
+  top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+  const int power = top == 0 ? 0 : 8 - __builtin_amdgcn_frexp_expf(__uint_as_float(top));
+  const bool bad = top >= 0x7F800000u;
+#pragma unroll
+  for (int s = 0; s < 4 * N; ++s) {
+    float v[8], rest[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = ldexpf(bf16_lo(w[s][i]), power);
+      v[2 * i + 1] = ldexpf(bf16_hi(w[s][i]), power);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t word = pack4_e4m3(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)word, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)word, true);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) rest[4 * i + j] = ldexpf(v[4 * i + j] - (j < 2 ? a[j] : b[j - 2]), kPiece);
+      hi[s / 4][2 * (s % 4) + i] = (int)(bad ? 0x7F7F7F7Fu : word);
+      lo[s / 4][2 * (s % 4) + i] = (int)pack4_e4m3(rest[4 * i], rest[4 * i + 1], rest[4 * i + 2], rest[4 * i + 3]);
+    }
+  }
+  return ldexpf(1.0f, -power);
+}
+
 // Many rows: the W waves of a workgroup take 32 rows each and share a ring of S stages of 64 tokens' codes in LDS, which
 // come straight from memory, 16 tokens a load. One barrier a stage: a wave waits for its own loads, the barrier for the
 // others', and behind it the stage before is free for the loads S - 1 stages ahead.
@@ -810,33 +853,41 @@ __device__ __forceinline__ f32x16 mfma16(const u32x4& a, const u32x4& b, const f
 // multiply-adds take 26 cycles there, one of 32 x 32 and four of them 31). Conversions and exponentials are as much work
 // here as the products, so that is worth more than the smaller tiles' fit. Row c of the lane's half of the wave, hf, and
 // tokens 8b + 4hf + 0..3 of each 32 in the four accumulator groups b: again what the second product wants.
-template <int D, int NQ, int W, bool F16>
-__global__ __launch_bounds__(64 * W, D * NQ > 128 ? 1 : 2) void tile_kernel(const AttnArgs a) {
-  constexpr int RW = 32 * NQ, R = RW * W, QS = D / 16, DT = D / 32, C = D / 16, KL = D / 32, ND = D / 64;
+template <int D, int W, bool F16>
+__global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void tile_kernel(const AttnArgs a) {
+  constexpr int R = 32 * W, QS = D / 16, DT = D / 32, C = D / 16, KL = D / 32, ND = D / 64;
   constexpr int kStep = 64, S = 3, kStage = 2 * kStep * D + 8 * kStep, kBlocks = 4 / W;  // blocks of 16 a wave loads
   const int head = blockIdx.x % a.hkv, index = blockIdx.x / a.hkv;
   const Item it = find<R>(a, index);
   if (!it.ok) return;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), c = lane & 31, hf = lane >> 5;
-  const int rows = it.count * a.group, r0 = it.tile * R, rw = r0 + RW * wave, ctx = it.len - it.count;
+  const int rows = it.count * a.group, r0 = it.tile * R, rw = r0 + 32 * wave, ctx = it.len - it.count;
   const int last_t = (min(r0 + R, rows) - 1) / a.group;
   const int visible = a.mask ? it.len : min(it.len, ctx + last_t + 1);
   const int from = it.split * it.chunk * kUnit;  // below len
   const int end = (int)min((int64_t)visible, from + (int64_t)it.chunk * kUnit);
   // the wave's own rows: positions some of them see, and those all of them see
-  const int own = rw >= rows ? 0 : a.mask ? end : min(end, ctx + (min(rw + RW, rows) - 1) / a.group + 1);
+  const int own = rw >= rows ? 0 : a.mask ? end : min(end, ctx + (min(rw + 32, rows) - 1) / a.group + 1);
   const int clear = min(end, ctx + (a.mask ? 0 : rw / a.group + 1));
 
-  u32x4 q[NQ][QS];
-  int row_t[NQ];
+  // The row's query: fp16 as it is, bf16 in two e4m3 pieces, then against the codes themselves.
+  constexpr bool kPieces = !F16 && D < 256;
+  u32x4 q[kPieces ? 1 : QS];
+  i32x8 q_hi[kPieces ? D / 64 : 1], q_lo[kPieces ? D / 64 : 1];
+  float row_scale = a.scale_log2;
+  const int row_t = min(rw + c, rows - 1) / a.group;
+  {
+    const int h = min(rw + c, rows - 1) - row_t * a.group;
+    const uint16_t* p = static_cast<const uint16_t*>(a.q) + (it.q0 + row_t) * a.q_token + (head * a.group + h) * a.q_head + (D / 2) * hf;
+    u32x4 w[QS];
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int row = min(rw + 32 * n + c, rows - 1), t = row / a.group;
-    row_t[n] = t;
-    const uint16_t* p = static_cast<const uint16_t*>(a.q) + (it.q0 + t) * a.q_token + (head * a.group + row - t * a.group) * a.q_head +
-                        (D / 2) * hf;
+    for (int s = 0; s < QS; ++s) w[s] = ld16(p + 8 * s);
+    if constexpr (kPieces) {
+      row_scale *= in_pieces<D / 64>(w, q_hi, q_lo);
+    } else {
 #pragma unroll
-    for (int s = 0; s < QS; ++s) q[n][s] = ld16(p + 8 * s);
+      for (int s = 0; s < QS; ++s) q[s] = w[s];
+    }
   }
 
   // [keys of 64 tokens][values][key scales][value scales]. Piece u of key row r lies at u ^ (r * C / 16), value row t at
@@ -901,17 +952,14 @@ __global__ __launch_bounds__(64 * W, D * NQ > 128 ? 1 : 2) void tile_kernel(cons
     }
   };
 
-  f32x16 o[NQ][DT], x[NQ];
-  float m[NQ], l[NQ], limit[NQ];
+  f32x16 o[DT], x;
+  float m, l, limit;
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
+  for (int i = 0; i < DT; ++i)
 #pragma unroll
-    for (int i = 0; i < DT; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[n][i][r] = 0.0f;
-    m[n] = l[n] = 0.0f;
-    limit[n] = -__builtin_inff();
-  }
+    for (int r = 0; r < 16; ++r) o[i][r] = 0.0f;
+  m = l = 0.0f;
+  limit = -__builtin_inff();
 
   auto across = [](float v, auto f) {  // over the two halves that share a row
     const uint32_t u = __float_as_uint(v);
@@ -951,70 +999,64 @@ __global__ __launch_bounds__(64 * W, D * NQ > 128 ? 1 : 2) void tile_kernel(cons
     __builtin_amdgcn_sched_barrier(0);  // all of it on its way before the first use waits
     return t;
   };
-  uint32_t sees[NQ] = {};
+  uint32_t sees = 0;
   auto scores = [&](const Read& t, bool edge) {
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
+    for (int r = 0; r < 16; ++r) x[r] = 0.0f;
+    if constexpr (kPieces) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) x[n][r] = 0.0f;
+      for (int i = 0; i < D / 64; ++i) {
+        const i32x8 k = cat(t.k[2 * i], t.k[2 * i + 1]);
+        x = mfma64<0>(k, q_hi[i], x);
+        x = mfma64<kPiece>(k, q_lo[i], x);
+      }
+    } else {
 #pragma unroll
-    for (int i = 0; i < KL; ++i) {
-      const u32x4 w = t.k[i];
+      for (int i = 0; i < KL; ++i) {
+        const u32x4 w = t.k[i];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const u32x4 k = {two<F16, false>(w[2 * e]), two<F16, true>(w[2 * e]), two<F16, false>(w[2 * e + 1]), two<F16, true>(w[2 * e + 1])};
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) x[n] = mfma16<F16>(k, q[n][2 * i + e], x[n]);
+        for (int e = 0; e < 2; ++e) {
+          const u32x4 k = {two<F16, false>(w[2 * e]), two<F16, true>(w[2 * e]), two<F16, false>(w[2 * e + 1]), two<F16, true>(w[2 * e + 1])};
+          x = mfma16<F16>(k, q[2 * i + e], x);
+        }
       }
     }
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      const f32x4 s = t.ks[b] * a.scale_log2;
+      const f32x4 s = t.ks[b] * row_scale;
 #pragma unroll
-      for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[n][4 * b + i] = fmaf(x[n][4 * b + i], s[i], -m[n]);
+      for (int i = 0; i < 4; ++i) x[4 * b + i] = fmaf(x[4 * b + i], s[i], -m);
     }
     if (edge) {
 #pragma unroll
-      for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x[n][r] = masked(x[n][r], sees[n], r);
+      for (int r = 0; r < 16; ++r) x[r] = masked(x[r], sees, r);
     }
-    bool rises = false;
+    float top = -__builtin_inff();
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      float top = -__builtin_inff();
-#pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, x[n][r]);
-      rises |= top > limit[n];
-    }
-    return __ballot(rises) != 0;
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, x[r]);
+    return __ballot(top > limit) != 0;
   };
   auto rise = [&] {
+    float top = x[0];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      float top = x[n][0];
-#pragma unroll
-      for (int r = 1; r < 16; ++r) top = fmaxf(top, x[n][r]);
-      top = across(top, [](float u, float v) { return fmaxf(u, v); });
-      const bool first = limit[n] != Range<F16>::kRise;
-      if (top > (first ? -__builtin_inff() : 0.0f)) {
-        top += Range<F16>::kHead;
-        limit[n] = Range<F16>::kRise;
-      } else {
-        top = 0.0f;
-      }
-      const float by = first ? 1.0f : __builtin_amdgcn_exp2f(-top);
-      m[n] += top;
-      l[n] *= by;
-#pragma unroll
-      for (int i = 0; i < DT; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[n][i][r] *= by;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[n][r] -= top;
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
+    top = across(top, [](float u, float v) { return fmaxf(u, v); });
+    const bool first = limit != Range<F16>::kRise;
+    if (top > (first ? -__builtin_inff() : 0.0f)) {
+      top += Range<F16>::kHead;
+      limit = Range<F16>::kRise;
+    } else {
+      top = 0.0f;
     }
+    const float by = first ? 1.0f : __builtin_amdgcn_exp2f(-top);
+    m += top;
+    l *= by;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[i][r] *= by;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] -= top;
   };
   auto sums = [&](Read& t, bool edge) {
 #pragma unroll
@@ -1026,23 +1068,20 @@ __global__ __launch_bounds__(64 * W, D * NQ > 128 ? 1 : 2) void tile_kernel(cons
 #pragma unroll
         for (int i = 0; i < 8; ++i) s[i / 4][i % 4] = split_scale(s[i / 4][i % 4], power[i / 4][i % 4]);
       }
-      u32x4 pt[NQ];
+      u32x4 pt;
+      float w[8];
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        float w[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float e = __builtin_amdgcn_exp2f(x[n][8 * kk + i]);
-          l[n] += e;
-          w[i] = e * s[i / 4][i % 4];
-        }
-        if (edge) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = masked_weight(w[i], sees[n], 8 * kk + i);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) pt[n][i] = pack_out2(w[2 * i], w[2 * i + 1], F16 ? AKLR_OUT_F16 : AKLR_OUT_BF16);
+      for (int i = 0; i < 8; ++i) {
+        const float e = __builtin_amdgcn_exp2f(x[8 * kk + i]);
+        l += e;
+        w[i] = e * s[i / 4][i % 4];
       }
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = masked_weight(w[i], sees, 8 * kk + i);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pt[i] = pack_out2(w[2 * i], w[2 * i + 1], F16 ? AKLR_OUT_F16 : AKLR_OUT_BF16);
       constexpr int E = VB == 2 ? 2 : 4;  // dimensions of a word
 #pragma unroll
       for (int y = 0; y < VN; ++y) {
@@ -1056,9 +1095,7 @@ __global__ __launch_bounds__(64 * W, D * NQ > 128 ? 1 : 2) void tile_kernel(cons
         }
 #pragma unroll
         for (int e = 0; e < E; ++e)
-#pragma unroll
-          for (int n = 0; n < NQ; ++n)
-            o[n][E * y + e] = mfma16<F16>(u32x4{y4[0][e][0], y4[0][e][1], y4[1][e][0], y4[1][e][1]}, pt[n], o[n][E * y + e]);
+          o[E * y + e] = mfma16<F16>(u32x4{y4[0][e][0], y4[0][e][1], y4[1][e][0], y4[1][e][1]}, pt, o[E * y + e]);
       }
     }
   };
@@ -1100,8 +1137,7 @@ __global__ __launch_bounds__(64 * W, D * NQ > 128 ? 1 : 2) void tile_kernel(cons
     const bool edge = !lifts;
     if (edge) {
       const uint32_t held = held_by<16, 8>(4 * hf, end - p, pages[2 * half] != 0, pages[2 * half + 1] != 0);
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) sees[n] = seen_by<16, 8>(a, held, p + 4 * hf - ctx, row_t[n], it.q0);
+      sees = seen_by<16, 8>(a, held, p + 4 * hf - ctx, row_t, it.q0);
       clean<16, 32, VN>(&t.v[0][0], t.vs, held);
       lifts = scores(t, true);
     }
@@ -1114,29 +1150,26 @@ __global__ __launch_bounds__(64 * W, D * NQ > 128 ? 1 : 2) void tile_kernel(cons
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing is on its way into the ring any more
 
   const rsrc_t to = slot_at<D, R>(a, head, it.slot + it.split * it.tiles);
+  l = across(l, [](float u, float v) { return u + v; });
+  if (limit != Range<F16>::kRise) m = kNone;
+  const int row = rw + c;
+  if (row < rows) {  // DT consecutive dimensions of it for each of the accumulators' 16 rows
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    l[n] = across(l[n], [](float u, float v) { return u + v; });
-    if (limit[n] != Range<F16>::kRise) m[n] = kNone;
-    const int row = rw + 32 * n + c;
-    if (row < rows) {  // DT consecutive dimensions of it for each of the accumulators' 16 rows
+    for (int r = 0; r < 16; r += (DT < 4 ? 2 : 1)) {
+      const int d = DT * (8 * (r / 4) + 4 * hf + r % 4);
+      constexpr int N = DT < 4 ? 4 : DT;
+      float v[N];
 #pragma unroll
-      for (int r = 0; r < 16; r += (DT < 4 ? 2 : 1)) {
-        const int d = DT * (8 * (r / 4) + 4 * hf + r % 4);
-        constexpr int N = DT < 4 ? 4 : DT;
-        float v[N];
+      for (int i = 0; i < N; ++i) v[i] = o[i % DT][r + i / DT];
+      if (it.splits > 1) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = o[n][i % DT][r + i / DT];
-        if (it.splits > 1) {
-#pragma unroll
-          for (int i = 0; i < N; i += 4)
-            store_partial4(to, (row - r0) * D + d + i, f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]});
-        } else {
-          finish<N, F16>(a, it, head, row, d, m[n], l[n], v);
-        }
+        for (int i = 0; i < N; i += 4)
+          store_partial4(to, (row - r0) * D + d + i, f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]});
+      } else {
+        finish<N, F16>(a, it, head, row, d, m, l, v);
       }
-      if (it.splits > 1 && hf == 0) store_partial4(to, R * D + 4 * (row - r0), f32x4{m[n], l[n], 0, 0});
     }
+    if (it.splits > 1 && hf == 0) store_partial4(to, R * D + 4 * (row - r0), f32x4{m, l, 0, 0});
   }
 }
 
@@ -1192,8 +1225,8 @@ int launch_attention(const AttnArgs& a, const AttnPlan& p, hipStream_t stream) {
     AKLR_LAUNCH_CHECK();
     return AKLR_OK;
   };
-  if (p.rows == 128) return go(tile_kernel<D, 1, 4, F16>, IC<128>{}, 256);
-  if (p.rows == 64) return go(tile_kernel<D, 1, 2, F16>, IC<64>{}, 128);
+  if (p.rows == 128) return go(tile_kernel<D, 4, F16>, IC<128>{}, 256);
+  if (p.rows == 64) return go(tile_kernel<D, 2, F16>, IC<64>{}, 128);
   if constexpr (D < 256)
     if (p.rows == 32) return go(stream_kernel<D, 2, F16>, IC<32>{}, kThreads);
   return go(stream_kernel<D, 1, F16>, IC<16>{}, kThreads);
