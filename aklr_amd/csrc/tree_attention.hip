@@ -856,7 +856,7 @@ __device__ __forceinline__ float in_pieces(const u32x4 (&w)[4 * N], i32x8 (&hi)[
 template <int D, int W, bool F16>
 __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void tile_kernel(const AttnArgs a) {
   constexpr int R = 32 * W, QS = D / 16, DT = D / 32, C = D / 16, KL = D / 32, ND = D / 64;
-  constexpr int kStep = 64, S = 3, kStage = 2 * kStep * D + 8 * kStep, kBlocks = 4 / W;  // blocks of 16 a wave loads
+  constexpr int kStep = 64, S = W == 2 ? 2 : 3, kStage = 2 * kStep * D + 8 * kStep, kBlocks = 4 / W;  // blocks of 16 a wave loads
   const int head = blockIdx.x % a.hkv, index = blockIdx.x / a.hkv;
   const Item it = find<R>(a, index);
   if (!it.ok) return;
@@ -1082,6 +1082,7 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void tile_kernel(const Att
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) pt[i] = pack_out2(w[2 * i], w[2 * i + 1], F16 ? AKLR_OUT_F16 : AKLR_OUT_BF16);
+      if (kk == 0) __builtin_amdgcn_s_setprio(1);
       constexpr int E = VB == 2 ? 2 : 4;  // dimensions of a word
 #pragma unroll
       for (int y = 0; y < VN; ++y) {
@@ -1124,6 +1125,7 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void tile_kernel(const Att
       if (p < own) {
         if (p + 32 > clear || !uniform(half ? pages[2] & pages[3] : pages[0] & pages[1])) break;
         Read t = read(codes, scale);
+        __builtin_amdgcn_s_setprio(0);
         lifts = scores(t, false);
         if (lifts) break;
         sums(t, false);
@@ -1183,7 +1185,7 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void tile_kernel(const Att
 // 8 kv heads of 4: 14.0 us joined by the last, 16.4 apart), and the last workgroup alone is bound by how long its loads
 // take (one sequence of 16000: 23.8 and 20.8; of 2000 with 16 rows of one kv head 14.3 and 11.8, of 16000 61.8 and 24.1;
 // 64 rows of each of 8 kv heads 165 and 37).
-constexpr int kSlots = 512, kTarget = 768, kJoinGroups = 2048, kApart = 240;
+constexpr int kCus = 256, kJoinGroups = 2048, kApart = 240;
 constexpr int kMostSplits = 254;  // an arrival word counts to 255
 
 struct AttnPlan {
@@ -1196,8 +1198,9 @@ struct AttnPlan {
 bool plan_attention(int64_t total, int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t capacity, AttnPlan* p) {
   const int64_t group = hq / hkv, rows = (total * group + batch - 1) / batch;  // of a sequence, on the mean
   p->rows = rows > 64 ? 128 : rows > 32 ? 64 : rows > 16 && d < 256 ? 32 : 16;
-  p->target = (kTarget + hkv - 1) / hkv < kMostSplits ? (kTarget + hkv - 1) / hkv : kMostSplits;
-  p->slots = (kSlots + hkv - 1) / hkv < kMostSplits ? (kSlots + hkv - 1) / hkv : kMostSplits;
+  const int64_t slots = kCus * (p->rows == 64 ? 4 : 2) / (d == 256 ? 2 : 1), target = slots * 3 / 2;
+  p->target = (target + hkv - 1) / hkv < kMostSplits ? (target + hkv - 1) / hkv : kMostSplits;
+  p->slots = (slots + hkv - 1) / hkv < kMostSplits ? (slots + hkv - 1) / hkv : kMostSplits;
   p->tiles = total * group / p->rows + (batch < total ? batch : total);
   const int64_t units = (capacity + kUnit - 1) / kUnit;
   p->cap = p->tiles + (units > 1 ? p->target : 0);
