@@ -1117,7 +1117,6 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void tile_kernel(const Att
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * kLoads) : "memory");
         stage_barrier();
         issue(slot == 0 ? S - 1 : slot - 1, p + (S - 1) * kStep, next);  // into the stage before this one
-        next = look(p + S * kStep);
         pages = *reinterpret_cast<const i32x4*>(here[slot]);
       }
       codes = ring[slot] + 32 * D * half;
@@ -1127,8 +1126,11 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void tile_kernel(const Att
         Read t = read(codes, scale);
         __builtin_amdgcn_s_setprio(0);
         lifts = scores(t, false);
+        if (half == 0) next = look(p + S * kStep);
         if (lifts) break;
         sums(t, false);
+      } else if (half == 0) {
+        next = look(p + S * kStep);
       }
       p += 32;
       slot = half == 0 ? slot : slot + 1 == S ? 0 : slot + 1;
@@ -1142,6 +1144,7 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void tile_kernel(const Att
       sees = seen_by<16, 8>(a, held, p + 4 * hf - ctx, row_t, it.q0);
       clean<16, 32, VN>(&t.v[0][0], t.vs, held);
       lifts = scores(t, true);
+      if (half == 0) next = look(p + S * kStep);
     }
     if (lifts) rise();
     sums(t, edge);
