@@ -802,48 +802,6 @@ __device__ __forceinline__ f32x16 mfma16(const u32x4& a, const u32x4& b, const f
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Codes against a piece of a query, whose values are 2^DOWN times too large.
-template <int DOWN>
-__device__ __forceinline__ f32x16 mfma64(const i32x8& k, const i32x8& q, const f32x16& c) {
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q, c, 0, 0, 0, 127, 0, 127 - DOWN);
-}
-
-// A row's bf16 query, half of it in each of two lanes 32 apart, as two e4m3 pieces of its values times a power of two that
-// brings the largest to [128, 256). The first keeps 4 of a value's 8 bits, the second, 2^kPiece times what is left, the
-// other 4. A value below 2^-13 of the row's largest loses some of them: at most 2^-22 of the largest. Returns what
-// takes the power back. An infinity makes the row NaN, as it would its scores.
-constexpr int kPiece = 5;
-template <int N>
-__device__ __forceinline__ float in_pieces(const u32x4 (&w)[4 * N], i32x8 (&hi)[N], i32x8 (&lo)[N]) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int s = 0; s < 4 * N; ++s)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, max(w[s][i] << 16 & 0x7FFF0000u, w[s][i] & 0x7FFF0000u));
-  top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-  const int power = top == 0 ? 0 : 8 - __builtin_amdgcn_frexp_expf(__uint_as_float(top));
-  const bool bad = top >= 0x7F800000u;
-#pragma unroll
-  for (int s = 0; s < 4 * N; ++s) {
-    float v[8], rest[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = ldexpf(bf16_lo(w[s][i]), power);
-      v[2 * i + 1] = ldexpf(bf16_hi(w[s][i]), power);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t word = pack4_e4m3(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-      const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)word, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)word, true);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) rest[4 * i + j] = ldexpf(v[4 * i + j] - (j < 2 ? a[j] : b[j - 2]), kPiece);
-      hi[s / 4][2 * (s % 4) + i] = (int)(bad ? 0x7F7F7F7Fu : word);
-      lo[s / 4][2 * (s % 4) + i] = (int)pack4_e4m3(rest[4 * i], rest[4 * i + 1], rest[4 * i + 2], rest[4 * i + 3]);
-    }
-  }
-  return ldexpf(1.0f, -power);
-}
-
 // Many rows: the W waves of a workgroup take 32 rows each and share a ring of S stages of 64 tokens' codes in LDS, which
 // come straight from memory, 16 tokens a load. One barrier a stage: a wave waits for its own loads, the barrier for the
 // others', and behind it the stage before is free for the loads S - 1 stages ahead.
@@ -870,24 +828,13 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void tile_kernel(const Att
   const int own = rw >= rows ? 0 : a.mask ? end : min(end, ctx + (min(rw + 32, rows) - 1) / a.group + 1);
   const int clear = min(end, ctx + (a.mask ? 0 : rw / a.group + 1));
 
-  // The row's query: fp16 as it is, bf16 in two e4m3 pieces, then against the codes themselves.
-  constexpr bool kPieces = !F16 && D < 256;
-  u32x4 q[kPieces ? 1 : QS];
-  i32x8 q_hi[kPieces ? D / 64 : 1], q_lo[kPieces ? D / 64 : 1];
-  float row_scale = a.scale_log2;
+  u32x4 q[QS];
   const int row_t = min(rw + c, rows - 1) / a.group;
   {
     const int h = min(rw + c, rows - 1) - row_t * a.group;
     const uint16_t* p = static_cast<const uint16_t*>(a.q) + (it.q0 + row_t) * a.q_token + (head * a.group + h) * a.q_head + (D / 2) * hf;
-    u32x4 w[QS];
 #pragma unroll
-    for (int s = 0; s < QS; ++s) w[s] = ld16(p + 8 * s);
-    if constexpr (kPieces) {
-      row_scale *= in_pieces<D / 64>(w, q_hi, q_lo);
-    } else {
-#pragma unroll
-      for (int s = 0; s < QS; ++s) q[s] = w[s];
-    }
+    for (int s = 0; s < QS; ++s) q[s] = ld16(p + 8 * s);
   }
 
   // [keys of 64 tokens][values][key scales][value scales]. Piece u of key row r lies at u ^ (r * C / 16), value row t at
@@ -1003,27 +950,18 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void tile_kernel(const Att
   auto scores = [&](const Read& t, bool edge) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] = 0.0f;
-    if constexpr (kPieces) {
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i) {
-        const i32x8 k = cat(t.k[2 * i], t.k[2 * i + 1]);
-        x = mfma64<0>(k, q_hi[i], x);
-        x = mfma64<kPiece>(k, q_lo[i], x);
-      }
-    } else {
+    for (int i = 0; i < KL; ++i) {
+      const u32x4 w = t.k[i];
 #pragma unroll
-      for (int i = 0; i < KL; ++i) {
-        const u32x4 w = t.k[i];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const u32x4 k = {two<F16, false>(w[2 * e]), two<F16, true>(w[2 * e]), two<F16, false>(w[2 * e + 1]), two<F16, true>(w[2 * e + 1])};
-          x = mfma16<F16>(k, q[2 * i + e], x);
-        }
+      for (int e = 0; e < 2; ++e) {
+        const u32x4 k = {two<F16, false>(w[2 * e]), two<F16, true>(w[2 * e]), two<F16, false>(w[2 * e + 1]), two<F16, true>(w[2 * e + 1])};
+        x = mfma16<F16>(k, q[2 * i + e], x);
       }
     }
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      const f32x4 s = t.ks[b] * row_scale;
+      const f32x4 s = t.ks[b] * a.scale_log2;
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[4 * b + i] = fmaf(x[4 * b + i], s[i], -m);
     }

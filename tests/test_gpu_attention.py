@@ -309,3 +309,44 @@ def test_offsets_past_32_bits():
                   else t.view(torch.uint8)[torch.tensor([pages - 1, 16384], device=DEV)].view(t.dtype) for t in cache)
     want = aklr_amd.tree_attention_fp8(q, *small, i32([[0, 0], [0, 1]]), i32([1000, 1324]), i32([0, 1, 2]))
     assert torch.equal(out, want) and out.float().abs().max() > 0.01
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("t", [3, 30, 50, 100])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_score_is_an_fp32_sum(t, d, dtype):
+    # Every token sees one position, itself, so the log of its sum is its score. The products are exact, d of them are
+    # summed with a rounding of at most 2^-24 of their size each, and three scalings round as much. With the score x in
+    # powers of two the reference is at most |x| + 20: four roundings of that size around the exponential, and the
+    # logarithm of a weight between 2^-20 and 2^20: under 2^-24 * (4 |x| + 128) together.
+    say(f"scores {t} {d} {dtype}")
+    p = problem([t], [t], 2, 1, d, 16, dtype, seed=7, mask=lambda rng, n: np.eye(n, dtype=bool))
+    out, lse = call(p, return_lse=True)
+    _, want, _, size = oc.attention(
+        p["q"].double().cpu().numpy(), u8(p["cache"][0]), u8(p["cache"][1]), *(x.cpu().numpy() for x in p["cache"][2:]),
+        p["table"].cpu().numpy(), p["lens"].cpu().numpy(), p["starts"].cpu().numpy(), p["mask"].cpu().numpy(), d ** -0.5)
+    tol = 2**-24 * ((d + 3) * size + 4 * np.abs(want) / np.log(2) + 128)
+    far = np.abs(lse.double().cpu().numpy() - want) - tol
+    assert (far <= 0).all(), far.max()
+    # and its value, whatever the weight: quotient and type round, and the weight: once to fp16 (2^-11) or bf16 (2^-8);
+    # up to 16 rows a bf16 one is two, and what the first leaves, at most 2^-8, is off by 2^-8 of that
+    at = p["table"][0].long()
+    v = (p["cache"][1].double() * p["cache"][3].double()[..., None])[at].transpose(1, 2).reshape(-1, 2, d)[:t]
+    few = 2**-11 if dtype == F16 else 2**-16 if t <= 16 else 2**-8
+    assert ((out.double() - v).abs() <= v.abs() * (torch.finfo(dtype).eps / 2 + few) * 1.01 + 2**-25).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lens,counts,h,group,d,page", [
+    ([9000], [1], 1, 16, 128, 16), ([9000], [1], 8, 1, 64, 64), ([9000], [1], 1, 3, 256, 16), ([5000], [33], 2, 4, 128, 32),
+    ([5000, 0, 4000], [5, 3, 9], 1, 8, 64, 16), ([6000, 130, 1], [20, 1, 1], 2, 4, 256, 48), ([7000], [7], 1, 4, 128, 16),
+    ([40 + 90 * i for i in range(70)], [1 + i % 3 for i in range(70)], 1, 5, 128, 16),
+    ([90 * i for i in range(70)], [i % 2 for i in range(70)], 1, 2, 64, 16)])
+def test_many_splits(lens, counts, h, group, d, page, dtype):
+    say(f"splits {lens[:3]} {counts[:3]} {h} {group} {d} {page} {dtype}")
+    p = problem(lens, counts, h, group, d, page, dtype, seed=11)
+    out, lse = call(p, return_lse=True)
+    check(p, out, lse, what="splits")
+    for _ in range(3):  # always in the same order
+        again = call(p, return_lse=True)
+        assert torch.equal(again[0], out) and torch.equal(again[1], lse)
