@@ -12,6 +12,11 @@ softmax_scale=None, return_lse=False, out=None)``:
   sequence has), or without a mask those up to itself: one token a sequence is decode, several a chunk of a prompt or a
   chain of drafts. ``softmax_scale``: head_dim ** -0.5 unless given.
 
+  Keys' pages lie as far apart as values', and their scales' likewise (the cache's own layout, or both in one
+  allocation). A block table reaches 2^28 positions, tokens * q_heads 2^28.
+
+  A position's weight may reach 2^20 before the division, so values past 2^100 can overflow bf16's range.
+
   Returns q's shape and dtype, with ``return_lse`` also the fp32 [tokens, q_heads] log of each softmax's sum, by which
   parts of a context can be joined. A token that sees nothing gets zeros and -inf. Nothing of a position that a token
   does not see reaches it, NaN included. Query tokens behind the last sequence (a padded batch) leave ``out`` as it
@@ -91,14 +96,14 @@ def tree_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_l
     _, kv_heads, page, cache_dim = k_cache.shape
     if head_dim != cache_dim or heads < kv_heads or heads % kv_heads or heads > 65536:
         return _OOC
-    if not vectors_ok(q, tokens, heads, head_dim, q.dtype) or tokens * (heads // kv_heads) >= 2**30:
+    if not vectors_ok(q, tokens, heads, head_dim, q.dtype):
         return _OOC
     if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or not seq_lens.is_contiguous():
         return _OOC
     batch = seq_lens.numel()
     if batch > 65536 or not starts_ok(starts) or starts.numel() != batch + 1 or not table_ok(block_table, batch):
         return _OOC
-    if block_table.shape[1] * page > 2**28:
+    if block_table.shape[1] * page > 2**28 or strides[0] >= 2**32 or strides[2] >= 2**30 or tokens * heads >= 2**28:
         return _OOC
     if tree_mask is not None:
         if tree_mask.dtype not in (torch.bool, torch.uint8) or tree_mask.dim() != 2 or tree_mask.shape[0] != tokens:

@@ -692,11 +692,11 @@ PyObject* tree_attention(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
   const int64_t tokens = q->size(0), heads = q->size(1), dim = q->size(2), batch = lens->numel();
   const auto type = q->scalar_type();
   if ((type != at::kBFloat16 && type != at::kHalf) || dim != c.dim || heads < c.heads || heads % c.heads || heads > 65536 ||
-      tokens < 1 || batch < 1 || !vectors_ok(*q, tokens, heads, dim, type) || tokens * (heads / c.heads) >= (int64_t{1} << 30))
+      tokens < 1 || batch < 1 || !vectors_ok(*q, tokens, heads, dim, type) || tokens * heads >= (int64_t{1} << 28))
     Py_RETURN_NONE;
   if (lens->scalar_type() != at::kInt || lens->dim() != 1 || !lens->is_contiguous() || batch > 65536 || !starts_ok(*starts) ||
       starts->numel() != batch + 1 || !table_ok(*table, batch) || table->size(1) * c.page > (int64_t{1} << 28) ||
-      c.step[0] != c.step[1] || c.step[2] != c.step[3])
+      c.step[0] != c.step[1] || c.step[2] != c.step[3] || c.step[0] >= (int64_t{1} << 32) || c.step[2] >= (int64_t{1} << 30))
     Py_RETURN_NONE;
   if (mask && ((mask->scalar_type() != at::kBool && mask->scalar_type() != at::kByte) || mask->dim() != 2 ||
                mask->size(0) != tokens || (mask->size(1) > 1 && mask->stride(1) != 1)))
@@ -720,7 +720,8 @@ PyObject* tree_attention(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
     if (bytes) ws = make({static_cast<int64_t>(bytes)}, at::kByte, *q);
     const auto ints = [](const Tensor* t) { return static_cast<const int32_t*>(t->const_data_ptr()); };
     st = aklr_tree_attention_fp8(q->const_data_ptr(), q->stride(0), q->stride(1), c.t[0]->const_data_ptr(),
-                                 c.t[1]->const_data_ptr(), c.scales(2), c.scales(3), c.step[0], c.step[2], ints(table), table_stride(*table), table->size(1), ints(lens), ints(starts),
+                                 c.t[1]->const_data_ptr(), c.scales(2), c.scales(3), c.step[0], c.step[2], ints(table),
+                                 table_stride(*table), table->size(1), ints(lens), ints(starts),
                                  at_or_null(mask), mask ? mask->stride(0) : 0, mask ? mask->size(1) : 0, o.mutable_data_ptr(),
                                  with_lse ? static_cast<float*>(l.mutable_data_ptr()) : nullptr, tokens, batch, heads, c.heads,
                                  dim, c.pages, c.page, static_cast<float>(scale), out_code(type),

@@ -11,7 +11,7 @@ AKLR_SCALAR_FP32_BEGIN
 namespace aklr {
 
 constexpr int kThreads = 256;
-constexpr int kManyGroups = 4096, kTokens = 4;
+constexpr int kManyGroups = 4096;
 constexpr int64_t kManyItems = 1 << 20;
 
 // Eight consecutive values of T (bf16 bits, fp16 or fp32) as fp32, and back with one rounding to nearest even.
@@ -108,6 +108,9 @@ struct VecArgs {
 // Quantization (the arithmetic of aklr_per_group_quant_fp8 at one group a head): s = max(amax, 1e-10) * fl32(1/448),
 // code = e4m3(clamp(x * (1/s))). A rotated k goes from fp32 straight into its code. A vector that holds a NaN or an
 // infinity gets zero codes under a NaN scale, so it reads as NaN throughout and no NaN code enters the cache.
+//
+// Bound by memory where there are many tokens (figures at launch_vec), by the launch and one chain of loads where few:
+// 3.2 us for 64 tokens of 8 heads written, 3.4 for 16 tokens of 129 heads rotated, 3.9 for 8 of 80 rotated and written.
 template <typename T, int D, bool ROT, bool WRITE>
 __global__ __launch_bounds__(kThreads) void vec_kernel(const VecArgs a, const int head_dim) {
   const int dim = D ? D : head_dim;
@@ -263,24 +266,20 @@ __global__ __launch_bounds__(kThreads) void vec_kernel(const VecArgs a, const in
 }
 
 // How many tokens a workgroup takes and how many workgroups share them: one item a lane, which is all that a write alone
-// needs (8191 tokens of 8 heads of 256: 22.5 us, with four tokens a workgroup 23.4). With a rotation, where that makes
-// many workgroups, one takes four whole tokens instead, so that the angles are worked out once for all heads and by all
-// of its lanes: 5003 tokens of 32 + 8 heads of 128 in 17.4 us instead of 19.5, rotated and written 8192 of them in 38.5
-// instead of 46.3 (one token a workgroup: 17.6 and 40.6).
+// needs (8191 tokens of 8 heads of 256: 22.5 us, 5.1 TB/s of reads and writes; a large copy reaches 5.2). With a rotation,
+// where that makes many workgroups, one takes all heads of a token, so that its angles are worked out once: 8192 tokens of
+// 32 + 8 heads of 128 rotated and written in 43.9 us instead of 49.9 (two tokens a workgroup 43.0, four 43.9), 5003 rotated
+// in 18.5 instead of 19.7 (two 19.7, four 21.7).
 template <typename T, int D, bool ROT, bool WRITE>
 int launch_vec(VecArgs& a, int head_dim, hipStream_t stream) {
   const int64_t row = (int64_t)((ROT ? a.q.heads : 0) + a.k.heads + (WRITE ? a.v.heads : 0)) * (head_dim / 16);
   if (row == 0 || a.tokens == 0) return AKLR_OK;
   a.per_wg = (int)(row >= kThreads ? 1 : kThreads / row);
-  const int most = ROT ? (2048 / a.rot ? 2048 / a.rot : 1) : 1 << 20;  // angles a workgroup keeps: 8 KiB
-  if (a.per_wg > most) a.per_wg = most;
+  if (ROT && a.per_wg > 2048 / a.rot) a.per_wg = 2048 / a.rot;  // angles a workgroup keeps: 8 KiB
   int64_t gy = (row * a.per_wg + kThreads - 1) / kThreads;
-  if (ROT && (a.tokens + a.per_wg - 1) / a.per_wg * gy > kManyGroups) {
-    while (a.per_wg < kTokens && 2 * a.per_wg <= most) a.per_wg *= 2;
-    gy = 1;
-  }
+  if (ROT && (a.tokens + a.per_wg - 1) / a.per_wg * gy > kManyGroups) gy = 1;
   const int64_t gx = (a.tokens + a.per_wg - 1) / a.per_wg;
-  if (gx > 0x7FFFFFFF || gy > 65535) return AKLR_ERR_INVALID_ARGUMENT;
+  if (gx > 0xFFFFFF || gy > 65535) return AKLR_ERR_INVALID_ARGUMENT;  // a launch has fewer than 2^32 threads
   const size_t lds = ROT ? (size_t)a.per_wg * (a.rot / 2) * sizeof(float2) : 0;
   hipLaunchKernelGGL((vec_kernel<T, D, ROT, WRITE>), dim3((unsigned)gx, (unsigned)gy), dim3(kThreads), lds, stream, a,
                      head_dim);
@@ -290,7 +289,9 @@ int launch_vec(VecArgs& a, int head_dim, hipStream_t stream) {
 
 // ---------------------------------------------------------------------------------------------------------------
 // A packed prefix out of the pages: workgroup x takes `rows` consecutive rows, y keys or values. Rows' places are looked
-// up once a row (a binary search of the sequence, then the block table), then a lane turns 16 codes into 16 values.
+// up once a row (a binary search of the sequence, then the block table), then a lane turns 16 codes into 16 values, two
+// of them where there are many: 188 k rows of 8 heads of 128 in 224 us (5.1 TB/s of codes and values, as a large copy)
+// instead of 240 with one or four items a lane and 266 with eight, 3 x 700 rows of 2 heads of 64 in 3.6 with one.
 struct ReadSide {
   const uint8_t* codes;
   const float* scales;
@@ -488,6 +489,7 @@ extern "C" int aklr_kv_cache_read_fp8(const void* k_codes, const void* v_codes, 
   const int64_t row = kv_heads * head_dim / 16;
   const int64_t fit = (kThreads * (total * row > kManyItems ? 2 : 1) + row - 1) / row;
   const int64_t rows = fit < kReadRows ? fit : kReadRows;
+  if ((total + rows - 1) / rows > 0xFFFFFF) return AKLR_ERR_INVALID_ARGUMENT;  // a launch has fewer than 2^32 threads
   const dim3 grid((unsigned)((total + rows - 1) / rows), 2);
   const auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, k, v, block_table, table_stride, table_cols, starts,

@@ -9,8 +9,8 @@ contiguous. page_size is a multiple of 16, up to 1024; head_dim 64, 128 or 256.
   values (bf16, fp16 or fp32) at ``slots`` (int32 or int64 [tokens]: page * page_size + place in the page; negative
   ones skip their token, as do those past the cache) and returns the four tensors. The arithmetic is
   ``per_group_quant_fp8``'s (aklr/ops/quant/reference.py:9-28) with one group a head. A vector that holds a NaN or an
-  infinity reads as NaN throughout. The slots of one call are distinct: which of two tokens a slot given twice holds
-  is not defined.
+  infinity reads as NaN throughout. The slots of one call are distinct: a slot given twice may end with parts of both
+  tokens.
 - ``rotary_kv_cache_write_fp8(q, k, v, positions, frequencies, k_cache, ..., slots, *, interleaved, magnitude, out)``
   is ``rotary_embedding`` and the write in one launch: it returns the rotated q and stores the rotated k, which is
   rounded only once, to its code.

@@ -188,6 +188,24 @@ def test_attention_forms(anywhere):
                 {"seq_lens": torch.zeros(4, dtype=torch.int32)[::2]}):
         assert serving(**{**a, **bad}) is OOC, bad
     assert isinstance(serving(**attend_args(t=3, hq=6)), KernelInfo)
+    # pages 2^32 bytes of codes or scales apart, keys' and values' not alike, and more rows than a launch has room for
+    pages = a["k_cache"].shape[0]
+    shape = a["k_cache"].shape[1:]
+    n = shape.numel()
+    far = torch.empty((pages - 1) * 2**32 + n, dtype=torch.uint8)
+    wide = torch.as_strided(far, (pages, *shape), (2**32, *a["k_cache"].stride()[1:])).view(torch.float8_e4m3fn)
+    near = torch.as_strided(far, (pages, *shape), (2**32 - 16, *a["k_cache"].stride()[1:])).view(torch.float8_e4m3fn)
+    assert serving(**{**a, "k_cache": wide, "v_cache": wide}) is OOC
+    assert isinstance(serving(**{**a, "k_cache": near, "v_cache": near}), KernelInfo)
+    assert serving(**{**a, "k_cache": near}) is OOC
+    far = far[:(pages - 1) * 2**32 + n // shape[-1] * 4].view(torch.float32)
+    wide = torch.as_strided(far, (pages, *shape[:2]), (2**30, shape[1], 1))
+    assert serving(**{**a, "k_scale": wide, "v_scale": wide}) is OOC
+    assert serving(**{**a, "k_scale": wide}) is OOC
+    q = torch.zeros((1, 1, 64), dtype=BF16)
+    for heads, served in ((2**14, False), (2**14 - shape[0], True)):
+        big = {"q": q.expand(2**14, heads, 64), "seq_lens": a["seq_lens"], "starts": a["starts"]}
+        assert (serving(**{**a, **big}) is OOC) == (not served), heads
 
 
 def test_pieces_of_rows_that_do_not_meet():

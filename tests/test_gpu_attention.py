@@ -350,3 +350,53 @@ def test_many_splits(lens, counts, h, group, d, page, dtype):
     for _ in range(3):  # always in the same order
         again = call(p, return_lse=True)
         assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("counts", [[130, 7], [40, 50], [0, 129], [33, 33]])
+@pytest.mark.parametrize("d,h,page", [(64, 65, 16), (128, 65, 48), (256, 17, 64)])
+def test_tiles_of_many_rows(d, h, page, counts, masked, dtype):
+    say(f"tiles {d} {h} {page} {counts} {masked} {dtype}")
+    lens = [counts[0] + 5, 1400]
+    p = problem(lens, counts, h, 1, d, page, dtype, seed=5, mask=tree if masked else None, extra_q=2)
+    out = torch.full_like(p["q"], 7.0)
+    call(p, out=out)
+    _, lse = call(p, return_lse=True, out=out)
+    check(p, out, lse)
+    assert (out[sum(counts):] == 7).all()
+    clean = out.clone()
+    # nothing that is not seen reaches a row: NaN and infinities behind the lengths, and in pages of no sequence
+    used = torch.zeros(p["cache"][2].shape[0], page, dtype=torch.bool, device=DEV)
+    for b, n in enumerate(lens):
+        at = torch.arange(n, device=DEV)
+        used[p["table"][b].long()[at // page], at % page] = True
+    for c in p["cache"][:2]:
+        c.view(torch.uint8).masked_fill_(~used[:, None, :, None], 0x7F)
+    for c, bad in zip(p["cache"][2:], (float("inf"), float("nan"))):
+        c.masked_fill_(~used[:, None, :], bad)
+    call(p, out=out)
+    assert torch.equal(out, clean)
+    # a query token's own position all NaN: only rows that see it turn NaN
+    t, b = counts[1] // 2, 1
+    pos, first = lens[1] - counts[1] + t, counts[0]
+    p["cache"][0].view(torch.uint8)[p["table"][b, pos // page].long(), :, pos % page, 3] = 0xFF
+    p["cache"][1].view(torch.uint8)[p["table"][b, pos // page].long(), :, pos % page, 5] = 0x7F
+    call(p, out=out)
+    rows = torch.arange(counts[1], device=DEV)
+    sees = p["mask"][first:first + counts[1], t] if masked else rows >= t
+    mine, before = out[first:first + counts[1]], clean[first:first + counts[1]]
+    assert mine[sees].isnan().all() and torch.equal(mine[~sees], before[~sees]) and torch.equal(out[:first], clean[:first])
+    # pages that the cache does not have are as if not there
+    p = problem(lens, counts, h, 1, d, page, dtype, seed=6, mask=tree if masked else None)
+    p["table"][1, 2], p["table"][1, 5] = -1, p["cache"][0].shape[0]
+    check(p, *call(p, return_lse=True))
+
+
+def test_tiles_of_rows_that_see_nothing():
+    say("tiles: rows that see nothing, lengths below the counts")
+    for counts, lens in (([100, 90], [20, 0]), ([40, 44], [44, 3])):
+        p = problem(lens, counts, 65, 1, 64, 16, mask=lambda rng, t: rng.random((t, t)) < 0.02)
+        check(p, *call(p, return_lse=True))
+        p["mask"] = None
+        check(p, *call(p, return_lse=True))
