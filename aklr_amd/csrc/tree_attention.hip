@@ -8,8 +8,10 @@
 //   o = sum (2^(x_p - m) * sv_p) cv_p / l.
 // A scale belongs to a token, so it multiplies a column of the scores and of the weights, never the codes: codes turn
 // into bf16 (fp16 for fp16 queries against keys) exactly, two an instruction, and the products run on matrix units.
-// The weights times sv are rounded to bf16 for that (half a step, at most 2^-8 of each term); scores, maxima, sums and outputs
-// stay in fp32.
+// The weights times sv become bf16 (fp16) for that: bf16 in two pieces, 16 bits, up to 32 rows, where memory is the bound;
+// in one (half a step, at most 2^-8 of each term) in tiles of more, which the products bound; fp16 in one (2^-11). Scores, maxima, sums and outputs
+// stay in fp32. Products of codes with e4m3 pieces of q would need no conversions of keys, but a chain of them sums to
+// 2^-15 of its size on this hardware (bf16 and fp16 products to 2^-23), which a log of a sum shows.
 #include "common.h"
 
 AKLR_SCALAR_FP32_BEGIN
@@ -18,17 +20,16 @@ namespace aklr {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4, kThreads = 256;
 constexpr int kUnit = 128;  // tokens a workgroup takes in one step: 32 a wave
 // Weights are 2^(x - m) for a reference m that is set kHead above the largest score so far and set again once a score
 // is kRise above it. Floating-point sums lose nothing by that, and a row's reference rises at most every kHead + kRise
 // powers of two: once for all where no score is 2^40 times the first ones'. Weights below 2^20 leave bf16 values to 2^100;
-// fp16 weights have 2^-14 to 2^15, so their range is kept narrower.
+// fp16 weights have all their bits from 2^-14 to 2^15, so theirs start at 1 and may rise to 2^14.
 template <bool F16>
 struct Range {
-  static constexpr float kHead = F16 ? 6.0f : 20.0f, kRise = F16 ? 14.0f : 20.0f;
+  static constexpr float kHead = F16 ? 0.0f : 20.0f, kRise = F16 ? 14.0f : 20.0f;
 };
 constexpr float kNone = -3e38f;   // the reference in a partial result of a row that saw nothing
 
@@ -323,9 +324,9 @@ __device__ __forceinline__ void lift(f32x4 (&x)[NQ][2], float (&m)[NQ], float (&
   }
 }
 
-// The weights, as the second product's operands. A bf16 keeps 8 bits of one, so what that leaves goes into a second: the
-// sums of values are then as exact as the codes, and where memory is the bound the matrix unit has the time for both
-// (64 sequences of 8193 tokens: 128.1 us with one, 128.6 with two; fp16 weights have 11 bits and stay one).
+// The weights, as the second product's operands. A bf16 keeps 8 bits of one, so what that leaves goes into a
+// second: an output is then as near as its type lets it be, and where memory is the bound the matrix unit has the time for
+// both (64 sequences of up to 8192 tokens, group 8: 128.1 us with one, 128.6 with two). fp16 weights have 11 and stay one.
 template <bool F16, int NQ>
 __device__ __forceinline__ void weigh(const f32x4 (&x)[NQ][2], const f32x4 (&vs)[2], bool edge,
                                       const uint32_t (&sees)[NQ], float (&l)[NQ], u32x4 (&hi)[NQ], u32x4 (&lo)[NQ]) {
@@ -478,6 +479,10 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const AttnArgs a) {
   join<D, R, F16>(a, it, head, first, min(left, first + each), r0, sum[0]);
 }
 
+// Up to 32 rows, or more in tiles of those: bound by memory, and where there is little by one chain of loads and a join.
+// 64 sequences of up to 8192 tokens, 8 kv heads of 128, group 8: 129 us, 5.0 TB/s; 156 with codes loaded into registers.
+// One sequence of 2048, group 4: 11.8 us.
+//
 // Rows by the 16 * NQ, tokens by the 32 of a wave. S^T = K Q^T puts a row in a lane (column c of the
 // accumulator) and tokens 4g..4g+3 of each 16 in lane group g, which is just what the second product wants of its
 // operand P^T, so the weights never move between lanes: O^T = V^T P^T sums over k in any order as long as both
@@ -802,7 +807,12 @@ __device__ __forceinline__ f32x16 mfma16(const u32x4& a, const u32x4& b, const f
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Many rows: the W waves of a workgroup take 32 rows each and share a ring of S stages of 64 tokens' codes in LDS, which
+// Many rows: bound by the vector unit's issue beside the matrix unit's time. A step of 32 rows and tokens is 16 products
+// (512 cycles) and 185 vector instructions, 64 of them conversions; counters show the vector unit half and the matrix unit a
+// third of the time busy, two waves on a SIMD. 2048 tokens of each of two prompts over 8192, 8 kv heads of 128, group 4:
+// 568 us, 870 TFLOP/s; without the raised priority of the second products 30 us more.
+//
+// The W waves of a workgroup take 32 rows each and share a ring of S stages of 64 tokens' codes in LDS, which
 // come straight from memory, 16 tokens a load. One barrier a stage: a wave waits for its own loads, the barrier for the
 // others', and behind it the stage before is free for the loads S - 1 stages ahead.
 //
@@ -1143,7 +1153,7 @@ bool plan_attention(int64_t total, int64_t batch, int64_t hq, int64_t hkv, int64
   // 132 over 8000 48 and 41; 16 of them 98 and 127, two of 8192 rows 114 and 164. 32 rows of 16 sequences in tiles of 64
   // 64.8, of 32 52.9, of 16 56.9; 4 rows of one in 32 50.5, of 16 44.3. Heads of 256 (16 rows beside 128): one of 132
   // over 8000 43 and 56, four 103 and 83, 64 of 33 over 1000 203 and 129.
-  const bool many = rows > 32 && batch * hkv * ((rows + 127) / 128) > (d == 256 ? 32 : 128);
+  const bool many = rows > 32 && batch * hkv * ((rows + 127) / 128) >= (d == 256 ? 64 : 128);
   p->rows = many ? rows > 64 ? 128 : 64 : rows > 16 && d < 256 ? 32 : 16;
   const int64_t slots = kCus * (p->rows == 64 ? 4 : 2) / (d == 256 ? 2 : 1), target = slots * 3 / 2;
   p->target = (target + hkv - 1) / hkv < kMostSplits ? (target + hkv - 1) / hkv : kMostSplits;

@@ -328,7 +328,7 @@ def test_a_score_is_an_fp32_sum(t, d, dtype):
     tol = 2**-24 * ((d + 3) * size + 4 * np.abs(want) / np.log(2) + 128)
     far = np.abs(lse.double().cpu().numpy() - want) - tol
     assert (far <= 0).all(), far.max()
-    # and its value, whatever the weight: quotient and type round, and the weight: once to fp16 (2^-11) or bf16 (2^-8);
+    # and its value, whatever the weight: quotient and type round, and the weight: to fp16 (2^-11) or bf16 (2^-8);
     # up to 16 rows a bf16 one is two, and what the first leaves, at most 2^-8, is off by 2^-8 of that
     at = p["table"][0].long()
     v = (p["cache"][1].double() * p["cache"][3].double()[..., None])[at].transpose(1, 2).reshape(-1, 2, d)[:t]
