@@ -464,7 +464,7 @@ struct Turn {  // what a rotation takes beside its vectors
     frequencies = dense(freq);
     if (!positions || !frequencies || !flag(inter, &interleaved) || !number(mag, &magnitude)) return false;
     if (!index_ok(*positions, tokens) || frequencies->scalar_type() != at::kDouble || frequencies->dim() != 1 ||
-        !frequencies->is_contiguous())
+        !frequencies->is_contiguous() || wants_grad(frequencies))
       return false;
     rot = 2 * frequencies->numel();
     return rot >= 16 && rot <= dim && rot % 16 == 0;
@@ -478,7 +478,7 @@ struct Cache {
   bool read(PyObject* const* o) {
     for (int i = 0; i < 4; ++i)
       if (!(t[i] = plain(o[i])) || t[i]->dim() != (i < 2 ? 4 : 3) || t[i]->device() != t[0]->device() ||
-          t[i]->scalar_type() != (i < 2 ? at::kFloat8_e4m3fn : at::kFloat))
+          t[i]->scalar_type() != (i < 2 ? at::kFloat8_e4m3fn : at::kFloat) || wants_grad(t[i]))
         return false;
     pages = t[0]->size(0), heads = t[0]->size(1), page = t[0]->size(2), dim = t[0]->size(3);
     if ((dim != 64 && dim != 128 && dim != 256) || page < 16 || page > 1024 || page % 16 || heads < 1 || heads > 1024 ||

@@ -70,6 +70,8 @@ def cache_strides(k_cache, v_cache, k_scale, v_scale):
         return None
     if k_scale.shape != k_cache.shape[:3] or v_scale.shape != k_cache.shape[:3]:
         return None
+    if wants_grad(k_cache, v_cache, k_scale, v_scale):
+        return None
     strides = []
     for t, multiple in ((k_cache, 16), (v_cache, 16), (k_scale, 4), (v_scale, 4)):
         s = _page_stride(t)

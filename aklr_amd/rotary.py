@@ -125,7 +125,7 @@ def rotary_ok(positions, frequencies, interleaved, magnitude, tokens, head_dim) 
         return False
     if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (tokens,) or not positions.is_contiguous():
         return False
-    if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous():
+    if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous() or wants_grad(frequencies):
         return False
     rot = 2 * frequencies.numel()
     return 16 <= rot <= head_dim and rot % 16 == 0

@@ -98,7 +98,9 @@ def test_cpu_tensors_and_disabled_ops_are_not_served(op, monkeypatch):
     assert fn(**make()) is FallbackReason.DISABLED
 
 
-@pytest.mark.parametrize("op,name", [("rotary", "q"), ("rotary", "k"), ("write", "k"), ("write", "v"), ("both", "q"), ("attend", "q")])
+@pytest.mark.parametrize("op,name", [("rotary", "q"), ("rotary", "k"), ("write", "k"), ("write", "v"), ("both", "q"), ("attend", "q"),
+                                     ("rotary", "frequencies"), ("both", "frequencies"), ("both", "k"), ("read", "k_scale"),
+                                     ("attend", "v_scale"), ("write", "k_scale")])
 def test_gradients_are_refused_not_lost(anywhere, op, name):
     fn, make = OPS[op]
     args = make()
