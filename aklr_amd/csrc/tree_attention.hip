@@ -489,10 +489,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const AttnArgs a) {
 // operands agree, and lane group g holds its own 4 + 4 tokens' values. The order of the head's dimension is free too: a
 // lane loads head_dim / 16 consecutive codes of each of its tokens (a token's 16 lanes a whole line), turns them over
 // in registers, and ends with head_dim / 4 consecutive outputs of its row.
-constexpr int stages(int d, int nq) { return d == 64 ? 4 : d == 128 && nq == 4 ? 4 : 2; }
-
 template <int D, int NQ, bool F16>
-__global__ __launch_bounds__(kThreads, D * NQ > 384 ? 1 : 2) void stream_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(kThreads, 2) void stream_kernel(const AttnArgs a) {
   constexpr int R = 16 * NQ, VW = D / 64;  // VW: words of a lane's codes of a token
   constexpr int KL = D / 64;               // 16-byte loads of a key row a lane (D = 64: one)
   constexpr int QS = D / 32;               // steps of 32 along the head
@@ -500,7 +498,7 @@ __global__ __launch_bounds__(kThreads, D * NQ > 384 ? 1 : 2) void stream_kernel(
   constexpr int C = D / 16;                // 16-byte pieces of a row of codes
   constexpr int ND = D / 64;               // 1 KiB direct loads of 16 rows
   constexpr int kStage = 2 * 32 * D + 256;  // bytes of 32 tokens: keys, values, their scales
-  constexpr int S = stages(D, NQ);
+  constexpr int S = D == 64 ? 4 : 2;  // what LDS holds for two workgroups (D = 256: one)
   const int head = blockIdx.x % a.hkv;
   const int index = blockIdx.x / a.hkv;
   const Item it = find<R>(a, index);
@@ -1127,9 +1125,11 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void tile_kernel(const Att
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Workgroups a call is cut into. Two run on a CU; where the tiles of rows are at most half of those, all run at once.
-// Where they are more, 768 beside them let short and long ones even out: 64 sequences and 8 kv heads took 142 us with
-// 512, 127 with 768, 136 with 1024 (more partial results), and 144 with 2048.
+// Workgroups a call is cut into: as many as run at once (two a CU, four of two waves, half of that with heads of 256) where
+// the tiles of rows are at most half of those. 16 sequences of 64 rows over 8 k tokens take 94 us in 512 workgroups of two
+// waves and 76 in 1024, one row over 16 k with heads of 256 36 us in 512 and 27 in 256. Where tiles are more, half as many
+// again beside them let short and long ones even out: 64 sequences and 8 kv heads took 142 us with 512, 127 with 768, 136
+// with 1024 (more partial results), and 144 with 2048.
 //
 // Joining: the last workgroup of a tile does it in the same launch where there is little to join, else a kernel of its
 // own with up to a workgroup for four rows. A launch costs 2 us more (one row of each of 16 sequences of 1000 tokens and
