@@ -8,8 +8,8 @@
 //   o = sum (2^(x_p - m) * sv_p) cv_p / l.
 // A scale belongs to a token, so it multiplies a column of the scores and of the weights, never the codes: codes turn
 // into bf16 (fp16 for fp16 queries against keys) exactly, two an instruction, and the products run on matrix units.
-// The weights times sv become bf16 (fp16) for that: bf16 in two pieces, 16 bits, up to 32 rows, where memory is the bound;
-// in one (half a step, at most 2^-8 of each term) in tiles of more, which the products bound; fp16 in one (2^-11). Scores, maxima, sums and outputs
+// The weights times sv become bf16 (fp16) for that: in two pieces up to 32 rows, where memory is the bound, in one (half
+// a step, at most 2^-8 of each term) in tiles of more, which the products bound. Scores, maxima, sums and outputs
 // stay in fp32. Products of codes with e4m3 pieces of q would need no conversions of keys, but a chain of them sums to
 // 2^-15 of its size on this hardware (bf16 and fp16 products to 2^-23), which a log of a sum shows.
 #include "common.h"
@@ -20,6 +20,7 @@ namespace aklr {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4, kThreads = 256;
 constexpr int kUnit = 128;  // tokens a workgroup takes in one step: 32 a wave
@@ -324,9 +325,9 @@ __device__ __forceinline__ void lift(f32x4 (&x)[NQ][2], float (&m)[NQ], float (&
   }
 }
 
-// The weights, as the second product's operands. A bf16 keeps 8 bits of one, so what that leaves goes into a
+// The weights, as the second product's operands. A bf16 keeps 8 bits of one (fp16 11), so what that leaves goes into a
 // second: an output is then as near as its type lets it be, and where memory is the bound the matrix unit has the time for
-// both (64 sequences of up to 8192 tokens, group 8: 128.1 us with one, 128.6 with two). fp16 weights have 11 and stay one.
+// both (64 sequences of up to 8192 tokens, group 8: 128.1 us with one bf16, 128.6 with two).
 template <bool F16, int NQ>
 __device__ __forceinline__ void weigh(const f32x4 (&x)[NQ][2], const f32x4 (&vs)[2], bool edge,
                                       const uint32_t (&sees)[NQ], float (&l)[NQ], u32x4 (&hi)[NQ], u32x4 (&lo)[NQ]) {
@@ -345,8 +346,11 @@ __device__ __forceinline__ void weigh(const f32x4 (&x)[NQ][2], const f32x4 (&vs)
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      hi[n][i] = pack_out2(w[2 * i], w[2 * i + 1], F16 ? AKLR_OUT_F16 : AKLR_OUT_BF16);
-      lo[n][i] = F16 ? 0 : pack_bf16x2(w[2 * i] - bf16_lo(hi[n][i]), w[2 * i + 1] - bf16_hi(hi[n][i]));
+      const uint32_t two = pack_out2(w[2 * i], w[2 * i + 1], F16 ? AKLR_OUT_F16 : AKLR_OUT_BF16);
+      const f16x2 h = __builtin_bit_cast(f16x2, two);
+      const float a = F16 ? (float)h[0] : bf16_lo(two), b = F16 ? (float)h[1] : bf16_hi(two);
+      hi[n][i] = two;
+      lo[n][i] = pack_out2(w[2 * i] - a, w[2 * i + 1] - b, F16 ? AKLR_OUT_F16 : AKLR_OUT_BF16);
     }
   }
 }
@@ -680,7 +684,7 @@ __global__ __launch_bounds__(kThreads, 2) void stream_kernel(const AttnArgs a) {
         for (int n = 0; n < NQ; ++n) {
           const u32x4 v = {lo[e][0], lo[e][1], hi[e][0], hi[e][1]};
           o[n][4 * w + e] = mfma32<F16>(v, w_hi[n], o[n][4 * w + e]);
-          if constexpr (!F16) o[n][4 * w + e] = mfma32<F16>(v, w_lo[n], o[n][4 * w + e]);
+          o[n][4 * w + e] = mfma32<F16>(v, w_lo[n], o[n][4 * w + e]);
         }
     }
   };
