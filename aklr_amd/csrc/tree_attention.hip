@@ -812,7 +812,7 @@ __device__ __forceinline__ f32x16 mfma16(const u32x4& a, const u32x4& b, const f
 // Many rows: bound by the vector unit's issue beside the matrix unit's time. A step of 32 rows and tokens is 16 products
 // (512 cycles) and 185 vector instructions, 64 of them conversions; counters show the vector unit half and the matrix unit a
 // third of the time busy, two waves on a SIMD. 2048 tokens of each of two prompts over 8192, 8 kv heads of 128, group 4:
-// 568 us, 870 TFLOP/s; without the raised priority of the second products 30 us more.
+// 568 to 593 us by the card, 833 to 870 TFLOP/s; without the raised priority of the second products 30 us more.
 //
 // The W waves of a workgroup take 32 rows each and share a ring of S stages of 64 tokens' codes in LDS, which
 // come straight from memory, 16 tokens a load. One barrier a stage: a wave waits for its own loads, the barrier for the
