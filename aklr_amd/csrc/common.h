@@ -62,7 +62,8 @@ typedef __attribute__((address_space(3))) void lds_void;
 // before later LDS reads of other buffers; the caller waits (s_waitcnt vmcnt) and synchronises
 // itself before reading what it loaded. `lds` must be wave-uniform. The statement declares no memory
 // clobber, so loads of read-only kernel inputs after it can still go through the scalar unit;
-// callers order it against LDS reads with barriers.
+// callers order it against LDS reads with barriers. The s_nop is the wait state that the hardware asks for
+// between a write of M0 and its use by a load into LDS; the compiler keeps it for its own loads only.
 __device__ __forceinline__ i32x4 make_rsrc_words(const void* base, uint32_t bytes) {
   const uint64_t a = reinterpret_cast<uint64_t>(base);
   i32x4 r;
@@ -76,23 +77,23 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 __device__ __forceinline__ void lds_dma16(const i32x4& rsrc, uint32_t lds, uint32_t voffset) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voffset), "s"(rsrc)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voffset), "s"(rsrc)
                : "m0");
 }
 __device__ __forceinline__ void lds_dma4(const i32x4& rsrc, uint32_t lds, uint32_t voffset) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(voffset), "s"(rsrc)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(voffset), "s"(rsrc)
                : "m0");
 }
 
 // The same loads with the K advance in soffset: the per-lane voffset stays fixed across a loop, so
 // issuing a stage costs no vector instructions. A descriptor whose byte count is 0 reads zeros.
 __device__ __forceinline__ void lds_dma16_so(const i32x4& rsrc, uint32_t lds, uint32_t voffset, uint32_t soffset) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voffset), "s"(rsrc),
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voffset), "s"(rsrc),
                "s"(soffset)
                : "m0");
 }
 __device__ __forceinline__ void lds_dma4_so(const i32x4& rsrc, uint32_t lds, uint32_t voffset, uint32_t soffset) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(lds), "v"(voffset), "s"(rsrc),
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(lds), "v"(voffset), "s"(rsrc),
                "s"(soffset)
                : "m0");
 }
