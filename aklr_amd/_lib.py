@@ -87,6 +87,7 @@ SIGNATURES: dict[str, tuple] = {
          _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _vp],
     ),
     "aklr_tree_attention_fp8_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64]),
+    "aklr_tree_attention_fp8_rows": (_c_int, [_c_i64] * 6 + [ctypes.POINTER(_c_int)]),
     "aklr_tree_attention_fp8": (
         _c_int,
         [_vp, _c_i64, _c_i64, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64,

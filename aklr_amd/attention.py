@@ -13,7 +13,7 @@ softmax_scale=None, return_lse=False, out=None)``:
   chain of drafts. ``softmax_scale``: head_dim ** -0.5 unless given.
 
   Keys' pages lie as far apart as values', and their scales' likewise (the cache's own layout, or both in one
-  allocation). A block table reaches 2^28 positions, tokens * q_heads 2^28.
+  allocation). A block table reaches 2^28 positions, tokens * q_heads 2^28, sequences times kv_heads about 2^24.
 
   A position's weight may reach 2^20 before the division, so values past 2^100 can overflow bf16's range.
 
@@ -121,5 +121,8 @@ def tree_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_l
             return _OOC
         if not all(apart(out, t) for t in inputs):
             return _OOC
+    if tokens and batch and not _lib.lib().aklr_tree_attention_fp8_rows(
+            tokens, batch, heads, kv_heads, head_dim, block_table.shape[1] * page, None):
+        return _OOC  # more workgroups than a launch has room for
     return _AttentionPlan(q, cache, strides, block_table, seq_lens, starts, tree_mask, float(softmax_scale),
                           bool(return_lse), out, "tree" if tree_mask is not None else "causal")

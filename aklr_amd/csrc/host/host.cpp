@@ -709,6 +709,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
   if (out && (out->sizes() != q->sizes() || out->scalar_type() != type || !out->is_contiguous() || !aligned16(*out) ||
               !c.clear_of(out) || !apart_all(out, {q, table, lens, starts, mask})))
     Py_RETURN_NONE;
+  if (!aklr_tree_attention_fp8_rows(tokens, batch, heads, c.heads, dim, table->size(1) * c.page, nullptr)) Py_RETURN_NONE;
   Tensor o, l, ws;
   int st;
   {

@@ -1215,6 +1215,16 @@ extern "C" size_t aklr_tree_attention_fp8_workspace_bytes(int64_t total_q, int64
   return p.bytes;
 }
 
+extern "C" int aklr_tree_attention_fp8_rows(int64_t total_q, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                            int64_t head_dim, int64_t capacity, int* joiners) {
+  AttnPlan p;
+  if (!attention_shape_ok(total_q, batch, q_heads, kv_heads, head_dim, capacity) || total_q == 0 || batch == 0 ||
+      !plan_attention(total_q, batch, q_heads, kv_heads, head_dim, capacity, &p))
+    return 0;
+  if (joiners) *joiners = (int)p.joiners;
+  return p.rows;
+}
+
 extern "C" int aklr_tree_attention_fp8(const void* q, int64_t q_token, int64_t q_head, const void* k_codes,
                                        const void* v_codes, const float* k_scales, const float* v_scales,
                                        int64_t code_page, int64_t scale_page,

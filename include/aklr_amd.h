@@ -331,6 +331,12 @@ int aklr_kv_cache_read_fp8(const void* k_codes, const void* v_codes, const float
  */
 size_t aklr_tree_attention_fp8_workspace_bytes(int64_t total_q, int64_t batch, int64_t q_heads, int64_t kv_heads,
                                                int64_t head_dim, int64_t capacity);
+/* Rows (query token, query head of a kv head's group) that aklr_tree_attention_fp8 gives a workgroup of such a call: 16
+ * or 32 stream the cache a wave at a time, 64 and 128 share it between waves; 0 where it does not serve the call (invalid
+ * sizes, or more workgroups than a launch has room for). joiners (may be NULL): workgroups of a launch of its own that
+ * join each tile's partial results, 0 where the last of those that wrote them does, or where there are none. */
+int aklr_tree_attention_fp8_rows(int64_t total_q, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                 int64_t capacity, int* joiners);
 int aklr_tree_attention_fp8(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_codes,
                             const void* v_codes, const float* k_scales, const float* v_scales, int64_t code_page,
                             int64_t scale_page, const int32_t* block_table, int64_t table_stride,

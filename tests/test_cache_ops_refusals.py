@@ -1,0 +1,38 @@
+"""Calls of the cache operators that are refused with a reason where they used to raise, or to be served wrongly. The plans
+are asked on CPU tensors in the place of GPU ones."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import aklr_amd
+from aklr_amd.dispatch import FallbackReason, KernelInfo
+from tests.test_cache_ops_host import BF16, OPS, anywhere, attend_args, both_args, cache_args, rot_args, write_args  # noqa: F401
+
+OOC = FallbackReason.OUT_OF_CONTRACT
+
+
+def i32(n):
+    return torch.zeros(n, dtype=torch.int32)
+
+
+def test_more_workgroups_than_a_launch_has_room_for(anywhere, native_lib):
+    # 65536 sequences of one token, 256 kv heads of one query head: 65536 / 16 + 65536 tiles a head, 17.8 million workgroups
+    c = {n: t for n, t in cache_args(h=256).items()}
+    q = torch.zeros((1, 1, 64), dtype=BF16)
+    for batch, served in ((65536, False), (60000, True)):
+        args = {"q": q.expand(batch, 256, 64), **c, "block_table": i32((batch, 1)), "seq_lens": i32(batch),
+                "starts": i32(batch + 1)}
+        assert isinstance(aklr_amd.tree_attention_fp8.serving(**args), KernelInfo) == served
+        assert bool(native_lib.aklr_tree_attention_fp8_rows(batch, batch, 256, 256, 64, 16, None)) == served
+
+
+def test_attention_rows_query(native_lib):
+    rows = native_lib.aklr_tree_attention_fp8_rows
+    join = ctypes.c_int(-1)
+    assert rows(1, 1, 8, 8, 128, 4096, None) == 16 and rows(20, 1, 8, 8, 128, 4096, None) == 32
+    assert rows(4096, 2, 32, 8, 128, 16384, ctypes.byref(join)) == 128 and join.value > 0
+    assert rows(2, 2, 4, 1, 64, 320, ctypes.byref(join)) == 16 and join.value == 0  # the last workgroup joins
+    assert rows(1, 1, 8, 8, 96, 4096, None) == 0 and rows(1, 1, 8, 3, 64, 4096, None) == 0 and rows(0, 1, 8, 8, 64, 4096, None) == 0
