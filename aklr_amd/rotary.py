@@ -188,13 +188,12 @@ def rotary_embedding(q, k, positions, frequencies, *, interleaved=False, magnitu
         return _OOC
     if not on_gpu(*given) or wants_grad(q, k):
         return _OOC
-    inputs = (q, k, positions, frequencies)
-    for out, like in ((out_q, q), (out_k, k)):
+    for out, like, other in ((out_q, q, k), (out_k, k, q)):
         if out is None:
             continue
         if not vectors_ok(out, tokens, like.shape[1], head_dim, q.dtype) or not no_inner_overlap(out):
             return _OOC
-        if not all(apart(out, t) for t in inputs if t is not like) or not (same_place(out, like) or apart(out, like)):
+        if not all(apart(out, t) for t in (other, positions, frequencies)) or not (same_place(out, like) or apart(out, like)):
             return _OOC
     if not apart(out_q, out_k):
         return _OOC

@@ -36,3 +36,15 @@ def test_attention_rows_query(native_lib):
     assert rows(4096, 2, 32, 8, 128, 16384, ctypes.byref(join)) == 128 and join.value > 0
     assert rows(2, 2, 4, 1, 64, 320, ctypes.byref(join)) == 16 and join.value == 0  # the last workgroup joins
     assert rows(1, 1, 8, 8, 96, 4096, None) == 0 and rows(1, 1, 8, 3, 64, 4096, None) == 0 and rows(0, 1, 8, 8, 64, 4096, None) == 0
+
+
+def test_one_tensor_as_queries_and_keys_is_not_rotated_in_place(anywhere):
+    # written in place as q while it is read as k, the keys would be rotated once or twice, as the workgroups come
+    serving = aklr_amd.rotary_embedding.serving
+    a = rot_args(hq=2, hk=2)
+    x = a["q"]
+    assert serving(**{**a, "k": x}, out_q=x) is OOC and serving(**{**a, "k": x}, out_k=x) is OOC
+    assert serving(**{**a, "k": x}, out_q=x, out_k=x) is OOC
+    assert isinstance(serving(**{**a, "k": x}), KernelInfo)  # into new memory
+    assert isinstance(serving(**{**a, "k": x}, out_q=a["k"]), KernelInfo)
+    assert isinstance(serving(**a, out_q=x, out_k=a["k"]), KernelInfo)
