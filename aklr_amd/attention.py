@@ -28,7 +28,6 @@ are outside this library's scope; the op follows the conventions of its other op
 """
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass
 
 import torch
@@ -36,7 +35,7 @@ import torch
 from . import _lib, workspace
 from .dispatch import FallbackReason, aligned, api, on_gpu
 from .kv_cache import _OUT, cache_strides, starts_ok, table_ok, table_stride
-from .rotary import apart, stream, vectors_ok, wants_grad
+from .rotary import apart, number_ok, stream, vectors_ok, wants_grad
 
 _OOC = FallbackReason.OUT_OF_CONTRACT
 
@@ -112,7 +111,7 @@ def tree_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_l
             return _OOC
     if softmax_scale is None:
         softmax_scale = head_dim ** -0.5
-    elif not isinstance(softmax_scale, (int, float)) or not math.isfinite(softmax_scale):
+    elif not number_ok(softmax_scale):
         return _OOC
     if not on_gpu(*given) or wants_grad(q):
         return _OOC

@@ -451,7 +451,7 @@ bool number(PyObject* o, double* out) {
   if (!PyFloat_CheckExact(o) && !PyLong_CheckExact(o)) return false;
   *out = PyFloat_AsDouble(o);
   if (PyErr_Occurred()) return PyErr_Clear(), false;
-  return std::isfinite(*out);
+  return std::fabs(*out) <= 0x1p127;  // what fp32 holds, with room for a factor of log2(e)
 }
 
 struct Turn {  // what a rotation takes beside its vectors

@@ -48,3 +48,11 @@ def test_one_tensor_as_queries_and_keys_is_not_rotated_in_place(anywhere):
     assert isinstance(serving(**{**a, "k": x}), KernelInfo)  # into new memory
     assert isinstance(serving(**{**a, "k": x}, out_q=a["k"]), KernelInfo)
     assert isinstance(serving(**a, out_q=x, out_k=a["k"]), KernelInfo)
+
+
+@pytest.mark.parametrize("op,name,good", [("rotary", "magnitude", 1e38), ("both", "magnitude", -2), ("attend", "softmax_scale", 0.0)])
+def test_numbers_an_fp32_does_not_hold(anywhere, op, name, good):
+    fn, make = OPS[op]
+    assert isinstance(fn.serving(**make(), **{name: good}), KernelInfo)
+    for bad in (10**400, -(10**400), 1e300, -1e39, float("nan"), torch.ones(2)):
+        assert fn.serving(**make(), **{name: bad}) is OOC, bad
