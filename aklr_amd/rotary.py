@@ -120,13 +120,17 @@ def same_place(a, b) -> bool:
     return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride() and a.dtype == b.dtype
 
 
+def flag_ok(x) -> bool:
+    return not hasattr(x, "__len__") and x in (True, False)
+
+
 def number_ok(x) -> bool:
     """A number that fp32 holds, with room for the kernels' factor of log2(e)."""
     return isinstance(x, (int, float)) and abs(x) <= 2.0**127
 
 
 def rotary_ok(positions, frequencies, interleaved, magnitude, tokens, head_dim) -> bool:
-    if interleaved not in (True, False) or not number_ok(magnitude):
+    if not flag_ok(interleaved) or not number_ok(magnitude):
         return False
     if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (tokens,) or not positions.is_contiguous():
         return False

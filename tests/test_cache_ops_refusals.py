@@ -56,3 +56,11 @@ def test_numbers_an_fp32_does_not_hold(anywhere, op, name, good):
     assert isinstance(fn.serving(**make(), **{name: good}), KernelInfo)
     for bad in (10**400, -(10**400), 1e300, -1e39, float("nan"), torch.ones(2)):
         assert fn.serving(**make(), **{name: bad}) is OOC, bad
+
+
+@pytest.mark.parametrize("op,name", [("rotary", "interleaved"), ("both", "interleaved"), ("attend", "return_lse")])
+def test_flags_that_are_none(anywhere, op, name):
+    fn, make = OPS[op]
+    assert isinstance(fn.serving(**make(), **{name: True}), KernelInfo) and isinstance(fn.serving(**make(), **{name: 0}), KernelInfo)
+    for bad in (torch.zeros(2), torch.zeros(1), None, "1", 2):
+        assert fn.serving(**make(), **{name: bad}) is OOC, bad
