@@ -35,7 +35,7 @@ import torch
 from . import _lib, workspace
 from .dispatch import FallbackReason, aligned, api, on_gpu
 from .kv_cache import _OUT, cache_strides, starts_ok, table_ok, table_stride
-from .rotary import apart, flag_ok, number_ok, stream, vectors_ok, wants_grad
+from .rotary import apart, flag_ok, number_ok, stream, tensors_ok, vectors_ok, wants_grad
 
 _OOC = FallbackReason.OUT_OF_CONTRACT
 
@@ -86,7 +86,7 @@ def tree_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_l
     cache = (k_cache, v_cache, k_scale, v_scale)
     inputs = [q, *cache, block_table, seq_lens, starts] + ([tree_mask] if tree_mask is not None else [])
     given = inputs + ([out] if out is not None else [])
-    if not all(isinstance(t, torch.Tensor) for t in given) or not flag_ok(return_lse):
+    if not tensors_ok(*given) or not flag_ok(return_lse):
         return _OOC
     strides = cache_strides(*cache)
     if strides is None or strides[0] != strides[1] or strides[2] != strides[3] or q.dim() != 3 or q.dtype not in _OUT:

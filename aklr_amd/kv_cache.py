@@ -31,8 +31,8 @@ import torch
 
 from . import _lib
 from .dispatch import FallbackReason, aligned, api, on_gpu
-from .rotary import (_DTYPES, _MAX_HEADS, apart, no_inner_overlap, rotary_ok, same_place, stream, vectors_ok,
-                     wants_grad)
+from .rotary import (_DTYPES, _MAX_HEADS, apart, no_inner_overlap, rotary_ok, same_place, stream, tensors_ok,
+                     vectors_ok, wants_grad)
 
 _OOC = FallbackReason.OUT_OF_CONTRACT
 _OUT = {torch.bfloat16: _lib.OUT_BF16, torch.float16: _lib.OUT_F16}
@@ -136,7 +136,7 @@ def _run_write(p: _WritePlan):
 
 def _write_plan(k, v, cache, slots):
     """The checks of both writes on what they share: the cache's strides, or None."""
-    if not all(isinstance(t, torch.Tensor) for t in (k, v, slots, *cache)):
+    if not tensors_ok(k, v, slots, *cache):
         return None
     strides = cache_strides(*cache)
     if strides is None or k.dim() != 3 or k.dtype not in _DTYPES:
@@ -169,7 +169,7 @@ def rotary_kv_cache_write_fp8(q, k, v, positions, frequencies, k_cache, v_cache,
                               interleaved=False, magnitude=1.0, out=None):
     cache = (k_cache, v_cache, k_scale, v_scale)
     more = [q, positions, frequencies] + ([out] if out is not None else [])
-    if not all(isinstance(t, torch.Tensor) for t in more):
+    if not tensors_ok(*more):
         return _OOC
     strides = _write_plan(k, v, cache, slots)
     if strides is None or q.dim() != 3 or not 1 <= q.shape[1] <= _MAX_HEADS:
@@ -228,7 +228,7 @@ def kv_cache_read_fp8(k_cache, v_cache, k_scale, v_scale, block_table, starts, t
                       out_v=None):
     cache = (k_cache, v_cache, k_scale, v_scale)
     outs = [o for o in (out_k, out_v) if o is not None]
-    if not all(isinstance(t, torch.Tensor) for t in (*cache, block_table, starts, *outs)):
+    if not tensors_ok(*cache, block_table, starts, *outs):
         return _OOC
     if isinstance(total, bool) or not isinstance(total, int) or not 0 <= total < 2**31:
         return _OOC

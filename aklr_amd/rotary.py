@@ -77,6 +77,18 @@ def wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def tensors_ok(*tensors) -> bool:
+    """Whether all are tensors with memory of their own: a function transform's (vmap, jvp, grad) have none to name."""
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            return False
+        try:
+            t.data_ptr()
+        except RuntimeError:
+            return False
+    return True
+
+
 def vectors_ok(t, tokens, heads, head_dim, dtype) -> bool:
     """A [tokens, heads, head_dim] tensor the kernels can read: 16-byte pieces along the last dimension."""
     if t.dim() != 3 or tuple(t.shape) != (tokens, heads, head_dim) or t.dtype != dtype or t.layout != torch.strided:
@@ -182,7 +194,7 @@ def _run_rotary(p: _RotaryPlan):
 @api("rotary_embedding@1.0", _run_rotary, native="rotary")
 def rotary_embedding(q, k, positions, frequencies, *, interleaved=False, magnitude=1.0, out_q=None, out_k=None):
     given = [q, positions, frequencies] + [t for t in (k, out_q, out_k) if t is not None]
-    if not all(isinstance(t, torch.Tensor) for t in given):
+    if not tensors_ok(*given):
         return _OOC
     if q.dim() != 3 or q.dtype not in _DTYPES or (k is None and out_k is not None):
         return _OOC

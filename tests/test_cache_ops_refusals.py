@@ -64,3 +64,23 @@ def test_flags_that_are_none(anywhere, op, name):
     assert isinstance(fn.serving(**make(), **{name: True}), KernelInfo) and isinstance(fn.serving(**make(), **{name: 0}), KernelInfo)
     for bad in (torch.zeros(2), torch.zeros(1), None, "1", 2):
         assert fn.serving(**make(), **{name: bad}) is OOC, bad
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_tensors_of_a_function_transform_are_refused(anywhere, op):
+    fn, make = OPS[op]
+    args = make()
+    for name, t in args.items():
+        if not isinstance(t, torch.Tensor) or t.dtype == torch.float8_e4m3fn:
+            continue
+        answers = []
+
+        def ask(x):
+            answers.append(fn.serving(**{**args, name: x}))
+            return x.float().sum()
+
+        torch.vmap(ask)(torch.stack([t, t]))
+        if t.is_floating_point():
+            torch.func.jvp(ask, (t,), (torch.ones_like(t),))
+            torch.func.grad(ask)(t)
+        assert answers and all(a is OOC for a in answers), (name, answers)
