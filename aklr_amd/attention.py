@@ -23,8 +23,8 @@ softmax_scale=None, return_lse=False, out=None)``:
   was. Lengths stay on the device: nothing waits for the GPU, and a captured call serves other lengths, tables and
   masks of the same shapes.
 
-Calls it does not serve return a ``FallbackReason``; so does a call that wants gradients. The reference's attention ops
-are outside this library's scope; the op follows the conventions of its other ops.
+Calls it does not serve return a ``FallbackReason``; so does a call that wants gradients or tangents. The reference's
+attention ops are outside this library's scope; the op follows the conventions of its other ops.
 """
 from __future__ import annotations
 

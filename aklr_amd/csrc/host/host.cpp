@@ -425,7 +425,9 @@ bool no_inner_overlap(const Tensor& t) {
   return true;
 }
 
-bool wants_grad(const Tensor* t) { return t && t->requires_grad() && c10::GradMode::is_enabled(); }
+bool wants_grad(const Tensor* t) {
+  return t && ((t->requires_grad() && c10::GradMode::is_enabled()) || t->_fw_grad(/*level=*/0).defined());
+}
 
 int float_code(at::ScalarType t) {
   return t == at::kBFloat16 ? AKLR_OUT_BF16 : t == at::kHalf ? AKLR_OUT_F16 : t == at::kFloat ? AKLR_F32 : -1;

@@ -21,7 +21,7 @@ contiguous. page_size is a multiple of 16, up to 1024; head_dim 64, 128 or 256.
   does not have reads as zeros.
 
 The reference's quantizers are the model (this cache is not in its scope here). Calls they do not serve return a
-``FallbackReason``; so does a call that wants gradients.
+``FallbackReason``; so does a call that wants gradients or tangents.
 """
 from __future__ import annotations
 

@@ -13,7 +13,8 @@ rounded once. The reference has no such op in this library's scope.
 
 ``rotary_frequencies`` builds the frequencies, plain or scaled for contexts longer than those a model was trained on.
 
-Calls it does not serve return a ``FallbackReason``; so does a call that wants gradients: these ops are for inference.
+Calls it does not serve return a ``FallbackReason``; so does a call that wants gradients or
+tangents: these ops are for inference.
 """
 from __future__ import annotations
 
@@ -21,6 +22,7 @@ import math
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .dispatch import FallbackReason, aligned, api, on_gpu
@@ -74,7 +76,10 @@ def rotary_magnitude(factor, scale=1.0):
 # ---------------------------------------------------------------------------------------------
 # checks shared with the cache ops
 def wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether a gradient, or the tangent of forward mode, would be lost."""
+    given = [t for t in tensors if t is not None]
+    return (torch.is_grad_enabled() and any(t.requires_grad for t in given)) or any(
+        forward_ad.unpack_dual(t).tangent is not None for t in given)
 
 
 def tensors_ok(*tensors) -> bool:

@@ -84,3 +84,18 @@ def test_tensors_of_a_function_transform_are_refused(anywhere, op):
             torch.func.jvp(ask, (t,), (torch.ones_like(t),))
             torch.func.grad(ask)(t)
         assert answers and all(a is OOC for a in answers), (name, answers)
+
+
+@pytest.mark.parametrize("op,name", [("rotary", "q"), ("rotary", "k"), ("rotary", "frequencies"), ("write", "k"), ("write", "v"),
+                                     ("write", "v_scale"), ("both", "q"), ("both", "v"), ("both", "frequencies"), ("read", "k_scale"),
+                                     ("attend", "q"), ("attend", "k_scale")])
+def test_tangents_are_refused_not_lost(anywhere, op, name):
+    fn, make = OPS[op]
+    args = make()
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(args[name], torch.ones_like(args[name]))
+        assert fn.serving(**{**args, name: dual}) is OOC
+        with torch.no_grad():
+            assert fn.serving(**{**args, name: dual}) is OOC
+        assert isinstance(fn.serving(**args), KernelInfo)
+    assert isinstance(fn.serving(**args), KernelInfo)
