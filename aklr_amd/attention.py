@@ -113,7 +113,7 @@ def tree_attention_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_l
         softmax_scale = head_dim ** -0.5
     elif not number_ok(softmax_scale):
         return _OOC
-    if not on_gpu(*given) or wants_grad(q):
+    if not on_gpu(*given) or wants_grad(q, out):
         return _OOC
     if out is not None:
         if tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype or not out.is_contiguous() or not aligned(out):

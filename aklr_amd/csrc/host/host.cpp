@@ -538,7 +538,9 @@ PyObject* rotary(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
     Py_RETURN_NONE;
   if (k && (k->dim() != 3 || k->size(1) < 1 || k->size(1) > 32768 || !vectors_ok(*k, tokens, k->size(1), dim, type))) Py_RETURN_NONE;
   Turn turn;
-  if (!turn.read(p[2], p[3], p[4], p[5], tokens, dim) || wants_grad(q) || wants_grad(k)) Py_RETURN_NONE;
+  if (!turn.read(p[2], p[3], p[4], p[5], tokens, dim)) Py_RETURN_NONE;
+  for (const Tensor* t : {q, k, oq, ok})
+    if (wants_grad(t)) Py_RETURN_NONE;
   if (!one_device(*q, k, turn.positions, turn.frequencies, oq, ok)) Py_RETURN_NONE;
   for (int i = 0; i < 2; ++i) {
     const Tensor *out = i ? ok : oq, *like = i ? k : q, *other = i ? q : k;
@@ -594,7 +596,8 @@ PyObject* write_cache(PyObject* qo, PyObject* ko, PyObject* vo, PyObject* const*
     if (!q || !given(out_object, &out) || q->dim() != 3 || q->size(1) < 1 || q->size(1) > 32768 ||
         !vectors_ok(*q, tokens, q->size(1), c.dim, type))
       Py_RETURN_NONE;
-    if (!turn.read(turn_objects[0], turn_objects[1], turn_objects[2], turn_objects[3], tokens, c.dim) || wants_grad(q)) Py_RETURN_NONE;
+    if (!turn.read(turn_objects[0], turn_objects[1], turn_objects[2], turn_objects[3], tokens, c.dim) || wants_grad(q) || wants_grad(out))
+      Py_RETURN_NONE;
     if (!one_device(*k, q, turn.positions, turn.frequencies, out)) Py_RETURN_NONE;
     for (const Tensor* t : {q, turn.positions, turn.frequencies, out})
       if (t && !c.clear_of(t)) Py_RETURN_NONE;
@@ -707,7 +710,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
     scale = 1 / std::sqrt(static_cast<double>(dim));
   else if (!number(p[9], &scale))
     Py_RETURN_NONE;
-  if (!one_device(*q, c.t[0], table, lens, starts, mask, out) || wants_grad(q)) Py_RETURN_NONE;
+  if (!one_device(*q, c.t[0], table, lens, starts, mask, out) || wants_grad(q) || wants_grad(out)) Py_RETURN_NONE;
   if (out && (out->sizes() != q->sizes() || out->scalar_type() != type || !out->is_contiguous() || !aligned16(*out) ||
               !c.clear_of(out) || !apart_all(out, {q, table, lens, starts, mask})))
     Py_RETURN_NONE;

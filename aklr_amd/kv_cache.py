@@ -179,7 +179,7 @@ def rotary_kv_cache_write_fp8(q, k, v, positions, frequencies, k_cache, v_cache,
         return _OOC
     if not rotary_ok(positions, frequencies, interleaved, magnitude, tokens, head_dim):
         return _OOC
-    if not on_gpu(k, *more) or wants_grad(q):
+    if not on_gpu(k, *more) or wants_grad(q, out):
         return _OOC
     if not all(apart(c, t) for c in cache for t in more):
         return _OOC
@@ -243,6 +243,6 @@ def kv_cache_read_fp8(k_cache, v_cache, k_scale, v_scale, block_table, starts, t
             return _OOC
         if not all(apart(o, t) for t in (*cache, block_table, starts)):
             return _OOC
-    if not apart(out_k, out_v) or not on_gpu(*cache, block_table, starts, *outs):
+    if not apart(out_k, out_v) or not on_gpu(*cache, block_table, starts, *outs) or wants_grad(*outs):
         return _OOC
     return _ReadPlan(cache, strides, block_table, starts, total, out_dtype, out_k, out_v)

@@ -212,7 +212,7 @@ def rotary_embedding(q, k, positions, frequencies, *, interleaved=False, magnitu
         return _OOC
     if not rotary_ok(positions, frequencies, interleaved, magnitude, tokens, head_dim):
         return _OOC
-    if not on_gpu(*given) or wants_grad(q, k):
+    if not on_gpu(*given) or wants_grad(q, k, out_q, out_k):
         return _OOC
     for out, like, other in ((out_q, q, k), (out_k, k, q)):
         if out is None:

@@ -99,3 +99,21 @@ def test_tangents_are_refused_not_lost(anywhere, op, name):
             assert fn.serving(**{**args, name: dual}) is OOC
         assert isinstance(fn.serving(**args), KernelInfo)
     assert isinstance(fn.serving(**args), KernelInfo)
+
+
+OUTS = {"rotary": ("out_q", "q"), "both": ("out", "q"), "read": ("out_k", None), "attend": ("out", "q")}
+
+
+@pytest.mark.parametrize("op", OUTS)
+def test_an_output_that_wants_gradients_or_has_a_tangent_is_refused(anywhere, op):
+    fn, make = OPS[op]
+    args, (name, like) = make(), OUTS[op]
+    out = torch.zeros_like(args[like]) if like else torch.zeros((args["total"], 2, 64), dtype=BF16)
+    assert isinstance(fn.serving(**args, **{name: out}), KernelInfo)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(out, torch.ones_like(out))
+        assert fn.serving(**args, **{name: dual}) is OOC
+    out.requires_grad_()
+    assert fn.serving(**args, **{name: out}) is OOC
+    with torch.no_grad():
+        assert isinstance(fn.serving(**args, **{name: out}), KernelInfo)
