@@ -12,6 +12,7 @@ namespace aklr {
 
 constexpr int kThreads = 256;
 constexpr int kManyGroups = 4096;
+constexpr int64_t kMostGroups = 1 << 23;  // of one launch along x: it has fewer than 2^32 threads
 constexpr int64_t kManyItems = 1 << 20;
 
 // Eight consecutive values of T (bf16 bits, fp16 or fp32) as fp32, and back with one rounding to nearest even.
@@ -89,7 +90,7 @@ struct VecArgs {
   const double* freq;
   const void* slots;  // write
   float magnitude;
-  int tokens, per_wg;  // tokens, and tokens a workgroup takes at once
+  int first, tokens, per_wg;  // the launch's tokens from `first` to before `tokens`, and how many a workgroup takes at once
   int rot, interleaved, pos64, slot64;
   int kv_heads, page;
   int64_t slot_count;
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(kThreads) void vec_kernel(const VecArgs a, const in
   const int units = dim / 16;
   const int rot_units = ROT ? a.rot / 16 : 0;
   extern __shared__ float2 turn[];  // [per_wg][rot / 2] (cos, sin)
-  const int t0 = blockIdx.x * a.per_wg;
+  const int t0 = a.first + blockIdx.x * a.per_wg;
   const int nt = min(a.per_wg, a.tokens - t0);
   const int heads = (ROT ? a.q.heads : 0) + a.k.heads + (WRITE ? a.v.heads : 0);
   const int row = heads * units;  // items a token
@@ -273,17 +274,22 @@ __global__ __launch_bounds__(kThreads) void vec_kernel(const VecArgs a, const in
 template <typename T, int D, bool ROT, bool WRITE>
 int launch_vec(VecArgs& a, int head_dim, hipStream_t stream) {
   const int64_t row = (int64_t)((ROT ? a.q.heads : 0) + a.k.heads + (WRITE ? a.v.heads : 0)) * (head_dim / 16);
-  if (row == 0 || a.tokens == 0) return AKLR_OK;
+  const int64_t tokens = a.tokens;
+  if (row == 0 || tokens == 0) return AKLR_OK;
   a.per_wg = (int)(row >= kThreads ? 1 : kThreads / row);
   if (ROT && a.per_wg > 2048 / a.rot) a.per_wg = 2048 / a.rot;  // angles a workgroup keeps: 8 KiB
   int64_t gy = (row * a.per_wg + kThreads - 1) / kThreads;
-  if (ROT && (a.tokens + a.per_wg - 1) / a.per_wg * gy > kManyGroups) gy = 1;
-  const int64_t gx = (a.tokens + a.per_wg - 1) / a.per_wg;
-  if (gx > 0xFFFFFF || gy > 65535) return AKLR_ERR_INVALID_ARGUMENT;  // a launch has fewer than 2^32 threads
+  if (ROT && (tokens + a.per_wg - 1) / a.per_wg * gy > kManyGroups) gy = 1;
+  if (gy > 65535) return AKLR_ERR_INVALID_ARGUMENT;
   const size_t lds = ROT ? (size_t)a.per_wg * (a.rot / 2) * sizeof(float2) : 0;
-  hipLaunchKernelGGL((vec_kernel<T, D, ROT, WRITE>), dim3((unsigned)gx, (unsigned)gy), dim3(kThreads), lds, stream, a,
-                     head_dim);
-  AKLR_LAUNCH_CHECK();
+  const int64_t most = kMostGroups * a.per_wg;
+  for (int64_t first = 0; first < tokens; first += most) {
+    a.first = (int)first;
+    a.tokens = (int)(first + most < tokens ? first + most : tokens);
+    hipLaunchKernelGGL((vec_kernel<T, D, ROT, WRITE>), dim3((unsigned)((a.tokens - first + a.per_wg - 1) / a.per_wg), (unsigned)gy),
+                       dim3(kThreads), lds, stream, a, head_dim);
+    AKLR_LAUNCH_CHECK();
+  }
   return AKLR_OK;
 }
 
