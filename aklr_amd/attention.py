@@ -15,7 +15,10 @@ softmax_scale=None, return_lse=False, out=None)``:
   Keys' pages lie as far apart as values', and their scales' likewise (the cache's own layout, or both in one
   allocation). A block table reaches 2^28 positions, tokens * q_heads 2^28, sequences times kv_heads about 2^24.
 
-  A position's weight may reach 2^20 before the division, so values past 2^100 can overflow bf16's range.
+  Scores, their maxima and sums are fp32. A position's weight times its value scale is rounded before the product with
+  its codes: to 16 bits in calls of up to 32 rows (query tokens x q_heads // kv_heads) a sequence on the mean, in calls of
+  few rows altogether, and for fp16 queries always; to 8 bits (bf16, half a step of the output's type) for bf16 queries in
+  larger calls. Such a weight may reach 2^20, so values past 2^100 can overflow, for both types.
 
   Returns q's shape and dtype, with ``return_lse`` also the fp32 [tokens, q_heads] log of each softmax's sum, by which
   parts of a context can be joined. A token that sees nothing gets zeros and -inf. Nothing of a position that a token

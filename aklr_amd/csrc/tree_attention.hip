@@ -7,9 +7,12 @@
 //   x_p = (q . ck_p) * (sk_p * softmax_scale * log2 e),  m = max x_p,  l = sum 2^(x_p - m),
 //   o = sum (2^(x_p - m) * sv_p) cv_p / l.
 // A scale belongs to a token, so it multiplies a column of the scores and of the weights, never the codes: codes turn
-// into bf16 (fp16 for fp16 queries against keys) exactly, two an instruction, and the products run on matrix units.
-// The weights times sv become bf16 (fp16) for that: in two pieces up to 32 rows, where memory is the bound, in one (half
-// a step, at most 2^-8 of each term) in tiles of more, which the products bound. Scores, maxima, sums and outputs
+// into bf16 (keys into fp16 against fp16 queries) exactly, two an instruction, and the products run on matrix units.
+// The weights times sv become bf16 for that, whatever the queries' type: fp16's range would hold neither a value that fp16
+// does not, nor the weights of a row that one position draws to itself. Up to 32 rows, where memory is the bound, and for
+// fp16 queries they are two bf16 pieces (what is lost is at most 2^-16 of a term); for bf16 ones in tiles of more rows,
+// which the products bound, they are one (2^-8, half a step of the output's type): 2048 tokens of two prompts over 8192 take
+// 581 us with one and 731 with two. (One fp16 piece, whose range needs the scales in the codes' conversions, took 742.) Scores, maxima, sums and outputs
 // stay in fp32. Products of codes with e4m3 pieces of q would need no conversions of keys, but a chain of them sums to
 // 2^-15 of its size on this hardware (bf16 and fp16 products to 2^-23), which a log of a sum shows.
 #include "common.h"
@@ -20,18 +23,13 @@ namespace aklr {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4, kThreads = 256;
 constexpr int kUnit = 128;  // tokens a workgroup takes in one step: 32 a wave
 // Weights are 2^(x - m) for a reference m that is set kHead above the largest score so far and set again once a score
 // is kRise above it. Floating-point sums lose nothing by that, and a row's reference rises at most every kHead + kRise
-// powers of two: once for all where no score is 2^40 times the first ones'. Weights below 2^20 leave bf16 values to 2^100;
-// fp16 weights have all their bits from 2^-14 to 2^15, so theirs start at 1 and may rise to 2^14.
-template <bool F16>
-struct Range {
-  static constexpr float kHead = F16 ? 0.0f : 20.0f, kRise = F16 ? 14.0f : 20.0f;
-};
+// powers of two: once for all where no score is 2^40 times the first ones'. Weights below 2^20 leave bf16 values to 2^100.
+constexpr float kHead = 20.0f, kRise = 20.0f;
 constexpr float kNone = -3e38f;   // the reference in a partial result of a row that saw nothing
 
 struct AttnArgs {
@@ -175,11 +173,11 @@ __device__ __forceinline__ float across(float v, F f) {  // f over the four 16-l
 }
 
 template <bool F16, bool HIGH>
-__device__ __forceinline__ uint32_t two(uint32_t codes, float scale = 1.0f) {  // two e4m3 codes of a word as bf16 (fp16)
+__device__ __forceinline__ uint32_t two(uint32_t codes) {  // two e4m3 codes of a word as bf16 (fp16)
   if constexpr (F16)
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, HIGH));
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, HIGH));
   else
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, HIGH));
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, HIGH));
 }
 
 template <bool F16>
@@ -255,14 +253,6 @@ __device__ __forceinline__ void clean(uint32_t (*v)[VW], f32x4* s, uint32_t held
   }
 }
 
-// fp16 weights: a token's scale becomes a power of two from 2^-60 to 2^6, which the conversion of its codes multiplies
-// by, times what is returned (1 to 2 for every scale that fp16 values have), so that weights keep fp16's 11 bits.
-__device__ __forceinline__ float split_scale(float s, float& power) {
-  const uint32_t bits = min(max(__float_as_uint(s) & 0x7F800000u, 0x21800000u), 0x42800000u);
-  power = __uint_as_float(bits);
-  return s * __uint_as_float(0x7F000000u - bits);
-}
-
 __device__ __forceinline__ float masked(float x, uint32_t sees, int i) {  // -infinity where bit i is not set
   const uint32_t on = spread(sees, i);
   return __uint_as_float((__float_as_uint(x) & on) | (0xFF800000u & ~on));
@@ -299,7 +289,7 @@ __device__ __forceinline__ bool relate(f32x4 (&x)[NQ][2], const f32x4 (&ks)[2], 
 }
 
 // What the rows summed so far shrinks to their new references.
-template <bool F16, int NQ, int DT>
+template <int NQ, int DT>
 __device__ __forceinline__ void lift(f32x4 (&x)[NQ][2], float (&m)[NQ], float (&limit)[NQ], float (&l)[NQ],
                                      f32x4 (&o)[NQ][DT]) {
 #pragma unroll
@@ -308,10 +298,10 @@ __device__ __forceinline__ void lift(f32x4 (&x)[NQ][2], float (&m)[NQ], float (&
 #pragma unroll
     for (int i = 1; i < 8; ++i) top = fmaxf(top, x[n][i / 4][i % 4]);
     top = across(top, [](float u, float v) { return fmaxf(u, v); });
-    const bool first = limit[n] != Range<F16>::kRise;
+    const bool first = limit[n] != kRise;
     if (top > (first ? -__builtin_inff() : 0.0f)) {
-      top += Range<F16>::kHead;
-      limit[n] = Range<F16>::kRise;
+      top += kHead;
+      limit[n] = kRise;
     } else {
       top = 0.0f;
     }
@@ -325,10 +315,17 @@ __device__ __forceinline__ void lift(f32x4 (&x)[NQ][2], float (&m)[NQ], float (&
   }
 }
 
-// The weights, as the second product's operands. A bf16 keeps 8 bits of one (fp16 11), so what that leaves goes into a
-// second: an output is then as near as its type lets it be, and where memory is the bound the matrix unit has the time for
-// both (64 sequences of up to 8192 tokens, group 8: 128.1 us with one bf16, 128.6 with two).
-template <bool F16, int NQ>
+// Two weights as bf16, and what that leaves of them, as another two.
+__device__ __forceinline__ uint32_t pieces(float a, float b, uint32_t& rest) {
+  const uint32_t two = pack_bf16x2(a, b);
+  rest = pack_bf16x2(a - bf16_lo(two), b - bf16_hi(two));
+  return two;
+}
+
+// The weights, as the second product's operands. A bf16 keeps 8 bits of one, so what that leaves goes into a second: an
+// output is then as near as its type lets it be, and where memory is the bound the matrix unit has the time for both (64
+// sequences of up to 8192 tokens, group 8: 128.1 us with one bf16, 128.6 with two).
+template <int NQ>
 __device__ __forceinline__ void weigh(const f32x4 (&x)[NQ][2], const f32x4 (&vs)[2], bool edge,
                                       const uint32_t (&sees)[NQ], float (&l)[NQ], u32x4 (&hi)[NQ], u32x4 (&lo)[NQ]) {
 #pragma unroll
@@ -346,50 +343,28 @@ __device__ __forceinline__ void weigh(const f32x4 (&x)[NQ][2], const f32x4 (&vs)
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t two = pack_out2(w[2 * i], w[2 * i + 1], F16 ? AKLR_OUT_F16 : AKLR_OUT_BF16);
-      const f16x2 h = __builtin_bit_cast(f16x2, two);
-      const float a = F16 ? (float)h[0] : bf16_lo(two), b = F16 ? (float)h[1] : bf16_hi(two);
-      hi[n][i] = two;
-      lo[n][i] = pack_out2(w[2 * i] - a, w[2 * i + 1] - b, F16 ? AKLR_OUT_F16 : AKLR_OUT_BF16);
+      uint32_t rest;
+      hi[n][i] = pieces(w[2 * i], w[2 * i + 1], rest);
+      lo[n][i] = rest;
     }
   }
 }
 
 // Four tokens' words of four codes turned over: out[e] holds dimension e of the four, two values a word.
-template <bool F16>
-__device__ __forceinline__ void turn_over(uint32_t a, uint32_t b, uint32_t c, uint32_t d, const float* power, u32x2 (&out)[4]) {
-  if constexpr (F16) {  // a power of two for each token, so a conversion takes one token's pair
-    const uint32_t al = two<true, false>(a, power[0]), ah = two<true, true>(a, power[0]);
-    const uint32_t bl = two<true, false>(b, power[1]), bh = two<true, true>(b, power[1]);
-    const uint32_t cl = two<true, false>(c, power[2]), ch = two<true, true>(c, power[2]);
-    const uint32_t dl = two<true, false>(d, power[3]), dh = two<true, true>(d, power[3]);
-    out[0] = u32x2{__builtin_amdgcn_perm(bl, al, 0x05040100), __builtin_amdgcn_perm(dl, cl, 0x05040100)};
-    out[1] = u32x2{__builtin_amdgcn_perm(bl, al, 0x07060302), __builtin_amdgcn_perm(dl, cl, 0x07060302)};
-    out[2] = u32x2{__builtin_amdgcn_perm(bh, ah, 0x05040100), __builtin_amdgcn_perm(dh, ch, 0x05040100)};
-    out[3] = u32x2{__builtin_amdgcn_perm(bh, ah, 0x07060302), __builtin_amdgcn_perm(dh, ch, 0x07060302)};
-  } else {
-    const uint32_t l0 = __builtin_amdgcn_perm(b, a, 0x05010400), l1 = __builtin_amdgcn_perm(d, c, 0x05010400);
-    const uint32_t h0 = __builtin_amdgcn_perm(b, a, 0x07030602), h1 = __builtin_amdgcn_perm(d, c, 0x07030602);
-    out[0] = u32x2{two<false, false>(l0), two<false, false>(l1)};
-    out[1] = u32x2{two<false, true>(l0), two<false, true>(l1)};
-    out[2] = u32x2{two<false, false>(h0), two<false, false>(h1)};
-    out[3] = u32x2{two<false, true>(h0), two<false, true>(h1)};
-  }
+__device__ __forceinline__ void turn_over(uint32_t a, uint32_t b, uint32_t c, uint32_t d, u32x2 (&out)[4]) {
+  const uint32_t l0 = __builtin_amdgcn_perm(b, a, 0x05010400), l1 = __builtin_amdgcn_perm(d, c, 0x05010400);
+  const uint32_t h0 = __builtin_amdgcn_perm(b, a, 0x07030602), h1 = __builtin_amdgcn_perm(d, c, 0x07030602);
+  out[0] = u32x2{two<false, false>(l0), two<false, false>(l1)};
+  out[1] = u32x2{two<false, true>(l0), two<false, true>(l1)};
+  out[2] = u32x2{two<false, false>(h0), two<false, false>(h1)};
+  out[3] = u32x2{two<false, true>(h0), two<false, true>(h1)};
 }
 
 // The same for two codes of a token.
-template <bool F16>
-__device__ __forceinline__ void turn_over2(uint32_t a, uint32_t b, uint32_t c, uint32_t d, const float* power, u32x2 (&out)[2]) {
-  if constexpr (F16) {
-    const uint32_t x = two<true, false>(a, power[0]), y = two<true, false>(b, power[1]);
-    const uint32_t z = two<true, false>(c, power[2]), w = two<true, false>(d, power[3]);
-    out[0] = u32x2{__builtin_amdgcn_perm(y, x, 0x05040100), __builtin_amdgcn_perm(w, z, 0x05040100)};
-    out[1] = u32x2{__builtin_amdgcn_perm(y, x, 0x07060302), __builtin_amdgcn_perm(w, z, 0x07060302)};
-  } else {
-    const uint32_t l0 = __builtin_amdgcn_perm(b, a, 0x05010400), l1 = __builtin_amdgcn_perm(d, c, 0x05010400);
-    out[0] = u32x2{two<false, false>(l0), two<false, false>(l1)};
-    out[1] = u32x2{two<false, true>(l0), two<false, true>(l1)};
-  }
+__device__ __forceinline__ void turn_over2(uint32_t a, uint32_t b, uint32_t c, uint32_t d, u32x2 (&out)[2]) {
+  const uint32_t l0 = __builtin_amdgcn_perm(b, a, 0x05010400), l1 = __builtin_amdgcn_perm(d, c, 0x05010400);
+  out[0] = u32x2{two<false, false>(l0), two<false, false>(l1)};
+  out[1] = u32x2{two<false, true>(l0), two<false, true>(l1)};
 }
 
 // Partial results: for each slot, o [R][D] not yet divided by l, then (m, l, -, -) [R].
@@ -666,25 +641,20 @@ __global__ __launch_bounds__(kThreads, 2) void stream_kernel(const AttnArgs a) {
     return relate<NQ>(x, scale, edge, sees, m, limit);
   };
   auto second = [&](Values& t, bool edge) {
-    float power[8];
-    if constexpr (F16) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t.s[i / 4][i % 4] = split_scale(t.s[i / 4][i % 4], power[i]);
-    }
     u32x4 w_hi[NQ], w_lo[NQ];
-    weigh<F16, NQ>(x, t.s, edge, sees, l, w_hi, w_lo);
+    weigh<NQ>(x, t.s, edge, sees, l, w_hi, w_lo);
 #pragma unroll
     for (int w = 0; w < VW; ++w) {  // a word holds 4 dimensions of a token; an operand wants one, of 8 tokens
       u32x2 lo[4], hi[4];
-      turn_over<F16>(t.v[0][w], t.v[1][w], t.v[2][w], t.v[3][w], power, lo);
-      turn_over<F16>(t.v[4][w], t.v[5][w], t.v[6][w], t.v[7][w], power + 4, hi);
+      turn_over(t.v[0][w], t.v[1][w], t.v[2][w], t.v[3][w], lo);
+      turn_over(t.v[4][w], t.v[5][w], t.v[6][w], t.v[7][w], hi);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
           const u32x4 v = {lo[e][0], lo[e][1], hi[e][0], hi[e][1]};
-          o[n][4 * w + e] = mfma32<F16>(v, w_hi[n], o[n][4 * w + e]);
-          o[n][4 * w + e] = mfma32<F16>(v, w_lo[n], o[n][4 * w + e]);
+          o[n][4 * w + e] = mfma32<false>(v, w_hi[n], o[n][4 * w + e]);
+          o[n][4 * w + e] = mfma32<false>(v, w_lo[n], o[n][4 * w + e]);
         }
     }
   };
@@ -719,7 +689,7 @@ __global__ __launch_bounds__(kThreads, 2) void stream_kernel(const AttnArgs a) {
       move();
     } while (plain());
     if (!plain()) break;
-    lift<F16, NQ, DT>(x, m, limit, l, o);
+    lift<NQ, DT>(x, m, limit, l, o);
     Values t = read_values(ring[wave][slot]);
     second(t, false);
     move();
@@ -734,7 +704,7 @@ __global__ __launch_bounds__(kThreads, 2) void stream_kernel(const AttnArgs a) {
     const uint32_t held = held_by<8, 16>(4 * g, end - p, is_page(at[0].id[0]), is_page(at[0].id[1]));
 #pragma unroll
     for (int n = 0; n < NQ; ++n) sees[n] = seen_by<8, 16>(a, held, p + 4 * g - ctx, row_t[n], it.q0);
-    if (first(stage, true)) lift<F16, NQ, DT>(x, m, limit, l, o);
+    if (first(stage, true)) lift<NQ, DT>(x, m, limit, l, o);
     Values t = read_values(stage);
     clean<8, 16, VW>(t.v, t.s, held);
     second(t, true);
@@ -750,7 +720,7 @@ __global__ __launch_bounds__(kThreads, 2) void stream_kernel(const AttnArgs a) {
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     l[n] = across(l[n], [](float u, float v) { return u + v; });
-    if (limit[n] != Range<F16>::kRise) m[n] = kNone;
+    if (limit[n] != kRise) m[n] = kNone;
     if (g == 0) wave_m[wave][16 * n + c] = m[n], wave_l[wave][16 * n + c] = l[n];
   }
   __syncthreads();
@@ -826,6 +796,7 @@ __device__ __forceinline__ f32x16 mfma16(const u32x4& a, const u32x4& b, const f
 template <int D, int W, bool F16>
 __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void tile_kernel(const AttnArgs a) {
   constexpr int R = 32 * W, QS = D / 16, DT = D / 32, C = D / 16, KL = D / 32, ND = D / 64;
+  constexpr bool kTwo = F16;  // bf16 pieces of a weight
   constexpr int kStep = 64, S = W == 2 ? 2 : 3, kStage = 2 * kStep * D + 8 * kStep, kBlocks = 4 / W;  // blocks of 16 a wave loads
   const int head = blockIdx.x % a.hkv, index = blockIdx.x / a.hkv;
   const Item it = find<R>(a, index);
@@ -991,10 +962,10 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void tile_kernel(const Att
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
     top = across(top, [](float u, float v) { return fmaxf(u, v); });
-    const bool first = limit != Range<F16>::kRise;
+    const bool first = limit != kRise;
     if (top > (first ? -__builtin_inff() : 0.0f)) {
-      top += Range<F16>::kHead;
-      limit = Range<F16>::kRise;
+      top += kHead;
+      limit = kRise;
     } else {
       top = 0.0f;
     }
@@ -1012,13 +983,8 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void tile_kernel(const Att
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {  // 16 tokens: 16kk + 8b + 4hf + 0..3
       auto& v = reinterpret_cast<uint32_t(&)[2][4][VN]>(t.v[2 * kk]);
-      f32x4 s[2] = {t.vs[2 * kk], t.vs[2 * kk + 1]};
-      float power[2][4] = {{1, 1, 1, 1}, {1, 1, 1, 1}};
-      if constexpr (F16) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s[i / 4][i % 4] = split_scale(s[i / 4][i % 4], power[i / 4][i % 4]);
-      }
-      u32x4 pt;
+      const f32x4 s[2] = {t.vs[2 * kk], t.vs[2 * kk + 1]};
+      u32x4 pt, rest;
       float w[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -1031,7 +997,11 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void tile_kernel(const Att
         for (int i = 0; i < 8; ++i) w[i] = masked_weight(w[i], sees, 8 * kk + i);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pt[i] = pack_out2(w[2 * i], w[2 * i + 1], F16 ? AKLR_OUT_F16 : AKLR_OUT_BF16);
+      for (int i = 0; i < 4; ++i) {
+        uint32_t left;
+        pt[i] = pieces(w[2 * i], w[2 * i + 1], left);
+        if constexpr (kTwo) rest[i] = left;
+      }
       if (kk == 0) __builtin_amdgcn_s_setprio(1);
       constexpr int E = VB == 2 ? 2 : 4;  // dimensions of a word
 #pragma unroll
@@ -1040,13 +1010,16 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void tile_kernel(const Att
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           if constexpr (E == 2)
-            turn_over2<F16>(v[b][0][0], v[b][1][0], v[b][2][0], v[b][3][0], power[b], y4[b]);
+            turn_over2(v[b][0][0], v[b][1][0], v[b][2][0], v[b][3][0], y4[b]);
           else
-            turn_over<F16>(v[b][0][y], v[b][1][y], v[b][2][y], v[b][3][y], power[b], y4[b]);
+            turn_over(v[b][0][y], v[b][1][y], v[b][2][y], v[b][3][y], y4[b]);
         }
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          o[E * y + e] = mfma16<F16>(u32x4{y4[0][e][0], y4[0][e][1], y4[1][e][0], y4[1][e][1]}, pt, o[E * y + e]);
+        for (int e = 0; e < E; ++e) {
+          const u32x4 z = {y4[0][e][0], y4[0][e][1], y4[1][e][0], y4[1][e][1]};
+          o[E * y + e] = mfma16<false>(z, pt, o[E * y + e]);
+          if constexpr (kTwo) o[E * y + e] = mfma16<false>(z, rest, o[E * y + e]);
+        }
       }
     }
   };
@@ -1106,7 +1079,7 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void tile_kernel(const Att
 
   const rsrc_t to = slot_at<D, R>(a, head, it.slot + it.split * it.tiles);
   l = across(l, [](float u, float v) { return u + v; });
-  if (limit != Range<F16>::kRise) m = kNone;
+  if (limit != kRise) m = kNone;
   const int row = rw + c;
   if (row < rows) {  // DT consecutive dimensions of it for each of the accumulators' 16 rows
 #pragma unroll

@@ -323,7 +323,8 @@ int aklr_kv_cache_read_fp8(const void* k_codes, const void* v_codes, const float
  * outside every sequence keep what out and lse hold. Positions past the block table's columns, and pages outside
  * [0, pages), are seen by none. starts ascend.
  * q: [total_q, q_heads, head_dim] bf16 or fp16 (dtype), strides in elements, multiples of 8; out: the same dtype,
- * contiguous; head h attends kv head h / (q_heads / kv_heads). lse: fp32 [total_q, q_heads]. mask: bytes, rows
+ * contiguous; head h attends kv head h / (q_heads / kv_heads). Weights are rounded to 16 bits, and to 8 (one bf16) for
+ * bf16 queries where aklr_tree_attention_fp8_rows is 64 or 128. lse: fp32 [total_q, q_heads]. mask: bytes, rows
  * mask_stride apart. head_dim 64, 128 or 256; page_size a multiple of 16 up to 1024; table_cols * page_size <= 2^28; pages
  * of keys and of values lie code_page elements apart, those of their scales scale_page.
  * Workspace: aklr_tree_attention_fp8_workspace_bytes(..., capacity = table_cols * page_size), any content. Results do
