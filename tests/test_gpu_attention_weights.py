@@ -54,20 +54,28 @@ def exact(p, scale):
     for b, n in enumerate(lens):
         lo, hi = starts[b], starts[b + 1]
         pages = p["table"][b, : -(-n // page)].long()
+        there = ((pages >= 0) & (pages < kc.shape[0])).repeat_interleave(page)[:n]
+        pages = pages.clamp(0, kc.shape[0] - 1)
         k, v = ((c.view(torch.uint8)[pages].view(c.dtype).float().double() * s[pages].double()[..., None]).permute(1, 0, 2, 3).reshape(heads, -1, d)[:, :n].contiguous()
                 for c, s in ((kc, ks), (vc, vs)))
         t, group = hi - lo, hq // heads
         q = p["q"][lo:hi].double().view(t, heads, group, d).transpose(0, 1).reshape(heads, t * group, d)
-        sees = torch.ones((t, n), dtype=torch.bool, device=DEV)
-        sees[:, n - t:] = torch.ones((t, t), device=DEV).tril().bool() if p["mask"] is None else p["mask"][lo:hi, :t]
-        sees = sees.repeat_interleave(group, 0)
+        if not t or not n:
+            rows[0][lo:hi] = -float("inf")
+            continue
+        j = torch.arange(n, device=DEV) - (n - t)
+        if p["mask"] is None:
+            sees = j <= torch.arange(t, device=DEV)[:, None]
+        else:
+            sees = (j < 0) | p["mask"][lo:hi, j.clamp(0, t - 1)].bool()
+        sees = (sees & there).repeat_interleave(group, 0)
 
         def place(x):  # [heads, t * group, ...] -> [t, hq, ...]
             return x.view(heads, t, group, *x.shape[2:]).transpose(0, 1).reshape(t, hq, *x.shape[2:])
 
         x = (torch.matmul(q, k.transpose(1, 2).contiguous()) * scale).masked_fill(~sees, -float("inf"))
         end = x.logsumexp(-1)
-        w = (x - end[..., None]).exp()
+        w = (x - end[..., None]).exp().masked_fill(~sees, 0)
         outs[0][lo:hi], outs[1][lo:hi], rows[0][lo:hi] = place(torch.matmul(w, v)), place(torch.matmul(w, v.abs())), place(end)
         size = torch.matmul(q.abs(), k.abs().transpose(1, 2).contiguous()).masked_fill(~sees, 0).amax(-1) * abs(scale)
         rows[1][lo:hi] = place(size)
@@ -84,14 +92,17 @@ def check(p, rows=None, scale=None, joined=None):
     want, wl, weighed, size, n = exact(p, scale)
     top = size.clamp_min(1) / np.log(2)
     e = 2**-24 * ((d + 3) * size + 8 * top + 128)
-    assert bool(((lse.double() - wl).abs() <= e + (n + 64) * 2**-24 + 2**-23 * wl.abs()).all())
+    end, empty = int(p["starts"][-1]), wl == -float("inf")
+    assert torch.equal(lse[:end] == -float("inf"), empty[:end]) and not bool(out[:end][empty[:end]].any())
+    out, lse, want, wl, weighed, e, empty = (x[:end] for x in (out, lse, want, wl, weighed, e, empty))
+    assert bool(((lse.double() - wl).abs() <= e + (n + 64) * 2**-24 + 2**-23 * wl.abs())[~empty].all())
     tol = weighed * (lost(got_rows, dtype) + 2 * e[..., None] + 2 * (n + 64) * 2**-24)
     tol = tol + want.abs() * torch.finfo(dtype).eps / 2 * 1.01 + (2**-25 if dtype == F16 else 0)
     finite = want.abs() <= torch.finfo(dtype).max
     assert not bool(out[finite].isnan().any())
     far = ((out.double() - want).abs() - tol)[finite]
     assert bool((far <= 0).all()), f"{float(far.max())} past the tolerance"
-    assert torch.equal(out, call(p, softmax_scale=scale))
+    assert torch.equal(out, call(p, softmax_scale=scale)[:end])
     return out, lse
 
 
