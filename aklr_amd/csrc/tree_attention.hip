@@ -484,7 +484,8 @@ __global__ __launch_bounds__(kThreads, 2) void stream_kernel(const AttnArgs a) {
   if (!it.ok) return;
   uint64_t* const word = a.word + (int64_t)head * a.words + it.row_tile;
   uint64_t seen = 0;
-  if (threadIdx.x == 0 && it.splits > 1 && !a.joiners) seen = splitk_peek(word);
+  const bool joins = NQ == 1 && !a.joiners;  // the last workgroup of a tile; 32 rows have the other kernel for it
+  if (threadIdx.x == 0 && it.splits > 1 && joins) seen = splitk_peek(word);
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int rows = it.count * a.group, r0 = it.tile * R, ctx = it.len - it.count;
   const int last_t = (min(r0 + R, rows) - 1) / a.group, first_t = r0 / a.group;
@@ -766,9 +767,11 @@ __global__ __launch_bounds__(kThreads, 2) void stream_kernel(const AttnArgs a) {
       finish<DT, F16>(a, it, head, row, d, best, total, v);
     }
   }
-  if (it.splits == 1 || a.joiners) return;
-  __shared__ unsigned arrived;
-  if (splitk_arrive(word, seen, it.splits, &arrived)) join<D, R, F16>(a, it, head, 0, min(R, rows - r0), r0, &sum[0][0][0]);
+  if constexpr (NQ == 1) {
+    if (it.splits == 1 || !joins) return;
+    __shared__ unsigned arrived;
+    if (splitk_arrive(word, seen, it.splits, &arrived)) join<D, R, F16>(a, it, head, 0, min(R, rows - r0), r0, &sum[0][0][0]);
+  }
 }
 
 template <bool F16>
