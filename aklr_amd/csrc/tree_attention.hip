@@ -1128,18 +1128,26 @@ struct AttnPlan {
 
 bool plan_attention(int64_t total, int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t capacity, AttnPlan* p) {
   const int64_t group = hq / hkv, rows = (total * group + batch - 1) / batch;  // of a sequence, on the mean
-  // Tiles of many rows where they fill the chip, else more workgroups of fewer. Heads of 128, 8 kv heads, in us with tiles
-  // of 128 and with 32: one sequence of 132 rows over 2000 tokens 23.1 and 17.2, of 2048 over 8000 125 and 126, four of
-  // 132 over 8000 48 and 41; 16 of them 98 and 127, two of 8192 rows 114 and 164. 32 rows of 16 sequences in tiles of 64
-  // 64.8, of 32 52.9, of 16 56.9; 4 rows of one in 32 50.5, of 16 44.3. Heads of 256 (16 rows beside 128): one of 132
-  // over 8000 43 and 56, four 103 and 83, 64 of 33 over 1000 203 and 129.
-  const bool many = rows > 32 && batch * hkv * ((rows + 127) / 128) >= (d == 256 ? 64 : 128);
+  const int64_t units = (capacity + kUnit - 1) / kUnit;
+  // Tiles of many rows where there is much to do, else more workgroups of fewer: a step of 128 tokens for 128 rows is
+  // the unit, a tile of 64 rows half of one, over as many tokens as the table has room for. In us with tiles of 128 (64) and
+  // with 32, contexts ragged between half and all of what is named:
+  //   heads of 128, 128 rows: 2048 units (32 sequences of 1000, 8 kv heads) 50 and 42, (8 of 4000) 49 and 43; 4096 (16 of
+  //     4000) 63 and 66; 4032 (32 of 8000, 2 kv heads) 62 and 84; 8000 (8 of 16000) 95 and 118; 64512 (32 of 8000, 32) 566 and 676;
+  //   trees of up to 33 tokens, group 4 (101 rows): 12, 14, 16 and 20 over 2000 (up to 2560) 49 49 52 60 and 42 43 47 50; over
+  //     16384 4 (4128) 68 and 59, 6 84 and 85, 12, 14, 15, 16 and 17 142 159 173 173 193 and 158 172 207 233 231;
+  //   64 rows: 1024 (8 of 4000) 43 and 30, 4000 (8 of 16000) 71 and 69, 8000 (16) 118 and 126;
+  //   heads of 64, 128 rows: 2048 (8 of 4000) 34 and 35, 8000 (8 of 16000) 76 and 90;
+  //   heads of 256 (16 rows beside 128): 512 (8 of 1000) 48 and 35, 1024 (4 of 4000) 60 and 56, 2048 (8) 80 and 89.
+  // Where a sequence's rows leave much of their last tile empty more would be better (132 of them 94 and 72 at 8192 units).
+  // 32 rows of 16 sequences in tiles of 64 64.8, of 32 52.9, of 16 56.9; 4 rows of one in 32 50.5, of 16 44.3.
+  const int64_t half_tiles = batch * hkv * units * (rows > 64 ? 2 * ((rows + 127) / 128) : 1);
+  const bool many = rows > 32 && half_tiles >= (d == 256 ? 2000 : 8000);
   p->rows = many ? rows > 64 ? 128 : 64 : rows > 16 && d < 256 ? 32 : 16;
   const int64_t slots = kCus * (p->rows == 64 ? 4 : 2) / (d == 256 ? 2 : 1), target = slots * 3 / 2;
   p->target = (target + hkv - 1) / hkv < kMostSplits ? (target + hkv - 1) / hkv : kMostSplits;
   p->slots = (slots + hkv - 1) / hkv < kMostSplits ? (slots + hkv - 1) / hkv : kMostSplits;
   p->tiles = total * group / p->rows + (batch < total ? batch : total);
-  const int64_t units = (capacity + kUnit - 1) / kUnit;
   p->cap = p->tiles + (units > 1 ? p->target : 0);
   const int64_t tiles = batch * ((rows + p->rows - 1) / p->rows);  // at the mean; with the most splits a tile can have
   const int64_t splits = units < p->slots / tiles ? units : p->slots / tiles;

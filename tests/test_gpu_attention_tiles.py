@@ -10,7 +10,7 @@ import aklr_amd
 from aklr_amd import workspace
 from tests.helpers import say
 from tests.test_gpu_attention import call, i32, problem, tree
-from tests.test_gpu_attention_weights import FORMS, FORMS_OF, check, exact, lost, rows_of
+from tests.test_gpu_attention_weights import FORMS, FORMS_OF, check, exact, lost, reach
 from tests.test_gpu_kv_cache import BF16, DEV, F16
 
 pytestmark = pytest.mark.gpu
@@ -53,7 +53,7 @@ def test_a_score_is_an_fp32_sum_in_every_form(d, form, dtype):
     say(f"scores {d} {form} {dtype}")
     b, t, h, group = FORMS[form]
     p = problem([t] * b, [t] * b, h, group, d, 16, dtype, seed=29, mask=lambda rng, n: np.eye(n, dtype=bool))
-    assert rows_of(p)[0] == form
+    reach(p, form)
     out, lse = call(p, return_lse=True)
     want, wl, weighed, size, _ = exact(p, d ** -0.5)
     assert bool(((lse.double() - wl).abs() <= 2**-24 * ((d + 3) * size + 4 * wl.abs() / np.log(2) + 128)).all())
@@ -61,13 +61,13 @@ def test_a_score_is_an_fp32_sum_in_every_form(d, form, dtype):
     assert bool(((out.double() - want).abs() <= tol).all())
 
 
-@pytest.mark.parametrize("d,h,group,counts,page,rows", [(64, 64, 5, [30, 12], 16, 128), (128, 32, 4, [17, 1, 20, 9], 32, 64),
-                                                        (256, 16, 7, [19, 3, 9, 10], 64, 128)])
-def test_one_piece_of_each_tile(d, h, group, counts, page, rows):
+@pytest.mark.parametrize("d,h,b,group,page,rows", [(64, 64, 64, 35, 16, 128), (128, 64, 128, 20, 32, 64), (256, 32, 32, 31, 64, 128)])
+def test_one_piece_of_each_tile(d, h, b, group, page, rows):
     # no more than 128 positions: nothing to join, and no workspace
     say(f"one piece {d} {rows}")
-    p = problem([128 - 11 * i if i % 2 == 0 else counts[i] for i in range(len(counts))], counts, h, group, d, page, BF16, seed=33, mask=tree)
-    p["table"] = p["table"][:, :128 // page].contiguous()
+    counts = [[3, 1, 0, 5, 2][i % 5] for i in range(b)]
+    p = problem([128 if i == 0 else c + 13 * i % 120 for i, c in enumerate(counts)], counts, h, group, d, page, BF16, seed=33, mask=tree)
+    assert p["table"].shape[1] * page == 128
     check(p, rows, joined=False)
     p["mask"] = None
     check(p, rows, joined=False)
@@ -92,7 +92,7 @@ def test_lengths_below_the_counts_and_missing_pages(d, h, group, counts, lens, p
 def test_nothing_unseen_reaches_a_row(d, h, group, counts, lens, page, rows, masked):
     say(f"NaN and infinities not seen {d} {rows} {masked}")
     p = problem(lens, counts, h, group, d, page, BF16, seed=37, mask=tree if masked else None)
-    assert rows_of(p)[0] == rows
+    reach(p, rows)
     want = call(p, return_lse=True)
     used = torch.zeros(p["cache"][2].shape[0], page, dtype=torch.bool, device=DEV)
     for b, n in enumerate(lens):
