@@ -53,7 +53,7 @@ struct AttnArgs {
   int slots, target;
   int dim;     // of a head
   int wide;    // page % 32 == 0
-  int cap;     // items a kv head can have
+  int held;    // partial results a kv head can have
   int words;   // tiles of rows a kv head can have: arrival words
   int joiners;  // workgroups of a kernel of its own that join a tile's partial results; 0: the last of those that wrote them does
   float scale_log2;
@@ -66,7 +66,7 @@ struct Item {
   int b, tiles, tile, split, splits, chunk;
   int q0, count, len;  // the sequence's first query token, how many, its positions
   int row_tile;        // the tile's number over all sequences
-  int slot;            // of the partial result of the tile's first split
+  int slot;            // of the partial result of the tile's first split, where there are several
   bool ok;
 };
 
@@ -108,15 +108,16 @@ __device__ __forceinline__ Item find(const AttnArgs& a, int index) {
   Item r{};
   const int target = all_tiles > 0 && 2 * all_tiles <= a.slots ? a.slots - all_tiles : a.target;
   r.chunk = uniform((int)fmin((double)work / target, (double)(1 << 23)) + 1);
-  int items_before = 0, tiles_before = 0;  // of the 64 sequences at hand
+  int items_before = 0, tiles_before = 0, held_before = 0;  // of the 64 sequences at hand
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     if (b0) s = look(b0 + lane);
     const int splits = (s.units + r.chunk - 1) / r.chunk;
-    int items = s.tiles * splits, tiles = s.tiles;  // inclusive sums over the lanes
+    // inclusive sums over the lanes; only a tile of several splits has partial results
+    int items = s.tiles * splits, tiles = s.tiles, held = splits > 1 ? items : 0;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
-      const int x = __shfl_up(items, d, 64), y = __shfl_up(tiles, d, 64);
-      if (lane >= d) items += x, tiles += y;
+      const int x = __shfl_up(items, d, 64), y = __shfl_up(tiles, d, 64), z = __shfl_up(held, d, 64);
+      if (lane >= d) items += x, tiles += y, held += z;
     }
     const uint64_t past = __ballot(TILE ? tiles_before + tiles > index : items_before + items > index);
     if (past) {
@@ -126,22 +127,26 @@ __device__ __forceinline__ Item find(const AttnArgs& a, int index) {
       r.tiles = take(s.tiles);
       r.splits = take(splits);
       r.chunk = (take(s.units) + r.splits - 1) / r.splits;  // of even length
-      r.slot = items_before + take(items) - r.tiles * r.splits;
+      r.slot = held_before + take(held) - r.tiles * r.splits;
       r.row_tile = tiles_before + take(tiles) - r.tiles;
-      r.split = TILE ? 0 : (index - r.slot) / r.tiles;
-      r.tile = TILE ? index - r.row_tile : index - r.slot - r.split * r.tiles;
+      const int nth = TILE ? index - r.row_tile : index - (items_before + take(items) - r.tiles * r.splits);
+      r.split = TILE ? 0 : nth / r.tiles;
+      r.tile = nth - r.split * r.tiles;
       r.tile = r.tiles - 1 - r.tile;  // the last first: under causal masks it sees the most
       r.slot += r.tile;
       r.row_tile += r.tile;
       r.q0 = take(s.q0);
       r.count = take(s.count);
       r.len = take(s.len);
-      // starts that do not ascend can make more of both than there is room for
-      r.ok = r.slot >= 0 && r.slot + (int64_t)(r.splits - 1) * r.tiles < a.cap && (unsigned)r.row_tile < (unsigned)a.words;
+      // starts that do not ascend can make more of all than there is room for, or than an int counts
+      r.ok = (unsigned)r.tile < (unsigned)r.tiles && (unsigned)r.split < (unsigned)r.splits &&
+             (unsigned)r.row_tile < (unsigned)a.words &&
+             (r.splits == 1 || (r.slot >= 0 && r.slot + (int64_t)(r.splits - 1) * r.tiles < a.held));
       return r;
     }
     items_before += __builtin_amdgcn_readlane(items, 63);
     tiles_before += __builtin_amdgcn_readlane(tiles, 63);
+    held_before += __builtin_amdgcn_readlane(held, 63);
   }
   return r;
 }
@@ -370,7 +375,7 @@ __device__ __forceinline__ void turn_over2(uint32_t a, uint32_t b, uint32_t c, u
 // Partial results: for each slot, o [R][D] not yet divided by l, then (m, l, -, -) [R].
 template <int D, int R>
 __device__ __forceinline__ rsrc_t slot_at(const AttnArgs& a, int head, int slot) {
-  return make_rsrc(a.part + ((int64_t)head * a.cap + slot) * (R * (D + 4)), R * (D + 4) * 4);
+  return make_rsrc(a.part + ((int64_t)head * a.held + slot) * (R * (D + 4)), R * (D + 4) * 4);
 }
 
 template <bool F16, int N>
@@ -1121,7 +1126,8 @@ constexpr int kMostSplits = 254;  // an arrival word counts to 255
 
 struct AttnPlan {
   int rows;     // a workgroup's
-  int64_t slots, target, tiles, cap;
+  int64_t slots, target, tiles;
+  int64_t cap, held;  // items a kv head can have, and partial results
   int64_t joiners;
   size_t words, bytes;
 };
@@ -1148,7 +1154,10 @@ bool plan_attention(int64_t total, int64_t batch, int64_t hq, int64_t hkv, int64
   p->target = (target + hkv - 1) / hkv < kMostSplits ? (target + hkv - 1) / hkv : kMostSplits;
   p->slots = (slots + hkv - 1) / hkv < kMostSplits ? (slots + hkv - 1) / hkv : kMostSplits;
   p->tiles = total * group / p->rows + (batch < total ? batch : total);
+  // With chunk > work / target, the sum over sequences of tiles * units / chunk stays below the target. Rounded up to whole
+  // splits that is a tile each more; of the sequences of several, at most twice as many, which are the partial results.
   p->cap = p->tiles + (units > 1 ? p->target : 0);
+  p->held = p->cap < 2 * p->target ? p->cap : 2 * p->target;
   const int64_t tiles = batch * ((rows + p->rows - 1) / p->rows);  // at the mean; with the most splits a tile can have
   const int64_t splits = units < p->slots / tiles ? units : p->slots / tiles;
   p->joiners = 0;
@@ -1158,7 +1167,7 @@ bool plan_attention(int64_t total, int64_t batch, int64_t hq, int64_t hkv, int64
   }
   if (p->cap * hkv > 0xFFFFFF) return false;  // a launch has fewer than 2^32 threads
   p->words = ((size_t)(p->tiles * hkv) * 8 + 15) / 16 * 16;
-  p->bytes = units > 1 ? p->words + (size_t)(p->cap * hkv * p->rows * (d + 4)) * sizeof(float) : 0;
+  p->bytes = units > 1 ? p->words + (size_t)(p->held * hkv * p->rows * (d + 4)) * sizeof(float) : 0;
   return true;
 }
 
@@ -1271,7 +1280,7 @@ extern "C" int aklr_tree_attention_fp8(const void* q, int64_t q_token, int64_t q
   a.pages = (int)pages;
   a.target = (int)p.target;
   a.slots = (int)p.slots;
-  a.cap = (int)p.cap;
+  a.held = (int)p.held;
   a.words = (int)p.tiles;
   a.joiners = (int)p.joiners;
   a.scale_log2 = softmax_scale * 1.44269504f;

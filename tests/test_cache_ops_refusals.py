@@ -29,6 +29,20 @@ def test_more_workgroups_than_a_launch_has_room_for(anywhere, native_lib):
         assert bool(native_lib.aklr_tree_attention_fp8_rows(batch, batch, 256, 256, 64, 16, None)) == served
 
 
+def test_attention_workspace_is_for_what_is_split(native_lib):
+    # partial results: at most as many pieces as twice the chip runs at once and half as many again (512 workgroups of 128
+    # rows: 1536), whatever the number of query tokens; beside them a word a tile
+    size, rows = native_lib.aklr_tree_attention_fp8_workspace_bytes, native_lib.aklr_tree_attention_fp8_rows
+    last = 0
+    for tokens in (1, 100, 1000, 8192, 65536, 1 << 20):
+        got = size(tokens, 2, 64, 8, 128, 1 << 17)
+        r = rows(tokens, 2, 64, 8, 128, 1 << 17, None)
+        tiles = 8 * (tokens * 8 // r + 2)
+        assert last <= got <= 1536 * r * (128 + 4) * 4 + 8 * tiles + 16
+        last = got
+    assert last < 120 << 20
+
+
 def test_attention_rows_query(native_lib):
     rows = native_lib.aklr_tree_attention_fp8_rows
     join = ctypes.c_int(-1)
