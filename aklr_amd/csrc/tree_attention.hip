@@ -151,16 +151,6 @@ __device__ __forceinline__ Item find(const AttnArgs& a, int index) {
   return r;
 }
 
-// Direct loads into LDS with the wait state the hardware asks for between a write of M0 and its use by one.
-__device__ __forceinline__ void to_lds16(const i32x4& rsrc, uint32_t lds, uint32_t voffset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voffset), "s"(rsrc)
-               : "m0");
-}
-__device__ __forceinline__ void to_lds4(const i32x4& rsrc, uint32_t lds, uint32_t voffset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(voffset), "s"(rsrc)
-               : "m0");
-}
-
 // A block table is read by scalar loads: a vector load's wait would also wait for the codes that are on their way.
 typedef const int32_t __attribute__((address_space(4))) const_i32;
 __device__ __forceinline__ const_i32* row_of(const int32_t* table, int64_t at) {
@@ -561,12 +551,12 @@ __global__ __launch_bounds__(kThreads, 2) void stream_kernel(const AttnArgs a) {
       const i32x4 k = words(kc + codes, 16 * D), v = words(vc + codes, 16 * D);
 #pragma unroll
       for (int i = 0; i < ND; ++i) {
-        to_lds16(k, to + 16 * D * h + 1024 * i, from_k[i]);
-        to_lds16(v, to + 32 * D + 16 * D * h + 1024 * i, from_v[i]);
+        lds_dma16(k, to + 16 * D * h + 1024 * i, from_k[i]);
+        lds_dma16(v, to + 32 * D + 16 * D * h + 1024 * i, from_v[i]);
       }
       if (lane < 16) {
-        to_lds4(words(ks + scales, 64), to + 64 * D + 64 * h, 4 * lane);
-        to_lds4(words(vs + scales, 64), to + 64 * D + 128 + 64 * h, 4 * lane);
+        lds_dma4(words(ks + scales, 64), to + 64 * D + 64 * h, 4 * lane);
+        lds_dma4(words(vs + scales, 64), to + 64 * D + 128 + 64 * h, 4 * lane);
       }
     };
     const bool real = is_page(x.id[0]);
@@ -878,13 +868,13 @@ __global__ __launch_bounds__(64 * W, D > 128 ? 1 : 2) void tile_kernel(const Att
       const uint32_t to = lds + slot * kStage + 16 * D * block;
 #pragma unroll
       for (int i = 0; i < ND; ++i) {
-        to_lds16(k, to + 1024 * i, from_k[i]);
-        to_lds16(v, to + kStep * D + 1024 * i, from_v[i]);
+        lds_dma16(k, to + 1024 * i, from_k[i]);
+        lds_dma16(v, to + kStep * D + 1024 * i, from_v[i]);
       }
       const uint32_t to_s = lds + slot * kStage + 2 * kStep * D + 64 * block;
       if (lane < 16) {
-        to_lds4(words(ks + scales, 64), to_s, 4 * lane);
-        to_lds4(words(vs + scales, 64), to_s + 4 * kStep, 4 * lane);
+        lds_dma4(words(ks + scales, 64), to_s, 4 * lane);
+        lds_dma4(words(vs + scales, 64), to_s + 4 * kStep, 4 * lane);
       }
       if (lane == 0) here[slot][block] = real;
     }

@@ -34,6 +34,6 @@ def test_a_wait_state_between_m0_and_a_load_into_lds(path):
 
 def test_the_statements_are_found():
     found = [code for path in SOURCES for code in statements(path.read_text())]
-    assert sum(any(INTO_LDS.search(line) for line in code) for code in found) == 6
+    assert sum(any(INTO_LDS.search(line) for line in code) for code in found) == 4
     assert list(statements('asm volatile("s_mov_b32 m0, %0\\n\\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(x));')) == [
         ["s_mov_b32 m0, %0", "buffer_load_dword %1, %2, 0 offen lds"]]
