@@ -6,7 +6,8 @@ softmax_scale=None, return_lse=False, out=None)``:
   q: bf16 or fp16 [tokens, q_heads, head_dim], query tokens ``starts[b]`` to ``starts[b + 1] - 1`` (int32 [batch + 1],
   ascending) are sequence b's; q_heads is a multiple of the cache's kv_heads, head h attends kv head
   h // (q_heads // kv_heads). Their keys and values are already in the cache, as the last of the sequence's
-  ``seq_lens[b]`` (int32) positions; ``block_table`` (int32 [batch, columns]) names its pages in order.
+  ``seq_lens[b]`` (int32) positions; ``block_table`` (int32 [batch, columns]) names its pages in order. A length past
+  the table's columns counts as what they hold; positions in pages that the cache does not have are not seen.
   Every query token sees all positions before its sequence's query tokens. Of those, query token i (counted over q)
   sees the j-th where ``tree_mask[i, j]`` (bool or uint8 [tokens, columns], columns at least the most query tokens a
   sequence has), or without a mask those up to itself: one token a sequence is decode, several a chunk of a prompt or a
@@ -18,7 +19,8 @@ softmax_scale=None, return_lse=False, out=None)``:
   Scores, their maxima and sums are fp32. A position's weight times its value scale is rounded before the product with
   its codes: to 16 bits in calls of up to 32 rows (query tokens x q_heads // kv_heads) a sequence on the mean, in calls of
   few rows altogether, and for fp16 queries always; to 8 bits (bf16, half a step of the output's type) for bf16 queries in
-  larger calls. Such a weight may reach 2^20, so values past 2^100 can overflow, for both types.
+  larger calls. Such a weight may reach 2^20, so values past 2^100 can overflow, and
+  make a row NaN, for both types.
 
   Returns q's shape and dtype, with ``return_lse`` also the fp32 [tokens, q_heads] log of each softmax's sum, by which
   parts of a context can be joined. A token that sees nothing gets zeros and -inf. Nothing of a position that a token

@@ -111,7 +111,7 @@ struct VecArgs {
 // infinity gets zero codes under a NaN scale, so it reads as NaN throughout and no NaN code enters the cache.
 //
 // Bound by memory where there are many tokens (figures at launch_vec), by the launch and one chain of loads where few:
-// 3.2 us for 64 tokens of 8 heads written, 3.4 for 16 tokens of 129 heads rotated, 3.9 for 8 of 80 rotated and written.
+// 3.4 us for 64 tokens of 8 heads written, 3.5 for 16 tokens of 129 heads rotated, 3.9 for 8 of 80 rotated and written.
 template <typename T, int D, bool ROT, bool WRITE>
 __global__ __launch_bounds__(kThreads) void vec_kernel(const VecArgs a, const int head_dim) {
   const int dim = D ? D : head_dim;
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(kThreads) void vec_kernel(const VecArgs a, const in
 }
 
 // How many tokens a workgroup takes and how many workgroups share them: one item a lane, which is all that a write alone
-// needs (8191 tokens of 8 heads of 256: 22.5 us, 5.1 TB/s of reads and writes; a large copy reaches 5.2). With a rotation,
+// needs (8191 tokens of 8 heads of 256: 22.9 us, 4.4 TB/s of reads and writes; a large copy reaches 5.2). With a rotation,
 // where that makes many workgroups, one takes all heads of a token, so that its angles are worked out once: 8192 tokens of
 // 32 + 8 heads of 128 rotated and written in 43.9 us instead of 49.9 (two tokens a workgroup 43.0, four 43.9), 5003 rotated
 // in 18.5 instead of 19.7 (two 19.7, four 21.7).

@@ -12,9 +12,10 @@
 // does not, nor the weights of a row that one position draws to itself. Up to 32 rows, where memory is the bound, and for
 // fp16 queries they are two bf16 pieces (what is lost is at most 2^-16 of a term); for bf16 ones in tiles of more rows,
 // which the products bound, they are one (2^-8, half a step of the output's type): 2048 tokens of two prompts over 8192 take
-// 581 us with one and 731 with two. (One fp16 piece, whose range needs the scales in the codes' conversions, took 742.) Scores, maxima, sums and outputs
-// stay in fp32. Products of codes with e4m3 pieces of q would need no conversions of keys, but a chain of them sums to
-// 2^-15 of its size on this hardware (bf16 and fp16 products to 2^-23), which a log of a sum shows.
+// 581 us with one and 731 with two. (One fp16 piece, whose range needs the scales in the codes' conversions, took 742.)
+// Scores, maxima, sums and outputs stay in fp32. Products of codes with e4m3 pieces of q would need no conversions of
+// keys, but a chain of them sums to 2^-15 of its size on this hardware (bf16 and fp16 products to 2^-23), which a log of a
+// sum shows.
 #include "common.h"
 
 AKLR_SCALAR_FP32_BEGIN
@@ -778,9 +779,10 @@ __device__ __forceinline__ f32x16 mfma16(const u32x4& a, const u32x4& b, const f
 }
 
 // Many rows: bound by the vector unit's issue beside the matrix unit's time. A step of 32 rows and tokens is 16 products
-// (512 cycles) and 185 vector instructions, 64 of them conversions; counters show the vector unit half and the matrix unit a
-// third of the time busy, two waves on a SIMD. 2048 tokens of each of two prompts over 8192, 8 kv heads of 128, group 4:
-// 568 to 593 us by the card, 833 to 870 TFLOP/s; without the raised priority of the second products 30 us more.
+// (512 cycles) and about 195 vector instructions, 64 of them conversions; counters show the vector unit's issue two thirds
+// and the matrix unit 37 % of the time busy, two waves on a SIMD. 2048 tokens of each of two prompts over 8192, 8 kv heads
+// of 128, group 4: 577 to 592 us, 834 to 856 TFLOP/s; without the raised priority of the second products 30 us more. fp16
+// queries, whose weights are two bf16 (24 products): 735 us.
 //
 // The W waves of a workgroup take 32 rows each and share a ring of S stages of 64 tokens' codes in LDS, which
 // come straight from memory, 16 tokens a load. One barrier a stage: a wave waits for its own loads, the barrier for the

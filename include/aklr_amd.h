@@ -320,8 +320,8 @@ int aklr_kv_cache_read_fp8(const void* k_codes, const void* v_codes, const float
  * over q, j < mask_cols; others are not seen), or, with mask NULL, those up to its own. out[token, head] = softmax over
  * the positions seen of softmax_scale * (q . k), times v; lse (may be NULL): log of the sum of the exponentials. A token
  * that sees nothing gets zeros and -infinity. What a token does not see does not reach it, NaN included. Query tokens
- * outside every sequence keep what out and lse hold. Positions past the block table's columns, and pages outside
- * [0, pages), are seen by none. starts ascend.
+ * outside every sequence keep what out and lse hold. A length past the block table's columns counts as what they hold;
+ * positions in pages outside [0, pages) are seen by none. starts ascend.
  * q: [total_q, q_heads, head_dim] bf16 or fp16 (dtype), strides in elements, multiples of 8; out: the same dtype,
  * contiguous; head h attends kv head h / (q_heads / kv_heads). Weights are rounded to 16 bits, and to 8 (one bf16) for
  * bf16 queries where aklr_tree_attention_fp8_rows is 64 or 128. lse: fp32 [total_q, q_heads]. mask: bytes, rows
