@@ -781,7 +781,7 @@ __device__ __forceinline__ f32x16 mfma16(const u32x4& a, const u32x4& b, const f
 // Many rows: bound by the vector unit's issue beside the matrix unit's time. A step of 32 rows and tokens is 16 products
 // (512 cycles) and about 195 vector instructions, 64 of them conversions; counters show the vector unit's issue two thirds
 // and the matrix unit 37 % of the time busy, two waves on a SIMD. 2048 tokens of each of two prompts over 8192, 8 kv heads
-// of 128, group 4: 577 to 592 us, 834 to 856 TFLOP/s; without the raised priority of the second products 30 us more. fp16
+// of 128, group 4: 577 to 606 us by the card, 815 to 856 TFLOP/s; without the raised priority of the second products 30 us more. fp16
 // queries, whose weights are two bf16 (24 products): 735 us.
 //
 // The W waves of a workgroup take 32 rows each and share a ring of S stages of 64 tokens' codes in LDS, which
