@@ -93,6 +93,33 @@ SIGNATURES: dict[str, tuple] = {
         [_vp, _c_i64, _c_i64, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64,
          _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float, _c_int, _vp, _c_size, _vp],
     ),
+    "aklr_kv_cache_copy_pages_fp8": (
+        _c_int,
+        [_vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp],
+    ),
+    "aklr_kv_cache_compact_fp8_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64, _c_i64]),
+    "aklr_kv_cache_compact_fp8": (
+        _c_int,
+        [_vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64, _vp,
+         _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _vp, _c_size, _vp],
+    ),
+    "aklr_kv_cache_update_pages_workspace_bytes": (_c_size, [_c_i64]),
+    "aklr_kv_cache_update_pages": (
+        _c_int,
+        [_vp, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _vp, _c_i64, _c_i64, _vp, _vp, _vp, _vp, _vp, _c_size, _vp],
+    ),
+    "aklr_verify_drafts_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64]),
+    "aklr_verify_drafts": (
+        _c_int,
+        [_vp, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_int, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _vp, _vp, _vp,
+         _c_int, _vp, _c_size, _vp],
+    ),
+    "aklr_lora_project_workspace_bytes": (_c_size, [_c_i64] * 5),
+    "aklr_lora_project": (
+        _c_int,
+        [_vp, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_int, _vp, _vp, _vp, _c_i64, _vp, _c_i64, _c_i64,
+         _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _vp, _c_size, _vp],
+    ),
     "aklr_probe_hbm_read": (_c_int, [_vp, _c_i64, _vp, _c_int, _c_int, _vp]),
 }
 

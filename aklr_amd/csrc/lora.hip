@@ -1,0 +1,519 @@
+// Low-rank adapters of many requests beside a projection that all share: out[t] = base[t] + s_a (x[t] A_a^T) B_a^T with
+// a = adapters[t], A_a [rank, K], B_a [N, rank]. gfx950 only.
+//
+// Two launches over tiles of up to 16 * MT tokens of one adapter, so that its weights are read once a tile:
+//   shrink  v[t, r] = sum_k x[t, k] A[r, k], K split over workgroups (fp32 parts in the workspace) and over a workgroup's
+//           four waves, on 16x16x32 products with the adapter's rows as one operand and tokens as the other;
+//   expand  the parts added in their order, v as two 16-bit pieces (hi + lo: what is left of v's rounding is 2^-17 of it
+//           for bf16, 2^-23 for fp16), products with B's rows, base added in fp32, one rounding.
+// Up to 256 tokens a workgroup finds its tile by itself, from all tokens' adapters; more are put in the adapters' order by a
+// launch before. A token's row of a tile changes no result: the products' columns do not meet.
+//
+// Bound by memory: decode by the adapters' weights, prompts by x, base and out (figures at plan_lora).
+#include "common.h"
+
+AKLR_SCALAR_FP32_BEGIN
+
+namespace aklr {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kThreads = 256;
+constexpr int kScan = 256;       // tokens that a workgroup looks through by itself
+constexpr int kMostAdapters = 4096;  // what the sort counts in LDS
+
+template <bool F16>
+__device__ __forceinline__ f32x4 product(const u32x4& a, const u32x4& b, const f32x4& c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+struct Tile {
+  int adapter;  // -1: tokens without one
+  int first;    // in the order of adapters
+  int count;
+  int pad;
+};
+
+struct LoraArgs {
+  const uint16_t *x, *a, *b, *base;
+  uint16_t* out;
+  int64_t x_row, a_adapter, a_row, b_adapter, b_row, base_row, out_row;  // elements
+  const void* ids;
+  const float* scales;
+  const int32_t* ranks;
+  float* part;  // [splits][tokens][rank rounded up to the products' rows]
+  int32_t* order;
+  Tile* tiles;
+  int32_t* tile_count;
+  int tokens, k, n, rank, adapters, ids64, splits, k_split, n_group, copies;
+};
+
+__device__ __forceinline__ int adapter_of(const LoraArgs& a, int t) {
+  const int64_t i = a.ids64 ? static_cast<const int64_t*>(a.ids)[t] : (int64_t) static_cast<const int32_t*>(a.ids)[t];
+  return i < 0 || i >= a.adapters ? -1 : (int)i;
+}
+
+__device__ __forceinline__ int rank_of(const LoraArgs& a, int adapter) {
+  if (adapter < 0) return 0;
+  return a.ranks ? min(max(a.ranks[adapter], 0), a.rank) : a.rank;
+}
+
+// The workgroup's tile: its tokens in `rows`, the first repeated behind them. False: there is none. With few tokens, `id`
+// is a token, and a tile begins at each of an adapter's tokens that has a whole number of tiles' tokens before it.
+template <int TM>
+__device__ __forceinline__ bool find_tile(const LoraArgs& a, int id, int (&rows)[TM], int* words, int& adapter, int& count) {
+  if (a.tokens > kScan) {
+    if (id >= *a.tile_count) return false;
+    const Tile t = a.tiles[id];
+    adapter = t.adapter;
+    count = t.count;
+    if ((int)threadIdx.x < TM) rows[threadIdx.x] = a.order[t.first + ((int)threadIdx.x < t.count ? threadIdx.x : 0)];
+    __syncthreads();
+    return true;
+  }
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int own = t < a.tokens ? adapter_of(a, t) : -2;
+  adapter = adapter_of(a, id);
+  const uint64_t same = __ballot(own == adapter);
+  if (lane == 0) words[wave] = __popcll(same);
+  __syncthreads();
+  int before = __popcll(same & ((1ull << lane) - 1)), all = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) {
+    before += w < wave ? words[w] : 0;
+    all += words[w];
+  }
+  if (t == id) words[4] = before;
+  __syncthreads();
+  const int first = words[4];
+  if (first % TM) return false;
+  count = min(TM, all - first);
+  if (own == adapter && before >= first && before < first + count) {
+    rows[before - first] = t;
+    if (before == first)
+      for (int i = count; i < TM; ++i) rows[i] = t;
+  }
+  __syncthreads();
+  return true;
+}
+
+// Tokens in the order of their adapters, those without one last, and the tiles of that order: one workgroup. Within an
+// adapter the order is that of arrival; no result depends on it. Consecutive tokens are mostly of one adapter: a wave whose
+// tokens all are counts them at once.
+constexpr int kSort = 1024;
+__global__ __launch_bounds__(kSort) void sort_kernel(const LoraArgs a, const int tm) {
+  extern __shared__ int32_t count[];  // [adapters + 1], then where each one's next token goes
+  __shared__ int sums[kSort / 64], tile_sums[kSort / 64];
+  const int groups = a.adapters + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int32_t* const next = count + groups;
+  for (int g = threadIdx.x; g < groups; g += kSort) count[g] = 0;
+  __syncthreads();
+  const int last = (a.tokens + kSort - 1) / kSort * kSort;
+  for (int t = threadIdx.x; t < last; t += kSort) {
+    int g = t < a.tokens ? adapter_of(a, t) : -2;
+    g = g == -1 ? a.adapters : g;
+    const int g0 = __builtin_amdgcn_readfirstlane(g);
+    const uint64_t same = __ballot(g == g0);
+    if (g0 >= 0 && lane == 0) atomicAdd(count + g0, __popcll(same));
+    if (g >= 0 && g != g0) atomicAdd(count + g, 1);
+  }
+  __syncthreads();
+  int tokens_before = 0, tiles_before = 0;
+  for (int g0 = 0; g0 < groups; g0 += kSort) {
+    const int g = g0 + threadIdx.x, c = g < groups ? count[g] : 0, tiles = (c + tm - 1) / tm;
+    int s = c, u = tiles;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int y = __shfl_up(s, d, 64), z = __shfl_up(u, d, 64);
+      if (lane >= d) s += y, u += z;
+    }
+    __syncthreads();
+    if (lane == 63) sums[wave] = s, tile_sums[wave] = u;
+    __syncthreads();
+    int at = tokens_before + s - c, tile = tiles_before + u - tiles;
+#pragma unroll
+    for (int w = 0; w < kSort / 64; ++w) {
+      at += w < wave ? sums[w] : 0;
+      tile += w < wave ? tile_sums[w] : 0;
+      tokens_before += sums[w];
+      tiles_before += tile_sums[w];
+    }
+    if (g < groups) {
+      next[g] = at;
+      for (int i = 0; i < tiles; ++i) a.tiles[tile + i] = {g == a.adapters ? -1 : g, at + i * tm, min(tm, c - i * tm), 0};
+    }
+  }
+  if (threadIdx.x == 0) *a.tile_count = tiles_before;
+  __syncthreads();
+  for (int t = threadIdx.x; t < last; t += kSort) {
+    int g = t < a.tokens ? adapter_of(a, t) : -2;
+    g = g == -1 ? a.adapters : g;
+    const int g0 = __builtin_amdgcn_readfirstlane(g);
+    const uint64_t same = __ballot(g == g0);
+    int at = 0;
+    if (g0 >= 0 && lane == 0) at = atomicAdd(next + g0, __popcll(same));
+    at = __builtin_amdgcn_readfirstlane(at) + __popcll(same & ((1ull << lane) - 1));
+    if (g >= 0 && g != g0) at = atomicAdd(next + g, 1);
+    if (g >= 0) a.order[at] = t;
+  }
+}
+
+// v's part of a tile and a range of K. A wave takes 64 of K at a time (whole lines of x's and A's rows), every fourth such
+// piece; NR * 16 rows of A against MT * 16 tokens, both straight from memory: a lane's 16 bytes of a row are its share of an
+// operand. The four waves' sums meet in LDS, in a fixed order.
+template <int MT, int NR, bool F16>
+__global__ __launch_bounds__(kThreads) void shrink_kernel(const LoraArgs a) {
+  constexpr int TM = 16 * MT;
+  __shared__ int rows[TM], words[5];
+  __shared__ f32x4 meet[2][NR][MT][64];
+  int adapter, count;
+  if (!find_tile<TM>(a, blockIdx.x, rows, words, adapter, count)) return;
+  const int rank = rank_of(a, adapter);
+  if (rank == 0) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
+  const int k0 = blockIdx.y * a.k_split, k1 = min(k0 + a.k_split, a.k);
+  const uint16_t* xr[MT];
+  const uint16_t* ar[NR];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) xr[m] = a.x + rows[m * 16 + li] * a.x_row;
+#pragma unroll
+  for (int r = 0; r < NR; ++r) ar[r] = a.a + adapter * a.a_adapter + min(r * 16 + li, rank - 1) * a.a_row;  // repeated rows are not used
+  const int used = (rank + 15) / 16;
+  struct Piece {
+    u32x4 x[2][MT], w[2][NR];
+  };
+  const auto fetch = [&](int k, Piece& p) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = k + h * 32 + g * 8;
+      const bool on = at < k1;  // k % 8 == 0: eight values are inside or past the end
+#pragma unroll
+      for (int r = 0; r < NR; ++r) p.w[h][r] = on && r < used ? ld16_nt(ar[r] + at) : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int m = 0; m < MT; ++m) p.x[h][m] = on ? ld16(xr[m] + at) : u32x4{0, 0, 0, 0};
+    }
+  };
+  f32x4 acc[NR][MT] = {};
+  Piece now;
+  int k = k0 + wave * 64;
+  if (k < k1) fetch(k, now);
+  while (k < k1) {
+    Piece next;
+    const int after = k + 256;
+    if (after < k1) fetch(after, next);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[r][m] = product<F16>(now.w[h][r], now.x[h][m], acc[r][m]);
+    now = next;
+    k = after;
+  }
+  if (wave >= 2) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) meet[wave - 2][r][m][lane] = acc[r][m];
+  }
+  __syncthreads();
+  if (wave < 2) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[r][m] += meet[wave][r][m][lane];
+  }
+  __syncthreads();
+  if (wave == 1) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) meet[0][r][m][lane] = acc[r][m];
+  }
+  __syncthreads();
+  if (wave == 0) {  // a lane has rows 16 r + 4 g .. + 3 of token li
+    float* const to = a.part + (int64_t)blockIdx.y * a.tokens * (NR * 16);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      if (m * 16 + li >= count) continue;
+      const int64_t row = (int64_t)rows[m * 16 + li] * (NR * 16) + 4 * g;
+#pragma unroll
+      for (int r = 0; r < NR; ++r) *reinterpret_cast<f32x4*>(to + row + 16 * r) = acc[r][m] + meet[0][r][m][lane];
+    }
+  }
+}
+
+// Two 16-bit pieces of x: hi, and what hi's rounding left.
+template <bool F16>
+__device__ __forceinline__ void pieces(float x, uint32_t& hi, uint32_t& lo) {
+  if constexpr (F16) {
+    const _Float16 h = (_Float16)x;
+    hi = __builtin_bit_cast(uint16_t, h);
+    lo = f32_to_f16_bits(__builtin_isfinite(x) ? x - (float)h : 0.0f);
+  } else {
+    hi = f32_to_bf16_bits(x);
+    lo = f32_to_bf16_bits((hi & 0x7F80u) != 0x7F80u ? x - bf16_lo(hi) : 0.0f);
+  }
+}
+
+template <bool F16>
+__device__ __forceinline__ float from16(uint32_t bits) {
+  if constexpr (F16)
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+  else
+    return bf16_lo(bits);
+}
+
+// The outputs of a tile for n_group columns. A wave takes 64 columns at a time, four products' rows: row i of the q-th is
+// column 16 (i / 4) + 4 q + i % 4, so that a lane ends with 16 columns side by side of one token, and a token's four lanes
+// with a whole line of base and out.
+template <int MT, int NR, bool F16>
+__global__ __launch_bounds__(kThreads) void expand_kernel(const LoraArgs a) {
+  constexpr int TM = 16 * MT, R = 16 * NR, kSteps = (R + 31) / 32, kRow = kSteps * 32 + 8;  // a row of pieces: 16 bytes more
+  __shared__ int rows[TM], words[5];
+  __shared__ __align__(16) uint16_t piece[2][TM][kRow];
+  __shared__ int power[TM];
+  int adapter, count;
+  if (!find_tile<TM>(a, blockIdx.x, rows, words, adapter, count)) return;
+  const int rank = rank_of(a, adapter);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
+  const int c0 = blockIdx.y * a.n_group, c1 = min(c0 + a.n_group, a.n);
+  if (rank == 0) {
+    if (!a.copies) return;
+    for (int i = 0; i < count; ++i)
+      for (int c = c0 + 8 * threadIdx.x; c < c1; c += 8 * kThreads)
+        *reinterpret_cast<u32x4*>(a.out + rows[i] * a.out_row + c) = ld16(a.base + rows[i] * a.base_row + c);
+    return;
+  }
+  constexpr int kLanes = R / 4;  // of a token: four values each
+#pragma unroll
+  for (int i = 0; i < (TM * kLanes + kThreads - 1) / kThreads; ++i) {
+    const int id = i * kThreads + threadIdx.x, t = id / kLanes, r = id % kLanes * 4;
+    if (TM * kLanes % kThreads != 0 && t >= TM) break;
+    f32x4 v = {0, 0, 0, 0};
+    if (t < count && r < rank) {
+      const float* from = a.part + (int64_t)rows[t] * R + r;
+      const int64_t step = (int64_t)a.tokens * R;
+      int s = 0;
+      for (; s + 4 <= a.splits; s += 4) {
+        f32x4 y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = *reinterpret_cast<const f32x4*>(from + (s + e) * step);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v += y[e];
+      }
+      for (; s < a.splits; ++s) v += *reinterpret_cast<const f32x4*>(from + s * step);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (r + e >= rank) v[e] = 0.0f;
+    }
+    if constexpr (F16) {  // fp16 has no room for every v: the largest of a token's becomes 0.5 to 1, by a power of two
+      float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+      for (int d = 1; d < kLanes; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
+      const int e = top > 0.0f && top < __builtin_inff() ? __builtin_amdgcn_frexp_expf(top) : 0;
+      if (r == 0) power[t] = e;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = __builtin_amdgcn_ldexpf(v[j], -e);
+    }
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) pieces<F16>(v[e], hi[e], lo[e]);
+    *reinterpret_cast<u32x2*>(&piece[0][t][r]) = u32x2{hi[0] | hi[1] << 16, hi[2] | hi[3] << 16};
+    *reinterpret_cast<u32x2*>(&piece[1][t][r]) = u32x2{lo[0] | lo[1] << 16, lo[2] | lo[3] << 16};
+    if (R < 32) {  // the products' K is 32
+      *reinterpret_cast<u32x2*>(&piece[0][t][r + R]) = u32x2{0, 0};
+      *reinterpret_cast<u32x2*>(&piece[1][t][r + R]) = u32x2{0, 0};
+    }
+  }
+  __syncthreads();
+  const float scale = a.scales ? a.scales[adapter] : 1.0f;
+  const int steps = (rank + 31) / 32;
+  for (int c = c0 + wave * 64; c < c1; c += kThreads) {
+    const int col = c + g * 16;  // the lane's columns
+    u32x4 old[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (m * 16 + li < count && col + 8 * h < c1) old[m][h] = ld16_nt(a.base + rows[m * 16 + li] * a.base_row + col + 8 * h);
+    f32x4 acc[4][MT] = {};
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      if (s >= steps) break;
+      const int r0 = s * 32 + g * 8;
+      u32x4 w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = min(c + (li >> 2) * 16 + q * 4 + (li & 3), a.n - 1);  // columns past the end are not stored
+        w[q] = r0 < rank ? ld16(a.b + adapter * a.b_adapter + n * a.b_row + r0) : u32x4{0, 0, 0, 0};
+        if (r0 < rank && r0 + 8 > rank) {  // what lies behind the rank may be anything
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (r0 + e >= rank) w[q][e / 2] &= e % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const u32x4 hi = *reinterpret_cast<const u32x4*>(&piece[0][m * 16 + li][r0]);
+        const u32x4 lo = *reinterpret_cast<const u32x4*>(&piece[1][m * 16 + li][r0]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[q][m] = product<F16>(w[q], lo, acc[q][m]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[q][m] = product<F16>(w[q], hi, acc[q][m]);
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      if (m * 16 + li >= count) continue;
+      const int e = F16 ? power[m * 16 + li] : 0;
+      uint16_t* const to = a.out + rows[m * 16 + li] * a.out_row + col;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (col + 8 * h >= c1) continue;
+        u32x4 word;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float y[2];
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            const int at = 8 * h + 2 * j + z;
+            float d = acc[at / 4][m][at % 4] * scale;
+            if constexpr (F16) d = __builtin_amdgcn_ldexpf(d, e);
+            y[z] = from16<F16>(z ? old[m][h][j] >> 16 : old[m][h][j] & 0xFFFFu) + d;
+          }
+          word[j] = pack_out2(y[0], y[1], F16 ? AKLR_OUT_F16 : AKLR_OUT_BF16);
+        }
+        __builtin_nontemporal_store(word, reinterpret_cast<u32x4*>(to + 8 * h));
+      }
+    }
+  }
+}
+
+}  // namespace aklr
+
+using namespace aklr;
+
+namespace {
+
+struct Plan {
+  int mt, nr;         // tiles of 16 tokens, of 16 rank rows
+  int64_t tiles;      // workgroups along x: the tokens where they look for their tiles, else the most tiles there can be
+  int64_t splits, k_split, n_group;
+  size_t order, tile, part, bytes;  // offsets in the workspace
+};
+
+int64_t up(int64_t v, int64_t q) { return (v + q - 1) / q * q; }
+
+Plan plan_lora(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapters) {
+  Plan p{};
+  p.nr = rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8;
+  const bool sorts = tokens > kScan;
+  p.mt = !sorts ? 1 : tokens < 2048 ? 2 : 4;
+  const int64_t tm = 16 * p.mt, groups = adapters + 1 < tokens ? adapters + 1 : tokens;
+  const int64_t most = (tokens + tm - 1) / tm + groups;  // sum of ceil(c / tm) over groups of c tokens
+  p.tiles = sorts ? most : tokens;
+  const int64_t real = most < tokens ? most : tokens;
+  int64_t splits = (1024 + real - 1) / real;
+  if (splits > (k + 511) / 512) splits = (k + 511) / 512;
+  p.k_split = up((k + splits - 1) / splits, 256);
+  p.splits = (k + p.k_split - 1) / p.k_split;
+  int64_t groups_n = (n + 255) / 256, loops = 1;
+  while (loops < 4 && real * ((groups_n + loops - 1) / loops) > 2048) loops *= 2;
+  p.n_group = 256 * loops;
+  size_t at = 0;
+  p.order = at;
+  if (sorts) at += up(4 * tokens, 256);
+  p.tile = at;
+  if (sorts) at += up(16 * (most + 1), 256);
+  p.part = at;
+  p.bytes = at + 4 * (size_t)(p.splits * tokens * 16 * p.nr);
+  return p;
+}
+
+bool sizes_ok(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapters) {
+  return tokens >= 1 && tokens <= (1 << 20) && k >= 8 && k <= 65536 && k % 8 == 0 && n >= 8 && n <= 262144 && n % 8 == 0 &&
+         rank >= 8 && rank <= 128 && rank % 8 == 0 && adapters >= 1 && adapters <= kMostAdapters;
+}
+
+bool row_ok(const void* p, int64_t stride, int64_t least) { return p && aklr_aligned16(p) && stride % 8 == 0 && stride >= least; }
+
+}  // namespace
+
+extern "C" size_t aklr_lora_project_workspace_bytes(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapters) {
+  return sizes_ok(tokens, k, n, rank, adapters) ? plan_lora(tokens, k, n, rank, adapters).bytes : 0;
+}
+
+extern "C" int aklr_lora_project(const void* x, int64_t x_stride, const void* a, int64_t a_adapter_stride,
+                                 int64_t a_row_stride, const void* b, int64_t b_adapter_stride, int64_t b_row_stride,
+                                 const void* adapters, int adapters_64, const float* scales, const int32_t* ranks,
+                                 const void* base, int64_t base_stride, void* out, int64_t out_stride, int64_t tokens,
+                                 int64_t k, int64_t n, int64_t rank, int64_t adapter_count, int dtype, void* workspace,
+                                 size_t workspace_bytes, hipStream_t stream) {
+  if (dtype != AKLR_OUT_BF16 && dtype != AKLR_OUT_F16) return AKLR_ERR_UNSUPPORTED;
+  if (tokens == 0) return AKLR_OK;
+  if (!sizes_ok(tokens, k, n, rank, adapter_count)) return AKLR_ERR_INVALID_ARGUMENT;
+  if (!row_ok(x, x_stride, 0) || !row_ok(a, a_row_stride, 0) || a_adapter_stride % 8 || !row_ok(b, b_row_stride, 0) ||
+      b_adapter_stride % 8 || !row_ok(base, base_stride, 0) || !row_ok(out, out_stride, tokens > 1 ? n : 0) || !adapters)
+    return AKLR_ERR_INVALID_ARGUMENT;
+  const Plan p = plan_lora(tokens, k, n, rank, adapter_count);
+  if (!workspace || !aklr_aligned16(workspace) || workspace_bytes < p.bytes) return AKLR_ERR_WORKSPACE;
+  uint8_t* const ws = static_cast<uint8_t*>(workspace);
+  LoraArgs g{};
+  g.x = static_cast<const uint16_t*>(x);
+  g.a = static_cast<const uint16_t*>(a);
+  g.b = static_cast<const uint16_t*>(b);
+  g.base = static_cast<const uint16_t*>(base);
+  g.out = static_cast<uint16_t*>(out);
+  g.x_row = x_stride;
+  g.a_adapter = a_adapter_stride;
+  g.a_row = a_row_stride;
+  g.b_adapter = b_adapter_stride;
+  g.b_row = b_row_stride;
+  g.base_row = base_stride;
+  g.out_row = out_stride;
+  g.ids = adapters;
+  g.scales = scales;
+  g.ranks = ranks;
+  g.part = reinterpret_cast<float*>(ws + p.part);
+  g.order = reinterpret_cast<int32_t*>(ws + p.order);
+  g.tile_count = reinterpret_cast<int32_t*>(ws + p.tile);
+  g.tiles = reinterpret_cast<Tile*>(ws + p.tile) + 1;
+  g.tokens = (int)tokens;
+  g.k = (int)k;
+  g.n = (int)n;
+  g.rank = (int)rank;
+  g.adapters = (int)adapter_count;
+  g.ids64 = adapters_64;
+  g.splits = (int)p.splits;
+  g.k_split = (int)p.k_split;
+  g.n_group = (int)p.n_group;
+  g.copies = base != out;
+  if (tokens > kScan) {
+    hipLaunchKernelGGL(sort_kernel, dim3(1), dim3(kSort), 8 * (adapter_count + 1), stream, g, 16 * p.mt);
+    AKLR_LAUNCH_CHECK();
+  }
+  const dim3 shrink((unsigned)p.tiles, (unsigned)p.splits), expand((unsigned)p.tiles, (unsigned)((n + p.n_group - 1) / p.n_group));
+  const auto go = [&](auto mt, auto nr, auto f16) -> int {
+    constexpr int MT = decltype(mt)::value, NR = decltype(nr)::value;
+    constexpr bool F16 = decltype(f16)::value;
+    hipLaunchKernelGGL((shrink_kernel<MT, NR, F16>), shrink, dim3(kThreads), 0, stream, g);
+    AKLR_LAUNCH_CHECK();
+    hipLaunchKernelGGL((expand_kernel<MT, NR, F16>), expand, dim3(kThreads), 0, stream, g);
+    AKLR_LAUNCH_CHECK();
+    return AKLR_OK;
+  };
+  const auto by_rank = [&](auto mt, auto f16) -> int {
+    return p.nr == 1 ? go(mt, IC<1>{}, f16) : p.nr == 2 ? go(mt, IC<2>{}, f16) : p.nr == 4 ? go(mt, IC<4>{}, f16) : go(mt, IC<8>{}, f16);
+  };
+  const auto by_rows = [&](auto f16) -> int {
+    return p.mt == 1 ? by_rank(IC<1>{}, f16) : p.mt == 2 ? by_rank(IC<2>{}, f16) : by_rank(IC<4>{}, f16);
+  };
+  return dtype == AKLR_OUT_F16 ? by_rows(IC<1>{}) : by_rows(IC<0>{});
+}
+
+AKLR_SCALAR_FP32_END

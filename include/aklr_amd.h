@@ -348,6 +348,85 @@ int aklr_tree_attention_fp8(const void* q, int64_t q_token_stride, int64_t q_hea
                             size_t workspace_bytes, hipStream_t stream);
 
 /*
+ * Pages of the cache of aklr_kv_cache_write_fp8: src[i] onto dst[i], all four tensors (indices int32, or int64 with
+ * indices_64, [count]). Pairs of which one is outside [0, pages) are skipped. The pages of dst are distinct and none of src;
+ * of others the content is not defined.
+ */
+int aklr_kv_cache_copy_pages_fp8(void* k_codes, void* v_codes, float* k_scales, float* v_scales, int64_t k_page,
+                                 int64_t v_page, int64_t ks_page, int64_t vs_page, const void* src, const void* dst,
+                                 int indices_64, int64_t count, int64_t kv_heads, int64_t head_dim, int64_t pages,
+                                 int64_t page_size, hipStream_t stream);
+
+/*
+ * Kept positions of a paged cache moved together: of the last T = starts[b + 1] - starts[b] of seq_lens[b] positions, number
+ * path[b * path_stride + i] becomes number i, for i < min(counts[b], most). path ascends. Entries outside [0, T), and those of
+ * which the source or the place lies in a page that the cache does not have, are skipped. batch <= 65536,
+ * table_cols * page_size <= 2^28. Workspace: aklr_kv_cache_compact_fp8_workspace_bytes(batch, most, kv_heads, head_dim), any
+ * content, up to 128 MiB; none for most <= 64.
+ */
+size_t aklr_kv_cache_compact_fp8_workspace_bytes(int64_t batch, int64_t most, int64_t kv_heads, int64_t head_dim);
+int aklr_kv_cache_compact_fp8(void* k_codes, void* v_codes, float* k_scales, float* v_scales, int64_t k_page,
+                              int64_t v_page, int64_t ks_page, int64_t vs_page, const int32_t* block_table,
+                              int64_t table_stride, int64_t table_cols, const int32_t* seq_lens, const int32_t* starts,
+                              const int32_t* path, int64_t path_stride, int64_t most, const int32_t* counts, int64_t batch,
+                              int64_t kv_heads, int64_t head_dim, int64_t pages, int64_t page_size, void* workspace,
+                              size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * Which pages each sequence holds next. page_refs [pages] counts the holders of each page (0: free), updated in place.
+ * Sequence b held the first ceil(lens[b] / page_size) entries of its row of block_table; it goes on from the first
+ * min(lens[p], new_lens[b]) positions of p = parents[b] (NULL: b; outside [0, batch): none) and gets pages up to new_lens[b]
+ * (lengths are cut to [0, table_cols * page_size]). Whole kept pages are shared. A page kept in part stays with the lowest
+ * sequence that keeps a part of it if no other holder is left, else it is copied: src[b], dst[b] name the pages to copy (-1:
+ * none). New pages are the lowest free ones in the order of sequences and columns. new_table [batch, table_cols] contiguous,
+ * -1 behind what is held; granted[b]: the positions sequence b has pages for. Entries outside [0, pages) hold nothing and
+ * stay -1. batch <= 65536, pages * page_size < 2^31, table_cols * page_size <= 2^28, batch * table_cols < 2^31. Workspace:
+ * aklr_kv_cache_update_pages_workspace_bytes(batch), any content.
+ */
+size_t aklr_kv_cache_update_pages_workspace_bytes(int64_t batch);
+int aklr_kv_cache_update_pages(int32_t* page_refs, int64_t pages, const int32_t* block_table, int64_t table_stride,
+                               int64_t table_cols, const int32_t* lens, const int32_t* new_lens, const int32_t* parents,
+                               int64_t batch, int64_t page_size, int32_t* new_table, int32_t* granted, int32_t* src,
+                               int32_t* dst, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * Drafted tokens against the target's probabilities. Query tokens starts[b] .. starts[b + 1] - 1 are sequence b's: the last
+ * one that stands, then drafts, each after its parent (parents[i], counted within the sequence, before i; NULL: the one
+ * before). At a node with target row p and draft row q its drafts are tried in order, from W = p, S = 1: token x stands if
+ * accept_uniforms[i] * S * q(x) < W(x), else W = max(W - S q, 0), S = sum(W); with draft_probs NULL if
+ * accept_uniforms[i] * S < W(x), else S -= W(x), W(x) = 0. Where none stands, the next token is the least v with
+ * W(0) + ... + W(v) > sample_uniforms[b] * sum(W); p itself where sum(W) is 0, -1 where p's is too. In 64 bits.
+ * target_probs, draft_probs: rows of vocab values of dtype (AKLR_OUT_BF16, AKLR_OUT_F16, AKLR_F32), rows *_stride elements
+ * apart; what is negative, infinite or NaN counts as 0. Uniforms are cut to [0, 1 - 2^-24], NaN to 0. A draft with a token
+ * outside [0, vocab), or a parent that does not come before it, is passed over, and so are those past `most`.
+ * out_tokens (draft_tokens' type) and path [batch, most]: the drafts that stand, then the next token; 0, then the numbers
+ * of the drafts that stand; -1 behind counts[b] entries (0 of a sequence without query tokens). tokens: rows of the two
+ * tensors, vocab <= 2^24, most <= 1024, batch <= 65536. Workspace: aklr_verify_drafts_workspace_bytes(...), any content.
+ */
+size_t aklr_verify_drafts_workspace_bytes(int64_t batch, int64_t vocab, int64_t most);
+int aklr_verify_drafts(const void* target_probs, int64_t target_stride, const void* draft_probs, int64_t draft_stride,
+                       int64_t tokens, int64_t vocab, const void* draft_tokens, int tokens_64, const int32_t* parents,
+                       const int32_t* starts, const float* accept_uniforms, const float* sample_uniforms, int64_t batch,
+                       int64_t most, void* out_tokens, int32_t* path, int32_t* counts, int dtype, void* workspace,
+                       size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * Low-rank adapters beside a shared projection: out[t] = base[t] + scales[i] * (x[t] a[i]^T) b[i]^T, i = adapters[t] (int32, or
+ * int64 with adapters_64); out[t] = base[t] where i is outside [0, adapter_count). x [tokens, k], a [adapter_count, rank, k],
+ * b [adapter_count, n, rank], base and out [tokens, n] of dtype (bf16, fp16), the last dimension contiguous, other strides in
+ * elements, multiples of 8, pointers aligned to 16 bytes; out is base (same pointer and stride) or apart from all inputs.
+ * scales fp32 (NULL: 1), ranks int32 (NULL: rank): of adapter i only the first ranks[i] rows of a and columns of b are used.
+ * k, n, rank multiples of 8; k <= 65536, n <= 262144, rank <= 128, tokens <= 2^20, adapter_count <= 4096.
+ * Workspace: aklr_lora_project_workspace_bytes(...), any content.
+ */
+size_t aklr_lora_project_workspace_bytes(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapter_count);
+int aklr_lora_project(const void* x, int64_t x_stride, const void* a, int64_t a_adapter_stride, int64_t a_row_stride,
+                      const void* b, int64_t b_adapter_stride, int64_t b_row_stride, const void* adapters, int adapters_64,
+                      const float* scales, const int32_t* ranks, const void* base, int64_t base_stride, void* out,
+                      int64_t out_stride, int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapter_count, int dtype,
+                      void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/*
  * Calibration kernel for the decode roofline (no counterpart in the reference): reads `bytes` from
  * `src` with the decode GEMM's access pattern -- 16-byte non-temporal loads, `unroll` (4 or 8) per lane
  * in flight, `workgroups` workgroups of 256 lanes each streaming one contiguous chunk -- and nothing
