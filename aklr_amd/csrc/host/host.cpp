@@ -4,7 +4,7 @@
 // outputs, or None where the general Python path has to decide: a call outside the contract, a disabled or
 // traced op, out=, trans_b=False, a tensor subclass, an active torch mode, a missing or unknown argument.
 // It serves exactly what that path would serve, in the same way: the checks of aklr_amd/gemm.py, quant.py, rotary.py,
-// kv_cache.py and attention.py, then torch's allocator for outputs and scratch and the C ABI on the current stream.
+// kv_cache.py, attention.py, drafts.py, kv_pages.py and lora.py, then torch's allocator for outputs and scratch and the C ABI on the current stream.
 // Nothing is kept between calls, and the GIL is released around allocation and launch.
 //
 // Why: a decode GEMM takes 3 to 20 us on the GPU, and its call took 12 to 17 us on the host (argument
@@ -744,12 +744,247 @@ PyObject* tree_attention(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------------------------
+// drafted tokens, pages of the cache, adapters: the checks of aklr_amd/drafts.py, kv_pages.py and lora.py
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+bool rows_ok(const Tensor& t) {
+  return t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1) && row_stride(t) >= t.size(1) &&
+         reinterpret_cast<uintptr_t>(t.const_data_ptr()) % t.element_size() == 0;
+}
+
+bool vector_ok(const Tensor& t, int64_t n, at::ScalarType type) {
+  return t.scalar_type() == type && t.dim() == 1 && t.size(0) == n && t.is_contiguous();
+}
+
+bool whole(PyObject* o, int64_t least, int64_t most, int64_t* out) {
+  if (!PyLong_CheckExact(o)) return false;
+  *out = PyLong_AsLongLong(o);
+  if (*out == -1 && PyErr_Occurred()) return PyErr_Clear(), false;
+  return *out >= least && *out <= most;
+}
+
+const int32_t* ints(const Tensor* t) { return t ? static_cast<const int32_t*>(t->const_data_ptr()) : nullptr; }
+const float* floats(const Tensor* t) { return t ? static_cast<const float*>(t->const_data_ptr()) : nullptr; }
+
+at::Tensor scratch(size_t bytes, const Tensor& like) {
+  return bytes ? make({static_cast<int64_t>(bytes)}, at::kByte, like) : at::Tensor();
+}
+void* data_or_null(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+
+PyObject* tuple_of(std::initializer_list<const Tensor*> ts) {
+  PyObject* r = PyTuple_New(static_cast<Py_ssize_t>(ts.size()));
+  if (!r) return nullptr;
+  Py_ssize_t i = 0;
+  for (const Tensor* t : ts) {
+    PyObject* o = THPVariable_Wrap(*t);
+    if (!o) return Py_DECREF(r), nullptr;
+    PyTuple_SET_ITEM(r, i++, o);
+  }
+  return r;
+}
+
+PyObject* verify(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  HANDLE_TH_ERRORS
+  static const char* const names[] = {"target_probs", "draft_tokens", "starts", "accept_uniforms", "sample_uniforms",
+                                      "most", "draft_probs", "parents"};
+  PyObject* p[8];
+  if (!bind(argv, argc, names, 8, 6, 6, p) || watched()) Py_RETURN_NONE;
+  const Tensor *target = dense(p[0]), *tokens = dense(p[1]), *starts = dense(p[2]), *accept = dense(p[3]),
+               *sample = dense(p[4]), *draft, *parents;
+  int64_t most;
+  if (!target || !tokens || !starts || !accept || !sample || !given(p[6], &draft) || !given(p[7], &parents) ||
+      !whole(p[5], 1, 1024, &most) || !rows_ok(*target))
+    Py_RETURN_NONE;
+  const int64_t n = target->size(0), vocab = target->size(1);
+  const auto type = target->scalar_type();
+  if (float_code(type) < 0 || n < 1 || n >= (int64_t{1} << 31) || vocab < 8 || vocab > (1 << 24) || !starts_ok(*starts)) Py_RETURN_NONE;
+  const int64_t batch = starts->numel() - 1;
+  if (batch < 1 || batch > 65536 || !index_ok(*tokens, n) || !vector_ok(*accept, n, at::kFloat) ||
+      !vector_ok(*sample, batch, at::kFloat) || (parents && !vector_ok(*parents, n, at::kInt)))
+    Py_RETURN_NONE;
+  if (draft && (!rows_ok(*draft) || draft->sizes() != target->sizes() || draft->scalar_type() != type)) Py_RETURN_NONE;
+  if (!one_device(*target, tokens, starts, accept, sample, draft, parents)) Py_RETURN_NONE;
+  for (const Tensor* t : {target, accept, sample, draft})
+    if (wants_grad(t)) Py_RETURN_NONE;
+  Tensor out, path, counts, ws;
+  int st;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard on(target->device());
+    out = make({batch, most}, tokens->scalar_type(), *target);
+    path = make({batch, most}, at::kInt, *target);
+    counts = make({batch}, at::kInt, *target);
+    const size_t bytes = aklr_verify_drafts_workspace_bytes(batch, vocab, most);
+    ws = scratch(bytes, *target);
+    st = aklr_verify_drafts(target->const_data_ptr(), row_stride(*target), at_or_null(draft), draft ? row_stride(*draft) : 0, n,
+                            vocab, tokens->const_data_ptr(), tokens->scalar_type() == at::kLong, ints(parents), ints(starts),
+                            floats(accept), floats(sample), batch, most, out.mutable_data_ptr(),
+                            static_cast<int32_t*>(path.mutable_data_ptr()), static_cast<int32_t*>(counts.mutable_data_ptr()),
+                            float_code(type), data_or_null(ws), bytes, stream_of(*target));
+  }
+  return st == AKLR_OK ? tuple_of({&out, &path, &counts}) : status_error(st, "verify_drafts");
+  END_HANDLE_TH_ERRORS
+}
+
+// The cache and what a call reads beside it share no memory, nor do the cache's tensors.
+bool cache_apart(const Cache& c, std::initializer_list<const Tensor*> others) {
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < i; ++j)
+      if (!apart(c.t[i], c.t[j])) return false;
+  return std::all_of(others.begin(), others.end(),
+                     [&](const Tensor* t) { return t->device() == c.t[0]->device() && c.clear_of(t); });
+}
+
+PyObject* kv_copy(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  HANDLE_TH_ERRORS
+  static const char* const names[] = {"k_cache", "v_cache", "k_scale", "v_scale", "src", "dst"};
+  PyObject* p[6];
+  if (!bind(argv, argc, names, 6, 6, 6, p) || watched()) Py_RETURN_NONE;
+  Cache c;
+  const Tensor *src = dense(p[4]), *dst = dense(p[5]);
+  if (!src || !dst || src->dim() != 1 || src->numel() < 1 || src->numel() >= (int64_t{1} << 31) || !index_ok(*src, src->numel()) ||
+      !vector_ok(*dst, src->numel(), src->scalar_type()) || !c.read(p) || !cache_apart(c, {src, dst}))
+    Py_RETURN_NONE;
+  int st;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard on(c.t[0]->device());
+    st = aklr_kv_cache_copy_pages_fp8(c.t[0]->mutable_data_ptr(), c.t[1]->mutable_data_ptr(), c.scales(2), c.scales(3),
+                                      c.step[0], c.step[1], c.step[2], c.step[3], src->const_data_ptr(), dst->const_data_ptr(),
+                                      src->scalar_type() == at::kLong, src->numel(), c.heads, c.dim, c.pages, c.page,
+                                      stream_of(*c.t[0]));
+  }
+  return st == AKLR_OK ? PyTuple_Pack(4, p[0], p[1], p[2], p[3]) : status_error(st, "kv_cache_copy_pages_fp8");
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* kv_compact(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  HANDLE_TH_ERRORS
+  static const char* const names[] = {"k_cache", "v_cache", "k_scale", "v_scale", "block_table", "seq_lens", "starts", "path",
+                                      "counts"};
+  PyObject* p[9];
+  if (!bind(argv, argc, names, 9, 9, 9, p) || watched()) Py_RETURN_NONE;
+  Cache c;
+  const Tensor *table = dense(p[4]), *lens = dense(p[5]), *starts = dense(p[6]), *path = dense(p[7]), *counts = dense(p[8]);
+  if (!table || !lens || !starts || !path || !counts || lens->dim() != 1) Py_RETURN_NONE;
+  const int64_t batch = lens->numel();
+  if (batch < 1 || batch > 65536 || !starts_ok(*starts) || starts->numel() != batch + 1 || !table_ok(*table, batch) ||
+      table->size(1) < 1 || !vector_ok(*lens, batch, at::kInt) || !vector_ok(*counts, batch, at::kInt) || !table_ok(*path, batch) ||
+      path->size(1) < 1 || path->size(1) >= (int64_t{1} << 31))
+    Py_RETURN_NONE;
+  if (!c.read(p) || !cache_apart(c, {table, lens, starts, path, counts}) || table->size(1) * c.page > (int64_t{1} << 28)) Py_RETURN_NONE;
+  const int64_t most = path->size(1);
+  int st;
+  Tensor ws;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard on(c.t[0]->device());
+    const size_t bytes = aklr_kv_cache_compact_fp8_workspace_bytes(batch, most, c.heads, c.dim);
+    ws = scratch(bytes, *c.t[0]);
+    st = aklr_kv_cache_compact_fp8(c.t[0]->mutable_data_ptr(), c.t[1]->mutable_data_ptr(), c.scales(2), c.scales(3), c.step[0],
+                                   c.step[1], c.step[2], c.step[3], ints(table), table_stride(*table), table->size(1), ints(lens),
+                                   ints(starts), ints(path), row_stride(*path), most, ints(counts), batch, c.heads, c.dim, c.pages,
+                                   c.page, data_or_null(ws), bytes, stream_of(*c.t[0]));
+  }
+  return st == AKLR_OK ? PyTuple_Pack(4, p[0], p[1], p[2], p[3]) : status_error(st, "kv_cache_compact_fp8");
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* kv_update(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  HANDLE_TH_ERRORS
+  static const char* const names[] = {"page_refs", "block_table", "lens", "new_lens", "page_size", "parents"};
+  PyObject* p[6];
+  if (!bind(argv, argc, names, 6, 6, 5, p) || watched()) Py_RETURN_NONE;
+  const Tensor *refs = plain(p[0]), *table = dense(p[1]), *lens = dense(p[2]), *wants = dense(p[3]), *parents;
+  int64_t page;
+  if (!refs || !table || !lens || !wants || !given(p[5], &parents) || !whole(p[4], 1, int64_t{1} << 31, &page) || lens->dim() != 1)
+    Py_RETURN_NONE;
+  const int64_t batch = lens->numel(), pages = refs->numel();
+  if (batch < 1 || batch > 65536 || pages < 1 || pages * page >= (int64_t{1} << 31) || !table_ok(*table, batch)) Py_RETURN_NONE;
+  const int64_t cols = table->size(1);
+  if (cols * page > (int64_t{1} << 28) || batch * cols >= (int64_t{1} << 31) || !vector_ok(*refs, pages, at::kInt) ||
+      !vector_ok(*lens, batch, at::kInt) || !vector_ok(*wants, batch, at::kInt) || (parents && !vector_ok(*parents, batch, at::kInt)))
+    Py_RETURN_NONE;
+  if (!one_device(*refs, table, lens, wants, parents) || !apart_all(refs, {table, lens, wants, parents})) Py_RETURN_NONE;
+  Tensor out, granted, src, dst, ws;
+  int st;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard on(refs->device());
+    out = make({batch, cols}, at::kInt, *refs);
+    granted = make({batch}, at::kInt, *refs);
+    src = make({batch}, at::kInt, *refs);
+    dst = make({batch}, at::kInt, *refs);
+    const size_t bytes = aklr_kv_cache_update_pages_workspace_bytes(batch);
+    ws = scratch(bytes, *refs);
+    const auto to = [](const Tensor& t) { return static_cast<int32_t*>(t.mutable_data_ptr()); };
+    st = aklr_kv_cache_update_pages(to(*refs), pages, ints(table), table_stride(*table), cols, ints(lens), ints(wants),
+                                    ints(parents), batch, page, to(out), to(granted), to(src), to(dst), data_or_null(ws), bytes,
+                                    stream_of(*refs));
+  }
+  return st == AKLR_OK ? tuple_of({&out, &granted, &src, &dst}) : status_error(st, "kv_cache_update_pages");
+  END_HANDLE_TH_ERRORS
+}
+
+// A tensor of 16-byte pieces along its last dimension.
+bool pieces_ok(const Tensor& t, at::ScalarType type, at::IntArrayRef shape) {
+  if (t.scalar_type() != type || t.sizes() != shape || t.stride(-1) != 1 || !aligned16(t)) return false;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d)
+    if (t.stride(d) % 8) return false;
+  return true;
+}
+
+PyObject* lora(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  HANDLE_TH_ERRORS
+  static const char* const names[] = {"x", "a", "b", "adapters", "base", "scales", "ranks", "out"};
+  PyObject* p[8];
+  if (!bind(argv, argc, names, 8, 5, 5, p) || watched()) Py_RETURN_NONE;
+  const Tensor *x = dense(p[0]), *a = dense(p[1]), *b = dense(p[2]), *ids = dense(p[3]), *base = dense(p[4]), *scales, *ranks, *out;
+  if (!x || !a || !b || !ids || !base || !given(p[5], &scales) || !given(p[6], &ranks) || !given(p[7], &out) || x->dim() != 2 ||
+      b->dim() != 3)
+    Py_RETURN_NONE;
+  const int64_t tokens = x->size(0), k = x->size(1), count = b->size(0), n = b->size(1), rank = b->size(2);
+  const auto type = x->scalar_type();
+  if ((type != at::kBFloat16 && type != at::kHalf) || k < 8 || k > 65536 || k % 8 || n < 8 || n > 262144 || n % 8 || rank < 8 ||
+      rank > 128 || rank % 8 || tokens < 1 || tokens > (1 << 20) || count < 1 || count > 4096)
+    Py_RETURN_NONE;
+  if (!pieces_ok(*x, type, {tokens, k}) || !pieces_ok(*a, type, {count, rank, k}) || !pieces_ok(*b, type, {count, n, rank}) ||
+      !pieces_ok(*base, type, {tokens, n}) || !index_ok(*ids, tokens) || (scales && !vector_ok(*scales, count, at::kFloat)) ||
+      (ranks && !vector_ok(*ranks, count, at::kInt)))
+    Py_RETURN_NONE;
+  if (!one_device(*x, a, b, ids, base, scales, ranks, out)) Py_RETURN_NONE;
+  for (const Tensor* t : {x, a, b, base, scales, out})
+    if (wants_grad(t)) Py_RETURN_NONE;
+  if (out && (!pieces_ok(*out, type, {tokens, n}) || !no_inner_overlap(*out) || !(same_place(*out, *base) || apart(out, base)) ||
+              !apart_all(out, {x, a, b, ids, scales, ranks})))
+    Py_RETURN_NONE;
+  Tensor o, ws;
+  int st;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard on(x->device());
+    o = out ? *out : make({tokens, n}, type, *x);
+    const size_t bytes = aklr_lora_project_workspace_bytes(tokens, k, n, rank, count);
+    ws = scratch(bytes, *x);
+    st = aklr_lora_project(x->const_data_ptr(), x->stride(0), a->const_data_ptr(), a->stride(0), a->stride(1), b->const_data_ptr(),
+                           b->stride(0), b->stride(1), ids->const_data_ptr(), ids->scalar_type() == at::kLong, floats(scales),
+                           ints(ranks), base->const_data_ptr(), base->stride(0), o.mutable_data_ptr(), o.stride(0), tokens, k, n, rank,
+                           count, out_code(type), data_or_null(ws), bytes, stream_of(*x));
+  }
+  if (st != AKLR_OK) return status_error(st, "lora_project");
+  if (out) return Py_INCREF(p[7]), p[7];
+  return THPVariable_Wrap(o);
+  END_HANDLE_TH_ERRORS
+}
+
 #define AKLR_HOST_FN(name) \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {AKLR_HOST_FN(quant_fp8), AKLR_HOST_FN(quant_mxfp8), AKLR_HOST_FN(quant_mxfp4),
                           AKLR_HOST_FN(gemm_fp8), AKLR_HOST_FN(quant_gemm_fp8), AKLR_HOST_FN(gemm_mxfp4),
                           AKLR_HOST_FN(rotary), AKLR_HOST_FN(kv_write), AKLR_HOST_FN(rotary_kv_write),
-                          AKLR_HOST_FN(kv_read), AKLR_HOST_FN(tree_attention),
+                          AKLR_HOST_FN(kv_read), AKLR_HOST_FN(tree_attention), AKLR_HOST_FN(verify),
+                          AKLR_HOST_FN(kv_copy), AKLR_HOST_FN(kv_compact), AKLR_HOST_FN(kv_update), AKLR_HOST_FN(lora),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", "the ops' per-call host work", -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};

@@ -177,6 +177,9 @@ __global__ __launch_bounds__(kThreads) void compact_long_kernel(const CompactArg
   const int tiles = (a.w1 - a.w0 + kRows - 1) / kRows;
   const int seq = blockIdx.x / tiles, b = a.b0 + seq;
   const int i0 = a.w0 + (blockIdx.x - seq * tiles) * kRows;
+  if (SAVE) {  // path ascends: where a tile's first item comes from behind the window, nothing of it is copied aside
+    if (i0 >= a.counts[b] || a.path[(int64_t)b * a.path_row + i0] >= a.w1) return;
+  }
   if (threadIdx.x < 64) {
     Place f = {-1, 0}, t = {-1, 0};
     int source = -1;
@@ -278,21 +281,16 @@ __device__ __forceinline__ int32_t ref_load(const int32_t* p) {
 }
 
 // A sequence a workgroup: it lets go of the pages it held, takes hold of the whole pages it keeps, and writes them into
-// the new table. One that keeps its own skips both for them. The page that it keeps a part of is let go of here; who may
+// the new table. The page that it keeps a part of is let go of here; who may
 // go on writing into it is decided once all have let go.
 __global__ __launch_bounds__(kThreads) void update_hold_kernel(const UpdateArgs a) {
   const int b = blockIdx.x;
   const Row r = row_of(a, b);
   const int held = (clamp_len(a, a.lens[b]) + a.page - 1) / a.page;
-  const bool same = r.parent == b;
   for (int c = threadIdx.x; c < a.cols; c += kThreads) {
-    int kept = -1;
-    if (c < r.full) {
-      kept = page_at(a, r.parent, c);
-      if (!same && kept >= 0) atomicAdd(a.refs + kept, 1);
-    }
-    if (c < held && !(same && c < r.full)) {
-      const int own = page_at(a, b, c);
+    const int kept = c < r.full ? page_at(a, r.parent, c) : -1, own = c < held ? page_at(a, b, c) : -1;
+    if (kept != own) {  // a page that it held and keeps, as forks of one prompt do, stays as it is
+      if (kept >= 0) atomicAdd(a.refs + kept, 1);
       if (own >= 0) atomicSub(a.refs + own, 1);
     }
     a.out[(int64_t)b * a.cols + c] = kept;
@@ -323,41 +321,58 @@ __device__ __forceinline__ int block_before(int x, int* sums, int& total) {
   return off + s - x;
 }
 
-constexpr int kLdsRows = 8192;  // of `before` in LDS; past them it is searched in memory
+constexpr int kLdsRows = 4096;  // sequences whose sums are searched in LDS; of more, in memory
 constexpr int kScan = 8;        // pages a lane looks at in one round
 constexpr int32_t kClaim = INT32_MIN;
+
+// Every atomic before it has been performed, for all lanes of the workgroup.
+__device__ __forceinline__ void settle() {
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+}
 
 // One workgroup for what hangs on an order. A partly kept page that nobody holds any more goes to the lowest of the
 // sequences that keep a part of it (each claims it by an atomic minimum); the others, and all that keep a part of a page
 // somebody still holds, copy it to a new one. New pages are then asked for in the order of sequences and columns, and the
 // k-th asked for is the k-th lowest free page: found by counting zeros in rounds of 8192 pages and, for each, searching
-// whose it is in the sums of what the sequences ask for.
+// whose it is in the sums of what the sequences ask for. Bound by its chain of loads and atomics: a lane keeps what it knows
+// of its first sequence, so that up to 1024 are read once.
 __global__ __launch_bounds__(kJoin) void update_grow_kernel(const UpdateArgs a) {
   __shared__ int sums[kJoin / 64];
-  __shared__ int32_t lds[kLdsRows];
+  __shared__ int32_t lds_before[kLdsRows], lds_begin[kLdsRows];
   const bool fits = a.batch <= kLdsRows;
+  struct Part {
+    Row r;
+    int page;  // of which a part is kept; -1: none, or one that the cache does not have
+  };
+  const auto read = [&](int b) {
+    Part p;
+    p.r = row_of(a, b);
+    p.page = p.r.part ? page_at(a, p.r.parent, p.r.full) : -1;
+    return p;
+  };
+  Part own{};
+  if ((int)threadIdx.x < a.batch) own = read(threadIdx.x);
+  const auto part = [&](int b) { return b < kJoin ? own : read(b); };
   for (int b = threadIdx.x; b < a.batch; b += kJoin) {
-    const Row r = row_of(a, b);
-    const int g = r.part ? page_at(a, r.parent, r.full) : -1;
-    if (g >= 0) {
-      const int32_t n = ref_load(a.refs + g);
-      if (n == 0 || (n < 0 && n < kClaim + a.batch)) atomicMin(a.refs + g, kClaim + b);
-    }
+    const Part p = part(b);
+    if (p.page < 0) continue;
+    const int32_t n = ref_load(a.refs + p.page);
+    if (n == 0 || (n < 0 && n < kClaim + a.batch)) atomicMin(a.refs + p.page, kClaim + b);
   }
-  __threadfence();
-  __syncthreads();
+  settle();
   int asked = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kJoin) {
     const int b = b0 + threadIdx.x;
     int need = 0, begin = 0;
+    bool copies = false;
     if (b < a.batch) {
-      const Row r = row_of(a, b);
-      const int g = r.part ? page_at(a, r.parent, r.full) : -1;
-      const bool takes = g >= 0 && ref_load(a.refs + g) == kClaim + b;
-      if (takes) a.out[(int64_t)b * a.cols + r.full] = g;
-      begin = r.full + (r.part && (takes || g < 0) ? 1 : 0);  // a part of no page stays one of none
-      need = max((r.want + a.page - 1) / a.page - begin, 0);
-      a.src[b] = a.dst[b] = -1;
+      const Part p = part(b);
+      const bool takes = p.page >= 0 && ref_load(a.refs + p.page) == kClaim + b;
+      if (takes) a.out[(int64_t)b * a.cols + p.r.full] = p.page;
+      copies = p.page >= 0 && !takes;
+      begin = p.r.full + (p.r.part && !copies ? 1 : 0);  // a part of no page stays one of none
+      need = max((p.r.want + a.page - 1) / a.page - begin, 0);
     }
     int total;
     const int off = asked + block_before(need, sums, total);
@@ -365,20 +380,18 @@ __global__ __launch_bounds__(kJoin) void update_grow_kernel(const UpdateArgs a) 
     if (b < a.batch) {
       a.begin[b] = begin;
       a.before[b] = off;
-      if (fits) lds[b] = off;
+      if (fits) lds_begin[b] = begin, lds_before[b] = off;
+      a.src[b] = copies ? -2 : -1;  // until it is known whether there is a page
     }
   }
-  __threadfence();
-  __syncthreads();
+  settle();
   for (int b = threadIdx.x; b < a.batch; b += kJoin) {  // claims become holders, now that all have read them
-    const Row r = row_of(a, b);
-    if (!r.part || a.begin[b] == r.full) continue;
-    const int g = page_at(a, r.parent, r.full);
-    if (g >= 0) __hip_atomic_store(a.refs + g, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const Part p = part(b);
+    if (p.page >= 0 && a.src[b] != -2) __hip_atomic_store(a.refs + p.page, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  __threadfence();
-  __syncthreads();
-  const int32_t* const before = fits ? lds : a.before;
+  settle();
+  const int32_t* const before = fits ? lds_before : a.before;
+  const int32_t* const begin = fits ? lds_begin : a.begin;
   int found = 0;
   for (int64_t p0 = 0; p0 < a.pages && found < asked; p0 += (int64_t)kJoin * kScan) {
     const int64_t p = p0 + (int64_t)threadIdx.x * kScan;
@@ -398,21 +411,20 @@ __global__ __launch_bounds__(kJoin) void update_grow_kernel(const UpdateArgs a) 
         else
           hi = mid;
       }
-      const int col = a.begin[lo] + k - before[lo];
-      a.out[(int64_t)lo * a.cols + col] = page;
+      a.out[(int64_t)lo * a.cols + begin[lo] + k - before[lo]] = page;
       __hip_atomic_store(a.refs + page, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const Row r = row_of(a, lo);
-      if (r.part && col == r.full) {
-        a.src[lo] = page_at(a, r.parent, r.full);
-        a.dst[lo] = page;
-      }
     }
     found += total;
   }
+  settle();
   for (int b = threadIdx.x; b < a.batch; b += kJoin) {
-    const int want = clamp_len(a, a.want[b]), begin = a.begin[b];
-    const int need = max((want + a.page - 1) / a.page - begin, 0), got = found - a.before[b];
-    a.granted[b] = got >= need ? want : min(want, (begin + max(got, 0)) * a.page);
+    const Part p = part(b);
+    const int first = begin[b], got = found - before[b];
+    const int need = max((p.r.want + a.page - 1) / a.page - first, 0);
+    a.granted[b] = got >= need ? p.r.want : min(p.r.want, (first + max(got, 0)) * a.page);
+    const bool copies = a.src[b] == -2 && got > 0;  // its first new page is the copy
+    a.src[b] = copies ? p.page : -1;
+    a.dst[b] = copies ? a.out[(int64_t)b * a.cols + first] : -1;
   }
 }
 

@@ -20,8 +20,9 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kThreads = 256;
-constexpr int kScan = 256;       // tokens that a workgroup looks through by itself
+constexpr int kScan = 256;  // tokens that a workgroup looks through by itself
 constexpr int kMostAdapters = 4096;  // what the sort counts in LDS
+constexpr int kIdBits = 13;          // of a token's adapter, one behind them included
 
 template <bool F16>
 __device__ __forceinline__ f32x4 product(const u32x4& a, const u32x4& b, const f32x4& c) {
@@ -32,9 +33,9 @@ __device__ __forceinline__ f32x4 product(const u32x4& a, const u32x4& b, const f
 }
 
 struct Tile {
-  int adapter;  // -1: tokens without one
-  int first;    // in the order of adapters
-  int count;
+  int adapter;  // `adapters`: tokens without one
+  int first;    // in `order`
+  int count;    // 0: no tile
   int pad;
 };
 
@@ -48,83 +49,128 @@ struct LoraArgs {
   float* part;  // [splits][tokens][rank rounded up to the products' rows]
   int32_t* order;
   Tile* tiles;
-  int32_t* tile_count;
   int tokens, k, n, rank, adapters, ids64, splits, k_split, n_group, copies;
 };
 
+// A token's adapter, `adapters` where it has none.
 __device__ __forceinline__ int adapter_of(const LoraArgs& a, int t) {
-  const int64_t i = a.ids64 ? static_cast<const int64_t*>(a.ids)[t] : (int64_t) static_cast<const int32_t*>(a.ids)[t];
-  return i < 0 || i >= a.adapters ? -1 : (int)i;
+  const uint32_t* const p = static_cast<const uint32_t*>(a.ids);
+  const uint32_t i = p[(int64_t)t << a.ids64];
+  if (a.ids64 && p[2 * (int64_t)t + 1] != 0) return a.adapters;
+  return i < (uint32_t)a.adapters ? (int)i : a.adapters;
 }
 
 __device__ __forceinline__ int rank_of(const LoraArgs& a, int adapter) {
-  if (adapter < 0) return 0;
+  if (adapter >= a.adapters) return 0;
   return a.ranks ? min(max(a.ranks[adapter], 0), a.rank) : a.rank;
 }
 
-// The workgroup's tile: its tokens in `rows`, the first repeated behind them. False: there is none. With few tokens, `id`
-// is a token, and a tile begins at each of an adapter's tokens that has a whole number of tiles' tokens before it.
+// Tile number `id` from the workspace: its tokens in `rows`, the first repeated behind them. False: there is none.
 template <int TM>
-__device__ __forceinline__ bool find_tile(const LoraArgs& a, int id, int (&rows)[TM], int* words, int& adapter, int& count) {
-  if (a.tokens > kScan) {
-    if (id >= *a.tile_count) return false;
-    const Tile t = a.tiles[id];
-    adapter = t.adapter;
-    count = t.count;
-    if ((int)threadIdx.x < TM) rows[threadIdx.x] = a.order[t.first + ((int)threadIdx.x < t.count ? threadIdx.x : 0)];
-    __syncthreads();
-    return true;
-  }
+__device__ __forceinline__ bool read_tile(const LoraArgs& a, int id, int (&rows)[TM], int& adapter, int& count) {
+  const Tile tile = a.tiles[id];
+  adapter = tile.adapter;
+  count = tile.count;
+  if (count == 0) return false;
+  if ((int)threadIdx.x < TM) rows[threadIdx.x] = a.order[tile.first + ((int)threadIdx.x < count ? threadIdx.x : 0)];
+  __syncthreads();
+  return true;
+}
+
+struct Find {  // what looking for a tile takes of LDS
+  uint64_t bits[kThreads / 64][kIdBits];
+  int words[kThreads / 64], counts[kThreads / 64], leader, first;
+};
+
+// The same with few tokens, by the workgroup itself: which tokens have a lane's adapter follows from ballots over the bits of
+// all tokens' numbers. A tile begins at each token that has a whole number of tiles' tokens of its adapter before it, and the
+// tiles are counted in the order of where they begin. `writes`: puts it into the workspace, for the second launch.
+template <int TM>
+__device__ __forceinline__ bool find_tile(const LoraArgs& a, int id, int (&rows)[TM], Find& f, int& adapter, int& count, bool writes) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int own = t < a.tokens ? adapter_of(a, t) : -2;
-  adapter = adapter_of(a, id);
-  const uint64_t same = __ballot(own == adapter);
-  if (lane == 0) words[wave] = __popcll(same);
-  __syncthreads();
-  int before = __popcll(same & ((1ull << lane) - 1)), all = 0;
+  const int own = t < a.tokens ? adapter_of(a, t) : (1 << kIdBits) - 1;
 #pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) {
-    before += w < wave ? words[w] : 0;
-    all += words[w];
+  for (int i = 0; i < kIdBits; ++i) {
+    const uint64_t on = __ballot(own >> i & 1);
+    if (lane == 0) f.bits[wave][i] = on;
   }
-  if (t == id) words[4] = before;
+  if (t == 0) f.leader = -1;
   __syncthreads();
-  const int first = words[4];
-  if (first % TM) return false;
-  count = min(TM, all - first);
-  if (own == adapter && before >= first && before < first + count) {
-    rows[before - first] = t;
-    if (before == first)
-      for (int i = count; i < TM; ++i) rows[i] = t;
+  int before = 0;
+  const int waves = (a.tokens + 63) / 64;
+  for (int w = 0; w < min(waves, wave + 1); ++w) {
+    uint64_t same = w < wave ? ~0ull : (1ull << lane) - 1;
+#pragma unroll
+    for (int i = 0; i < kIdBits; ++i) same &= f.bits[w][i] ^ ((uint64_t)(own >> i & 1) - 1);
+    before += __popcll(same);
+  }
+  const bool begins = t < a.tokens && before % TM == 0;
+  const uint64_t on = __ballot(begins);
+  if (lane == 0) f.words[wave] = __popcll(on);
+  __syncthreads();
+  int number = __popcll(on & ((1ull << lane) - 1));
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) number += w < wave ? f.words[w] : 0;
+  if (begins && number == id) {
+    f.leader = own;
+    f.first = before;
   }
   __syncthreads();
+  adapter = f.leader;
+  if (adapter < 0) {
+    if (writes && t == 0) a.tiles[id] = {0, 0, 0, 0};
+    return false;
+  }
+  const int at = before - f.first;
+  const bool in = own == adapter && at >= 0 && at < TM;
+  const uint64_t ins = __ballot(in);
+  if (lane == 0) f.counts[wave] = __popcll(ins);
+  if (in) rows[at] = t;
+  __syncthreads();
+  count = f.counts[0] + f.counts[1] + f.counts[2] + f.counts[3];
+  if (t >= count && t < TM) rows[t] = rows[0];
+  __syncthreads();
+  if (writes) {
+    if (t < count) a.order[id * TM + t] = rows[t];
+    if (t == 0) a.tiles[id] = {adapter, id * TM, count, 0};
+  }
   return true;
 }
 
 // Tokens in the order of their adapters, those without one last, and the tiles of that order: one workgroup. Within an
 // adapter the order is that of arrival; no result depends on it. Consecutive tokens are mostly of one adapter: a wave whose
-// tokens all are counts them at once.
-constexpr int kSort = 1024;
-__global__ __launch_bounds__(kSort) void sort_kernel(const LoraArgs a, const int tm) {
-  extern __shared__ int32_t count[];  // [adapters + 1], then where each one's next token goes
+// tokens all are counts them at once. Up to 8192 tokens are read once.
+constexpr int kSort = 1024, kHeld = 8;
+__global__ __launch_bounds__(kSort) void sort_kernel(const LoraArgs a, const int tm, const int most) {
+  extern __shared__ int32_t counts[];  // [adapters + 1], then where each one's next token goes
   __shared__ int sums[kSort / 64], tile_sums[kSort / 64];
   const int groups = a.adapters + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int32_t* const next = count + groups;
-  for (int g = threadIdx.x; g < groups; g += kSort) count[g] = 0;
+  int32_t* const next = counts + groups;
+  int g[kHeld];
+  const auto read = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int t = t0 + i * kSort + threadIdx.x;
+      g[i] = t < a.tokens ? adapter_of(a, t) : -1;
+    }
+  };
+  read(0);
+  for (int i = threadIdx.x; i < groups; i += kSort) counts[i] = 0;
   __syncthreads();
-  const int last = (a.tokens + kSort - 1) / kSort * kSort;
-  for (int t = threadIdx.x; t < last; t += kSort) {
-    int g = t < a.tokens ? adapter_of(a, t) : -2;
-    g = g == -1 ? a.adapters : g;
-    const int g0 = __builtin_amdgcn_readfirstlane(g);
-    const uint64_t same = __ballot(g == g0);
-    if (g0 >= 0 && lane == 0) atomicAdd(count + g0, __popcll(same));
-    if (g >= 0 && g != g0) atomicAdd(count + g, 1);
+  for (int t0 = 0; t0 < a.tokens; t0 += kHeld * kSort) {
+    if (t0 > 0) read(t0);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int g0 = __builtin_amdgcn_readfirstlane(g[i]);
+      const uint64_t same = __ballot(g[i] == g0);
+      if (g0 >= 0 && lane == 0) atomicAdd(counts + g0, __popcll(same));
+      if (g[i] >= 0 && g[i] != g0) atomicAdd(counts + g[i], 1);
+    }
   }
   __syncthreads();
   int tokens_before = 0, tiles_before = 0;
   for (int g0 = 0; g0 < groups; g0 += kSort) {
-    const int g = g0 + threadIdx.x, c = g < groups ? count[g] : 0, tiles = (c + tm - 1) / tm;
+    const int id = g0 + threadIdx.x, c = id < groups ? counts[id] : 0, tiles = (c + tm - 1) / tm;
     int s = c, u = tiles;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -142,23 +188,25 @@ __global__ __launch_bounds__(kSort) void sort_kernel(const LoraArgs a, const int
       tokens_before += sums[w];
       tiles_before += tile_sums[w];
     }
-    if (g < groups) {
-      next[g] = at;
-      for (int i = 0; i < tiles; ++i) a.tiles[tile + i] = {g == a.adapters ? -1 : g, at + i * tm, min(tm, c - i * tm), 0};
+    if (id < groups) {
+      next[id] = at;
+      for (int i = 0; i < tiles; ++i) a.tiles[tile + i] = {id, at + i * tm, min(tm, c - i * tm), 0};
     }
   }
-  if (threadIdx.x == 0) *a.tile_count = tiles_before;
+  for (int i = tiles_before + threadIdx.x; i < most; i += kSort) a.tiles[i] = {0, 0, 0, 0};
   __syncthreads();
-  for (int t = threadIdx.x; t < last; t += kSort) {
-    int g = t < a.tokens ? adapter_of(a, t) : -2;
-    g = g == -1 ? a.adapters : g;
-    const int g0 = __builtin_amdgcn_readfirstlane(g);
-    const uint64_t same = __ballot(g == g0);
-    int at = 0;
-    if (g0 >= 0 && lane == 0) at = atomicAdd(next + g0, __popcll(same));
-    at = __builtin_amdgcn_readfirstlane(at) + __popcll(same & ((1ull << lane) - 1));
-    if (g >= 0 && g != g0) at = atomicAdd(next + g, 1);
-    if (g >= 0) a.order[at] = t;
+  for (int t0 = 0; t0 < a.tokens; t0 += kHeld * kSort) {
+    if (a.tokens > kHeld * kSort) read(t0);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int g0 = __builtin_amdgcn_readfirstlane(g[i]);
+      const uint64_t same = __ballot(g[i] == g0);
+      int at = 0;
+      if (g0 >= 0 && lane == 0) at = atomicAdd(next + g0, __popcll(same));
+      at = __builtin_amdgcn_readfirstlane(at) + __popcll(same & ((1ull << lane) - 1));
+      if (g[i] >= 0 && g[i] != g0) at = atomicAdd(next + g[i], 1);
+      if (g[i] >= 0) a.order[at] = t0 + i * kSort + threadIdx.x;
+    }
   }
 }
 
@@ -168,10 +216,15 @@ __global__ __launch_bounds__(kSort) void sort_kernel(const LoraArgs a, const int
 template <int MT, int NR, bool F16>
 __global__ __launch_bounds__(kThreads) void shrink_kernel(const LoraArgs a) {
   constexpr int TM = 16 * MT;
-  __shared__ int rows[TM], words[5];
+  __shared__ int rows[TM];
   __shared__ f32x4 meet[2][NR][MT][64];
   int adapter, count;
-  if (!find_tile<TM>(a, blockIdx.x, rows, words, adapter, count)) return;
+  if constexpr (MT == 1) {
+    __shared__ Find find;
+    if (!find_tile<TM>(a, blockIdx.x, rows, find, adapter, count, blockIdx.y == 0)) return;
+  } else {
+    if (!read_tile<TM>(a, blockIdx.x, rows, adapter, count)) return;
+  }
   const int rank = rank_of(a, adapter);
   if (rank == 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
@@ -192,7 +245,7 @@ __global__ __launch_bounds__(kThreads) void shrink_kernel(const LoraArgs a) {
       const int at = k + h * 32 + g * 8;
       const bool on = at < k1;  // k % 8 == 0: eight values are inside or past the end
 #pragma unroll
-      for (int r = 0; r < NR; ++r) p.w[h][r] = on && r < used ? ld16_nt(ar[r] + at) : u32x4{0, 0, 0, 0};
+      for (int r = 0; r < NR; ++r) p.w[h][r] = on && r < used ? (MT == 1 ? ld16_nt(ar[r] + at) : ld16(ar[r] + at)) : u32x4{0, 0, 0, 0};
 #pragma unroll
       for (int m = 0; m < MT; ++m) p.x[h][m] = on ? ld16(xr[m] + at) : u32x4{0, 0, 0, 0};
     }
@@ -269,16 +322,17 @@ __device__ __forceinline__ float from16(uint32_t bits) {
 }
 
 // The outputs of a tile for n_group columns. A wave takes 64 columns at a time, four products' rows: row i of the q-th is
-// column 16 (i / 4) + 4 q + i % 4, so that a lane ends with 16 columns side by side of one token, and a token's four lanes
-// with a whole line of base and out.
+// column 32 (q / 2) + 8 (i / 4) + 4 (q % 2) + i % 4, so that a lane ends with twice eight columns side by side of one token,
+// and a token's four lanes with half a line of base and out an instruction. B's rows stay in registers for all the tile's
+// tokens; base comes sixteen tokens ahead, the first of it and of B before v's parts.
 template <int MT, int NR, bool F16>
 __global__ __launch_bounds__(kThreads) void expand_kernel(const LoraArgs a) {
   constexpr int TM = 16 * MT, R = 16 * NR, kSteps = (R + 31) / 32, kRow = kSteps * 32 + 8;  // a row of pieces: 16 bytes more
-  __shared__ int rows[TM], words[5];
+  __shared__ int rows[TM];
   __shared__ __align__(16) uint16_t piece[2][TM][kRow];
   __shared__ int power[TM];
   int adapter, count;
-  if (!find_tile<TM>(a, blockIdx.x, rows, words, adapter, count)) return;
+  if (!read_tile<TM>(a, blockIdx.x, rows, adapter, count)) return;
   const int rank = rank_of(a, adapter);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
   const int c0 = blockIdx.y * a.n_group, c1 = min(c0 + a.n_group, a.n);
@@ -288,6 +342,29 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(const LoraArgs a) {
       for (int c = c0 + 8 * threadIdx.x; c < c1; c += 8 * kThreads)
         *reinterpret_cast<u32x4*>(a.out + rows[i] * a.out_row + c) = ld16(a.base + rows[i] * a.base_row + c);
     return;
+  }
+  const int steps = (rank + 31) / 32;
+  u32x4 w[kSteps][4], old[2];
+  const auto load_w = [&](int c) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int r0 = s * 32 + g * 8;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = min(c + (q >> 1) * 32 + (li >> 2) * 8 + (q & 1) * 4 + (li & 3), a.n - 1);  // those past the end are not stored
+        w[s][q] = r0 < rank ? ld16(a.b + adapter * a.b_adapter + n * a.b_row + r0) : u32x4{0, 0, 0, 0};
+      }
+    }
+  };
+  const auto load_old = [&](int c, int m, u32x4 (&o)[2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (m * 16 + li < count && c + g * 8 + 32 * h < c1) o[h] = ld16(a.base + rows[m * 16 + li] * a.base_row + c + g * 8 + 32 * h);
+  };
+  int c = c0 + wave * 64;
+  if (c < c1) {
+    load_w(c);
+    load_old(c, 0, old);
   }
   constexpr int kLanes = R / 4;  // of a token: four values each
 #pragma unroll
@@ -332,65 +409,63 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(const LoraArgs a) {
   }
   __syncthreads();
   const float scale = a.scales ? a.scales[adapter] : 1.0f;
-  const int steps = (rank + 31) / 32;
-  for (int c = c0 + wave * 64; c < c1; c += kThreads) {
-    const int col = c + g * 16;  // the lane's columns
-    u32x4 old[MT][2];
+  while (c < c1) {
+    const int after = c + kThreads;
+    if (rank % 8) {  // what lies behind the rank may be anything
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+      for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (m * 16 + li < count && col + 8 * h < c1) old[m][h] = ld16_nt(a.base + rows[m * 16 + li] * a.base_row + col + 8 * h);
-    f32x4 acc[4][MT] = {};
+        for (int e = 0; e < 8; ++e)
+          if (s * 32 + g * 8 + e >= rank) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      if (s >= steps) break;
-      const int r0 = s * 32 + g * 8;
-      u32x4 w[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int n = min(c + (li >> 2) * 16 + q * 4 + (li & 3), a.n - 1);  // columns past the end are not stored
-        w[q] = r0 < rank ? ld16(a.b + adapter * a.b_adapter + n * a.b_row + r0) : u32x4{0, 0, 0, 0};
-        if (r0 < rank && r0 + 8 > rank) {  // what lies behind the rank may be anything
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (r0 + e >= rank) w[q][e / 2] &= e % 2 ? 0x0000FFFFu : 0xFFFF0000u;
-        }
-      }
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const u32x4 hi = *reinterpret_cast<const u32x4*>(&piece[0][m * 16 + li][r0]);
-        const u32x4 lo = *reinterpret_cast<const u32x4*>(&piece[1][m * 16 + li][r0]);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) acc[q][m] = product<F16>(w[q], lo, acc[q][m]);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) acc[q][m] = product<F16>(w[q], hi, acc[q][m]);
-      }
+            for (int q = 0; q < 4; ++q) w[s][q][e / 2] &= e % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+          }
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      if (m * 16 + li >= count) continue;
-      const int e = F16 ? power[m * 16 + li] : 0;
-      uint16_t* const to = a.out + rows[m * 16 + li] * a.out_row + col;
+      u32x4 next[2];
+      if (m + 1 < MT)
+        load_old(c, m + 1, next);
+      else if (after < c1)
+        load_old(after, 0, next);
+      f32x4 acc[4] = {};
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (col + 8 * h >= c1) continue;
-        u32x4 word;
+      for (int s = 0; s < kSteps; ++s) {
+        if (s >= steps) break;
+        const u32x4 hi = *reinterpret_cast<const u32x4*>(&piece[0][m * 16 + li][s * 32 + g * 8]);
+        const u32x4 lo = *reinterpret_cast<const u32x4*>(&piece[1][m * 16 + li][s * 32 + g * 8]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float y[2];
+        for (int q = 0; q < 4; ++q) acc[q] = product<F16>(w[s][q], lo, acc[q]);
 #pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            const int at = 8 * h + 2 * j + z;
-            float d = acc[at / 4][m][at % 4] * scale;
-            if constexpr (F16) d = __builtin_amdgcn_ldexpf(d, e);
-            y[z] = from16<F16>(z ? old[m][h][j] >> 16 : old[m][h][j] & 0xFFFFu) + d;
-          }
-          word[j] = pack_out2(y[0], y[1], F16 ? AKLR_OUT_F16 : AKLR_OUT_BF16);
-        }
-        __builtin_nontemporal_store(word, reinterpret_cast<u32x4*>(to + 8 * h));
+        for (int q = 0; q < 4; ++q) acc[q] = product<F16>(w[s][q], hi, acc[q]);
       }
+      if (m + 1 == MT && after < c1) load_w(after);
+      if (m * 16 + li < count) {
+        const int e = F16 ? power[m * 16 + li] : 0;
+        uint16_t* const to = a.out + rows[m * 16 + li] * a.out_row + c + g * 8;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (c + g * 8 + 32 * h >= c1) continue;
+          u32x4 word;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float y[2];
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              const int at = 8 * h + 2 * j + z;
+              float d = acc[at / 4][at % 4];
+              if constexpr (F16) d = __builtin_amdgcn_ldexpf(d, e);
+              y[z] = fmaf(d, scale, from16<F16>(z ? old[h][j] >> 16 : old[h][j] & 0xFFFFu));
+            }
+            word[j] = pack_out2(y[0], y[1], F16 ? AKLR_OUT_F16 : AKLR_OUT_BF16);
+          }
+          *reinterpret_cast<u32x4*>(to + 32 * h) = word;
+        }
+      }
+      old[0] = next[0];
+      old[1] = next[1];
     }
+    c = after;
   }
 }
 
@@ -402,10 +477,12 @@ namespace {
 
 struct Plan {
   int mt, nr;         // tiles of 16 tokens, of 16 rank rows
-  int64_t tiles;      // workgroups along x: the tokens where they look for their tiles, else the most tiles there can be
+  int64_t tiles;      // workgroups along x: the most tiles there can be
   int64_t splits, k_split, n_group;
   size_t order, tile, part, bytes;  // offsets in the workspace
 };
+
+constexpr int64_t kAtOnce = 1024;  // workgroups that run at once, about
 
 int64_t up(int64_t v, int64_t q) { return (v + q - 1) / q * q; }
 
@@ -416,20 +493,20 @@ Plan plan_lora(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapt
   p.mt = !sorts ? 1 : tokens < 2048 ? 2 : 4;
   const int64_t tm = 16 * p.mt, groups = adapters + 1 < tokens ? adapters + 1 : tokens;
   const int64_t most = (tokens + tm - 1) / tm + groups;  // sum of ceil(c / tm) over groups of c tokens
-  p.tiles = sorts ? most : tokens;
-  const int64_t real = most < tokens ? most : tokens;
-  int64_t splits = (1024 + real - 1) / real;
+  p.tiles = most < tokens ? most : tokens;
+  int64_t splits = kAtOnce / p.tiles;
   if (splits > (k + 511) / 512) splits = (k + 511) / 512;
+  if (splits < 1) splits = 1;
   p.k_split = up((k + splits - 1) / splits, 256);
   p.splits = (k + p.k_split - 1) / p.k_split;
   int64_t groups_n = (n + 255) / 256, loops = 1;
-  while (loops < 4 && real * ((groups_n + loops - 1) / loops) > 2048) loops *= 2;
+  while (loops < 4 && p.tiles * ((groups_n + loops - 1) / loops) > 2 * kAtOnce) loops *= 2;
   p.n_group = 256 * loops;
   size_t at = 0;
   p.order = at;
-  if (sorts) at += up(4 * tokens, 256);
+  at += up(4 * (sorts ? tokens : p.tiles * tm), 256);
   p.tile = at;
-  if (sorts) at += up(16 * (most + 1), 256);
+  at += up(16 * p.tiles, 256);
   p.part = at;
   p.bytes = at + 4 * (size_t)(p.splits * tokens * 16 * p.nr);
   return p;
@@ -481,8 +558,7 @@ extern "C" int aklr_lora_project(const void* x, int64_t x_stride, const void* a,
   g.ranks = ranks;
   g.part = reinterpret_cast<float*>(ws + p.part);
   g.order = reinterpret_cast<int32_t*>(ws + p.order);
-  g.tile_count = reinterpret_cast<int32_t*>(ws + p.tile);
-  g.tiles = reinterpret_cast<Tile*>(ws + p.tile) + 1;
+  g.tiles = reinterpret_cast<Tile*>(ws + p.tile);
   g.tokens = (int)tokens;
   g.k = (int)k;
   g.n = (int)n;
@@ -494,7 +570,7 @@ extern "C" int aklr_lora_project(const void* x, int64_t x_stride, const void* a,
   g.n_group = (int)p.n_group;
   g.copies = base != out;
   if (tokens > kScan) {
-    hipLaunchKernelGGL(sort_kernel, dim3(1), dim3(kSort), 8 * (adapter_count + 1), stream, g, 16 * p.mt);
+    hipLaunchKernelGGL(sort_kernel, dim3(1), dim3(kSort), 8 * (adapter_count + 1), stream, g, 16 * p.mt, (int)p.tiles);
     AKLR_LAUNCH_CHECK();
   }
   const dim3 shrink((unsigned)p.tiles, (unsigned)p.splits), expand((unsigned)p.tiles, (unsigned)((n + p.n_group - 1) / p.n_group));

@@ -21,6 +21,8 @@ namespace aklr {
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kMost = 1024;  // query tokens of a sequence
 constexpr int kUnit = 512;   // values of a row that one wave adds up to a partial sum: 8 a lane
+constexpr int kGroup = 2;    // units whose loads a wave has in flight
+constexpr int kNone = 0x7FFFFFFF;
 
 enum Status : int { kRefused, kEnd, kWholeRow, kDone };
 
@@ -54,7 +56,10 @@ template <>
 __device__ __forceinline__ float widen<_Float16>(_Float16 x) { return (float)x; }
 
 // Entries that are no probabilities (negative, NaN, infinite) count as zero.
-__device__ __forceinline__ float proper(float x) { return x > 0.0f && x < __builtin_inff() ? x : 0.0f; }
+__device__ __forceinline__ float proper(float x) {
+  constexpr int kPositiveFinite = 0x180;  // subnormal, normal
+  return __builtin_amdgcn_classf(x, kPositiveFinite) ? x : 0.0f;
+}
 
 __device__ __forceinline__ double unit_number(float u) {
   return u > 0.0f ? (double)fminf(u, 0x1.fffffep-1f) : 0.0;
@@ -64,25 +69,37 @@ __device__ __forceinline__ double weight(float p, float q, double a) {  // no co
   return fmax(__dsub_rn((double)p, __dmul_rn(a, (double)q)), 0.0);
 }
 
-// Eight values of a row from v on, past its end zeros. Rows start at any multiple of their element: the loads are 16 bytes
-// wide whatever the alignment.
+// Eight values of a row. Rows start at any multiple of their element: the loads are 16 bytes wide whatever the alignment.
 template <typename T>
-__device__ __forceinline__ void eight(const T* row, int v, int vocab, float (&f)[8]) {
-  T x[8];
-  if (v + 8 <= vocab) {
-    __builtin_memcpy(x, row + v, sizeof(x));
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = widen<T>(x[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = v + e < vocab ? widen<T>(row[v + e]) : 0.0f;
+struct Eight {
+  u32x4 x[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(x, p, sizeof(x)); }
+  __device__ __forceinline__ float operator[](int e) const {
+    if constexpr (sizeof(T) == 4) {
+      return proper(__uint_as_float(x[e / 4][e % 4]));
+    } else {
+      const uint16_t h = (uint16_t)(x[0][e / 2] >> (e % 2 * 16));
+      return proper(widen<T>(__builtin_bit_cast(T, h)));
+    }
   }
-}
+};
 
-__device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
-  return x;
+// x plus what lane `CTRL` says holds, in the rows of 16 lanes that MASK names (0 from no lane).
+template <int CTRL, int MASK>
+__device__ __forceinline__ double plus_dpp(double x) {
+  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(x), CTRL, MASK, 0xF, true);
+  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(x), CTRL, MASK, 0xF, true);
+  return x + __hiloint2double(hi, lo);
+}
+// The sum of the lanes of a wave's half up to this one; the second half's has the first's with WHOLE.
+template <bool WHOLE>
+__device__ __forceinline__ double sum_upto(double x) {
+  x = plus_dpp<0x111, 0xF>(x);  // row_shr:1
+  x = plus_dpp<0x112, 0xF>(x);
+  x = plus_dpp<0x114, 0xF>(x);
+  x = plus_dpp<0x118, 0xF>(x);
+  x = plus_dpp<0x142, 0xA>(x);  // row_bcast:15 into rows 1 and 3
+  return WHOLE ? plus_dpp<0x143, 0xC>(x) : x;  // row_bcast:31 into rows 2 and 3
 }
 
 struct Drafts {  // a sequence's tokens, in LDS
@@ -92,14 +109,14 @@ struct Drafts {  // a sequence's tokens, in LDS
 };
 
 template <typename T, bool CHAIN, bool SURE>
-__global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyArgs a, const int round, const int rounds) {
+__global__ __launch_bounds__(kThreads, 4) void verify_kernel(const VerifyArgs a, const int round, const int rounds) {
   __shared__ Drafts d;
   __shared__ State st;
   __shared__ int gones;
   __shared__ double wave_total[kWaves];
   __shared__ unsigned slot;
-  __shared__ int chosen, chosen_last, chosen_unit;
-  __shared__ double chosen_before;
+  __shared__ int again, first_unit[kWaves], last_unit[kWaves];
+  __shared__ double unit_before[kWaves];
   const int seq = (int)(blockIdx.x / (unsigned)a.splits), split = (int)(blockIdx.x % (unsigned)a.splits);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   uint64_t seen = 0;
@@ -109,6 +126,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyArgs a, co
   const int n = lo < 0 || hi <= lo ? 0 : (int)(hi - lo < a.most ? hi - lo : a.most);
   if (n == 0) {  // no such sequence: nothing stands, nothing follows
     if (round == 0 && split == 0) {
+#pragma unroll 1
       for (int i = threadIdx.x; i < a.most; i += kThreads) {
         a.path[(int64_t)seq * a.most + i] = -1;
         if (a.token64)
@@ -134,6 +152,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyArgs a, co
 
   // The sequence's drafts into LDS, with what the two rows of their parents hold for them.
   const auto gather = [&]() {
+#pragma unroll 1
     for (int i = threadIdx.x; i < n; i += kThreads) {
       const int64_t x = token_at(i);
       int parent = CHAIN ? i - 1 : a.parents[lo + i];
@@ -147,7 +166,8 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyArgs a, co
   };
   // The first draft from `i` on that follows `node`, or n. One wave.
   const auto child = [&](int node, int i) {
-    if (CHAIN) return node + 1 < n && i <= node + 1 && d.parent[node + 1] == node ? node + 1 : n;
+    if (CHAIN) return i == node + 1 && i < n && d.parent[i] == node ? i : n;
+#pragma unroll 1
     for (int base = i & ~63; base < n; base += 64) {
       const int j = base + lane;
       const uint64_t on = __ballot(j >= i && j < n && d.parent[j] == node);
@@ -155,88 +175,49 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyArgs a, co
     }
     return n;
   };
-  // One wave: goes on from `st` until a row has to be added up, for a rejection or for the token that follows.
-  const auto search = [&](State& s, int& refused, bool writes) {
-    for (;;) {
-      const int j = child(s.node, s.next);
-      if (j >= n) {
-        s.status = kEnd;
-        return;
-      }
-      s.next = j + 1;
-      const float q = SURE ? 1.0f : d.q[j];
-      double w;
-      if (SURE) {
-        bool twice = false;
-        for (int g = lane; g < refused; g += 64) twice |= d.gone[g] == d.token[j];
-        w = __ballot(twice) ? 0.0 : (double)d.p[j];
-      } else {
-        w = weight(d.p[j], q, s.a);
-      }
-      if (__dmul_rn(__dmul_rn(unit_number(d.u[j]), s.s), (double)q) < w) {
-        if (writes && lane == 0) {
-          a.path[(int64_t)seq * a.most + s.count] = j;
-          put_token(s.count - 1, token_at(j));
-        }
-        s.node = j;
-        s.count += 1;
-        s.a = 0.0;
-        s.s = 1.0;
-        refused = 0;
-        continue;
-      }
-      if (SURE) {
-        s.s -= w;
-        if (lane == 0) d.gone[refused] = d.token[j];
-        refused += 1;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        continue;
-      }
-      s.a += s.s;
-      s.status = kRefused;
-      return;
-    }
-  };
-  const auto search_all = [&](bool writes) {  // by the first wave; the state is everybody's afterwards
-    __syncthreads();
-    if (wave == 0) {
-      State s = st;
-      int refused = gones;
-      search(s, refused, writes);
-      if (lane == 0) {
-        st = s;
-        gones = refused;
-      }
-    }
-    __syncthreads();
-  };
 
-  if (round == 0) {
-    gather();
-    if (threadIdx.x == 0) {
-      st = {0, 1, 1, kEnd, 0.0, 1.0};
-      gones = 0;
-      if (split == 0) a.path[(int64_t)seq * a.most] = 0;
-    }
-    search_all(split == 0);
-  } else {
-    if (threadIdx.x == 0) {
-      st = a.states[seq];
-      gones = 0;
-    }
-    __syncthreads();
-    if (st.status == kDone) return;
+  const float chance = a.sample[seq];
+  bool searches = round == 0, writes = split == 0, alone = false;
+  if (searches) gather();
+  if (threadIdx.x == 0) {
+    st = round == 0 ? State{0, 1, 1, kEnd, 0.0, 1.0} : a.states[seq];
+    gones = 0;
+    if (searches && writes) a.path[(int64_t)seq * a.most] = 0;
   }
+  __syncthreads();
+  if (st.status == kDone) return;
+  double* const partial = a.partial + (int64_t)seq * a.units;
+  int from = (split * kWaves + wave) * a.per_wave, step = 1, to = min(from + a.per_wave, a.units);
+  double total = 0.0, before = 0.0, mine = 0.0;  // of the row's sums; of the units before this lane's; of this lane's
+  const int per = (a.units + kThreads - 1) / kThreads, u0 = threadIdx.x * per, u1 = min(u0 + per, a.units);
 
-  // What eight values from v on weigh.
-  const auto weights = [&](const State& s, int v, double (&w)[8]) {
-    float p[8], q[8];
-    eight(target(s.node), v, a.vocab, p);
-    const bool less = !SURE && s.a != 0.0;
-    if (less) eight(draft(s.node), v, a.vocab, q);
+  // The eight values of lane `l` of a unit, and how many of them belong to the lane before: the row's last ones are read from
+  // eight before its end.
+  const auto place = [&](int unit, int& skip) {
+    const int v = unit * kUnit + lane * 8, v0 = min(v, a.vocab - 8);
+    skip = v - v0;
+    return v0;
+  };
+  const auto fetch = [&](int v, Eight<T>& p, Eight<T>& q) {
+    p.load(target(st.node) + v);
+    if (!SURE && st.a != 0.0) q.load(draft(st.node) + v);
+  };
+  const auto weigh = [&](int v, int skip, const Eight<T>& p, const Eight<T>& q, double (&w)[8]) {
+    const double by = st.a;
+    if (!SURE && by != 0.0) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = less ? weight(proper(p[e]), proper(q[e]), s.a) : (double)proper(p[e]);
-    if (SURE && s.status != kWholeRow)
+      for (int e = 0; e < 8; ++e) w[e] = weight(p[e], q[e], by);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = p[e];
+    }
+    if (skip > 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < skip) w[e] = 0.0;
+    }
+    if (SURE && st.status != kWholeRow)
+#pragma unroll 1
       for (int g = 0; g < gones; ++g) {
         const int at = d.gone[g] - v;
 #pragma unroll
@@ -244,148 +225,203 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(const VerifyArgs a, co
           if (at == e) w[e] = 0.0;
       }
   };
-  double* const partial = a.partial + (int64_t)seq * a.units;
-  const auto add_up = [&](int from, int to, int step) {  // the units from, from + step, ... of this wave
-    const State s = st;
-    for (int u = from; u < to; u += step) {
-      double w[8];
-      weights(s, u * kUnit + lane * 8, w);
-      const double sum = wave_sum(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
-      if (lane == 0) __hip_atomic_store(partial + u, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-  };
-  const int w0 = (split * kWaves + wave) * a.per_wave;
-  add_up(w0, min(w0 + a.per_wave, a.units), 1);
-  if (a.splits > 1) {
-    if (!splitk_arrive(a.words + seq, seen, a.splits, &slot)) return;
-  }
-  if (round != 0) gather();
 
-  // The last workgroup of the sequence: the sums of the units, in their order.
   for (;;) {
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    const int per = (a.units + kThreads - 1) / kThreads;
-    const int u0 = threadIdx.x * per, u1 = min(u0 + per, a.units);
-    double mine = 0.0;
-    for (int u = u0; u < u1; ++u) mine += __hip_atomic_load(partial + u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    double upto = mine;
-#pragma unroll
-    for (int s = 1; s < 64; s *= 2) {
-      const double y = __shfl_up(upto, s, 64);
-      if (lane >= s) upto += y;
-    }
-    if (lane == 63) wave_total[wave] = upto;
-    __syncthreads();
-    double total = 0.0, before = upto - mine;
-    for (int w = 0; w < kWaves; ++w) {
-      if (w == wave) before += total;
-      total += wave_total[w];
-    }
-    if (st.status == kRefused) {
-      __syncthreads();
-      if (wave == 0) {  // another child of the node: it is tried against what the rejection leaves
-        const bool more = child(st.node, st.next) < n;
+    bool sums = true;  // whether the row has to be added up
+    if (searches) {
+      if (wave == 0) {  // goes on until a row has to be, for a rejection or for the token that follows
+        State s = st;
+        int refused = gones;
+        bool moved = round == 0 && !alone;
+        for (;;) {
+          const int j = child(s.node, s.next);
+          if (j >= n) {
+            s.status = kEnd;
+            break;
+          }
+          moved = true;
+          s.next = j + 1;
+          const double u = __dmul_rn(unit_number(d.u[j]), s.s);
+          double w;
+          if (SURE) {
+            bool twice = false;
+#pragma unroll 1
+            for (int g = lane; g < refused; g += 64) twice |= d.gone[g] == d.token[j];
+            w = __ballot(twice) ? 0.0 : (double)d.p[j];
+          } else {
+            w = weight(d.p[j], d.q[j], s.a);
+          }
+          if ((SURE ? u : __dmul_rn(u, (double)d.q[j])) < w) {
+            if (writes && lane == 0) {
+              a.path[(int64_t)seq * a.most + s.count] = j;
+              put_token(s.count - 1, d.token[j]);
+            }
+            s.node = j;
+            s.count += 1;
+            s.a = 0.0;
+            s.s = 1.0;
+            refused = 0;
+          } else if (SURE) {
+            s.s -= w;
+            if (lane == 0) d.gone[refused] = d.token[j];
+            refused += 1;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          } else {
+            s.a += s.s;
+            s.status = kRefused;
+            break;
+          }
+        }
         if (lane == 0) {
-          st.s = total;
-          if (!more) st.status = kEnd;
+          st = s;
+          gones = refused;
+          again = moved;
         }
       }
       __syncthreads();
-      if (st.status == kRefused) {
-        search_all(true);
-        if (round + 1 < rounds) {  // the next launch's
-          if (threadIdx.x == 0) a.states[seq] = st;
-          return;
-        }
-        add_up(wave, a.units, kWaves);
-        continue;
+      sums = again;  // not if there was no other draft to try: the row's sums are there
+      if (sums && alone && round + 1 < rounds) {  // the next launch adds it up
+        if (threadIdx.x == 0) a.states[seq] = st;
+        return;
       }
     }
-    if (!(total > 0.0) && st.status != kWholeRow) {  // nothing is left of the row: the target's own
+    if (sums) {
+      // Units kGroup at a time: all their loads, then their sums, which the lanes add up together: a half of them the one,
+      // the other half the other.
+      bool first = true;
+#pragma unroll 1
+      for (int u = from; u < to || first; u += kGroup * step) {
+        Eight<T> p[kGroup], q[kGroup];
+        int skip[kGroup], v[kGroup];
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) {
+          v[j] = place(min(u + j * step, a.units - 1), skip[j]);
+          fetch(v[j], p[j], q[j]);
+        }
+        if (first && round != 0 && !alone) gather();  // beside the loads; the workgroup that goes on with the search needs it
+        first = false;
+        double sum[kGroup];
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) {
+          double w[8];
+          weigh(v[j], skip[j], p[j], q[j], w);
+          sum[j] = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+        }
+        static_assert(kGroup == 2, "the exchange below");
+        const bool upper = lane >= 32;
+        const double all = sum_upto<false>((upper ? sum[1] : sum[0]) + __shfl_xor(upper ? sum[0] : sum[1], 32, 64));
+        const int at = u + (lane >> 5) * step;
+        if ((lane & 31) == 31 && at < to) __hip_atomic_store(partial + at, all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      if (!alone && a.splits > 1 && !splitk_arrive(a.words + seq, seen, a.splits, &slot)) return;
+      // the last workgroup of the sequence: the sums of the units in their order
+      alone = writes = true;
+      from = wave, step = kWaves, to = a.units;
+      __builtin_amdgcn_s_waitcnt(0);
       __syncthreads();
-      if (threadIdx.x == 0) {
+      mine = 0.0;
+#pragma unroll 1
+      for (int u = u0; u < u1; ++u) mine += __hip_atomic_load(partial + u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const double upto = sum_upto<true>(mine);
+      if (lane == 63) wave_total[wave] = upto;
+      __syncthreads();
+      total = 0.0;
+      before = upto - mine;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        if (w == wave) before += total;
+        total += wave_total[w];
+      }
+    }
+    searches = st.status == kRefused;
+    const bool nothing = !(total > 0.0) && st.status == kEnd;
+    __syncthreads();
+    if (!searches && !nothing) break;
+    if (threadIdx.x == 0) {
+      if (searches) {
+        st.s = total;  // what the rejection leaves, for the node's next draft
+      } else {  // nothing is left of the row: the target's own
         st.status = kWholeRow;
         st.a = 0.0;
       }
-      __syncthreads();
-      add_up(wave, a.units, kWaves);
-      continue;
-    }
-    // the unit in which the running sum passes the number, then the value
-    const double level = unit_number(a.sample[seq]) * total;
-    if (threadIdx.x == 0) {
-      chosen = chosen_unit = 0x7FFFFFFF;
-      chosen_last = -1;
     }
     __syncthreads();
-    if (total > 0.0) {
-      double run = before;
-      int found = 0x7FFFFFFF, last = -1;
-      double found_before = 0.0;
-      for (int u = u0; u < u1; ++u) {
-        const double x = __hip_atomic_load(partial + u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (x > 0.0) {
-          last = u;
-          if (found == 0x7FFFFFFF && run + x > level) {
-            found = u;
-            found_before = run;
-          }
+  }
+
+  // the unit in which the running sum passes the number, then the value; the last that weighs if rounding takes the last step
+  const double level = unit_number(chance) * total;
+  const int count = st.count;
+  if (total > 0.0) {
+    int found = kNone, end = -1;
+    double run = before, found_before = 0.0;
+#pragma unroll 1
+    for (int u = u0; u < u1; ++u) {
+      const double x = per == 1 ? mine : __hip_atomic_load(partial + u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (x > 0.0) {
+        end = u;
+        if (found == kNone && run + x > level) {
+          found = u;
+          found_before = run;
         }
-        run += x;
       }
-      if (found != 0x7FFFFFFF) atomicMin(&chosen_unit, found);
-      if (last >= 0) atomicMax(&chosen_last, last);
-      __syncthreads();
-      if (chosen_unit == found && found != 0x7FFFFFFF) chosen_before = found_before;
-      if (threadIdx.x == 0 && chosen_unit == 0x7FFFFFFF) {  // rounding took the last step: the last value that weighs
-        chosen_unit = chosen_last;
-        chosen_before = __builtin_inf();
+      run += x;
+    }
+    const uint64_t on = __ballot(found != kNone), any = __ballot(end >= 0);
+    if (on ? lane == __ffsll((unsigned long long)on) - 1 : any && lane == 63 - __clzll((long long)any)) {
+      first_unit[wave] = found;
+      last_unit[wave] = end;
+      unit_before[wave] = found_before;
+    } else if (!any && lane == 0) {
+      first_unit[wave] = kNone;
+      last_unit[wave] = -1;
+    }
+    __syncthreads();
+    int unit = -1;
+    double sum = -__builtin_inf();
+#pragma unroll
+    for (int w = kWaves - 1; w >= 0; --w) {
+      if (unit < 0) unit = last_unit[w];
+    }
+#pragma unroll
+    for (int w = kWaves - 1; w >= 0; --w) {
+      if (first_unit[w] != kNone) {
+        unit = first_unit[w];
+        sum = unit_before[w];
       }
-      __syncthreads();
-      if (wave == 0) {
-        const State s = st;
-        double w[8];
-        const int v = chosen_unit * kUnit + lane * 8;
-        weights(s, v, w);
-        double own = 0.0;
+    }
+    if (wave == 0) {
+      double w[8];
+      Eight<T> p, q;
+      int skip;
+      const int v = place(unit, skip);
+      fetch(v, p, q);
+      weigh(v, skip, p, q, w);
+      const double own = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+      sum += sum_upto<true>(own) - own;
+      int pick = kNone, final = -1;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) own += w[e];
-        double to = own;
-#pragma unroll
-        for (int step = 1; step < 64; step *= 2) {
-          const double y = __shfl_up(to, step, 64);
-          if (lane >= step) to += y;
+      for (int e = 0; e < 8; ++e) {
+        sum += w[e];
+        if (w[e] > 0.0) {
+          final = v + e;
+          if (pick == kNone && sum > level) pick = v + e;
         }
-        double sum = chosen_before + (to - own);
-        int first = 0x7FFFFFFF, last_one = -1;
-        if (chosen_before == __builtin_inf()) sum = -__builtin_inf();
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          sum += w[e];
-          if (w[e] > 0.0) {
-            last_one = v + e;
-            if (first == 0x7FFFFFFF && sum > level) first = v + e;
-          }
-        }
-        const uint64_t on = __ballot(first != 0x7FFFFFFF), any = __ballot(last_one >= 0);
-        const int pick = on ? __shfl(first, __ffsll((unsigned long long)on) - 1, 64)
-                            : __shfl(last_one, 63 - __clzll((long long)any), 64);
-        if (lane == 0) chosen = pick;
       }
-      __syncthreads();
+      const uint64_t passed = __ballot(pick != kNone), weighs = __ballot(final >= 0);
+      pick = passed ? __shfl(pick, __ffsll((unsigned long long)passed) - 1, 64) : __shfl(final, 63 - __clzll((long long)weighs), 64);
+      if (lane == 0) put_token(count - 1, pick);
     }
-    const int count = st.count;
-    for (int i = count + threadIdx.x; i < a.most; i += kThreads) {
-      a.path[(int64_t)seq * a.most + i] = -1;
-      put_token(i, -1);
-    }
-    if (threadIdx.x == 0) {
-      put_token(count - 1, total > 0.0 ? chosen : -1);
-      a.counts[seq] = count;
-      if (rounds > 1) a.states[seq].status = kDone;
-    }
-    return;
+  } else if (threadIdx.x == 0) {
+    put_token(count - 1, -1);
+  }
+#pragma unroll 1
+  for (int i = count + threadIdx.x; i < a.most; i += kThreads) {
+    a.path[(int64_t)seq * a.most + i] = -1;
+    put_token(i, -1);
+  }
+  if (threadIdx.x == 0) {
+    a.counts[seq] = count;
+    if (rounds > 1) a.states[seq].status = kDone;
   }
 }
 
@@ -395,23 +431,26 @@ using namespace aklr;
 
 namespace {
 
+constexpr int64_t kAtOnce = 512, kMostSplits = 16;
+constexpr int kRounds = 4;
+
 struct Plan {
   int units, splits, per_wave, rounds;
 };
 
-// How many workgroups share a row: one unit a wave until they fill the chip twice over (four of 512 lanes a CU), and at
-// most 255, what an arrival word counts. Only trees whose drafts have rows need more than one sum of a row a sequence;
+// How many workgroups share a row: one unit a wave while that makes no more workgroups than run at once (two of 512 lanes a
+// CU), and at most 255, what an arrival word counts. Only trees whose drafts have rows need more than one sum of a row a sequence;
 // they get `rounds` launches for it, and what is left after those the last workgroup does alone.
 Plan plan_verify(int64_t batch, int64_t vocab, bool chain, bool sure, int64_t most) {
   Plan p;
   p.units = (int)((vocab + kUnit - 1) / kUnit);
   int64_t splits = (p.units + kWaves - 1) / kWaves;
-  const int64_t room = batch < 2048 ? 2048 / batch : 1;
+  const int64_t room = batch < kAtOnce ? kAtOnce / batch : 1;
   if (splits > room) splits = room;
-  if (splits > 255) splits = 255;
+  if (splits > kMostSplits) splits = kMostSplits;
   p.per_wave = (int)((p.units + splits * kWaves - 1) / (splits * kWaves));
   p.splits = (int)((p.units + p.per_wave * kWaves - 1) / (p.per_wave * kWaves));
-  p.rounds = chain || sure || most <= 2 ? 1 : most < 6 ? (int)most - 1 : 5;
+  p.rounds = chain || sure || most <= 2 ? 1 : most <= kRounds ? (int)most - 1 : kRounds;
   return p;
 }
 
@@ -427,7 +466,7 @@ Layout layout_of(int64_t batch, int64_t units) {
 }
 
 bool sizes_ok(int64_t batch, int64_t vocab, int64_t most) {
-  return batch >= 1 && batch <= 65536 && vocab >= 1 && vocab <= (1 << 24) && most >= 1 && most <= kMost;
+  return batch >= 1 && batch <= 65536 && vocab >= 8 && vocab <= (1 << 24) && most >= 1 && most <= kMost;
 }
 
 }  // namespace

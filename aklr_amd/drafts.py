@@ -4,7 +4,7 @@
 parents=None)`` comes after a pass of ``tree_attention_fp8`` over the same query tokens: ``starts[b]`` to
 ``starts[b + 1] - 1`` (int32 [batch + 1], ascending) are sequence b's, the first its last token that stands, the others
 drafts. Drafted token i follows ``parents[i]`` (int32 [tokens], counted within the sequence and before i), or without
-``parents`` the token before it: a chain. ``target_probs`` [tokens, vocabulary] holds the target model's probabilities
+``parents`` the token before it: a chain. ``target_probs`` [tokens, vocabulary] (8 to 2^24 tokens) holds the target model's probabilities
 after each query token, ``draft_probs`` (the same shape and type, bf16, fp16 or fp32) those that the drafts after it were
 drawn from, independently of each other; without it the drafts were certain (a greedy draft, the likeliest tokens).
 
@@ -41,7 +41,7 @@ from .kv_cache import starts_ok
 from .rotary import _DTYPES, stream, tensors_ok, wants_grad
 
 _OOC = FallbackReason.OUT_OF_CONTRACT
-_MOST, _MAX_VOCAB, _MAX_BATCH = 1024, 1 << 24, 65536
+_MOST, _MIN_VOCAB, _MAX_VOCAB, _MAX_BATCH = 1024, 8, 1 << 24, 65536
 
 
 @dataclass
@@ -95,7 +95,7 @@ def _run_verify(p: _VerifyPlan):
     return out, path, counts
 
 
-@api("verify_drafts@1.0", _run_verify)
+@api("verify_drafts@1.0", _run_verify, native="verify")
 def verify_drafts(target_probs, draft_tokens, starts, accept_uniforms, sample_uniforms, most, *, draft_probs=None,
                   parents=None):
     given = [target_probs, draft_tokens, starts, accept_uniforms, sample_uniforms]
@@ -105,7 +105,7 @@ def verify_drafts(target_probs, draft_tokens, starts, accept_uniforms, sample_un
     if isinstance(most, bool) or not isinstance(most, int) or not 1 <= most <= _MOST:
         return _OOC
     tokens, vocab = target_probs.shape
-    if not 1 <= vocab <= _MAX_VOCAB or tokens >= 2**31 or not starts_ok(starts) or starts.numel() > _MAX_BATCH + 1:
+    if not _MIN_VOCAB <= vocab <= _MAX_VOCAB or tokens >= 2**31 or not starts_ok(starts) or starts.numel() > _MAX_BATCH + 1:
         return _OOC
     if draft_probs is not None and not rows_ok(draft_probs, target_probs):
         return _OOC

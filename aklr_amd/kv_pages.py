@@ -84,7 +84,7 @@ def _run_copy(p: _CopyPlan):
     return p.cache
 
 
-@api("kv_cache_copy_pages_fp8@1.0", _run_copy)
+@api("kv_cache_copy_pages_fp8@1.0", _run_copy, native="kv_copy")
 def kv_cache_copy_pages_fp8(k_cache, v_cache, k_scale, v_scale, src, dst):
     cache = (k_cache, v_cache, k_scale, v_scale)
     if not tensors_ok(*cache, src, dst) or src.dim() != 1 or src.numel() >= 2**31:
@@ -129,7 +129,7 @@ def _run_compact(p: _CompactPlan):
     return p.cache
 
 
-@api("kv_cache_compact_fp8@1.0", _run_compact)
+@api("kv_cache_compact_fp8@1.0", _run_compact, native="kv_compact")
 def kv_cache_compact_fp8(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, starts, path, counts):
     cache = (k_cache, v_cache, k_scale, v_scale)
     if not tensors_ok(*cache, block_table, seq_lens, starts, path, counts) or seq_lens.dim() != 1:
@@ -179,7 +179,7 @@ def _run_update(p: _UpdatePlan):
     return table, granted, src, dst
 
 
-@api("kv_cache_update_pages@1.0", _run_update)
+@api("kv_cache_update_pages@1.0", _run_update, native="kv_update")
 def kv_cache_update_pages(page_refs, block_table, lens, new_lens, page_size, parents=None):
     given = [block_table, lens, new_lens] + ([parents] if parents is not None else [])
     if not tensors_ok(page_refs, *given) or page_refs.dim() != 1 or lens.dim() != 1:

@@ -72,7 +72,7 @@ def _run_lora(p: _LoraPlan):
     return out
 
 
-@api("lora_project@1.0", _run_lora)
+@api("lora_project@1.0", _run_lora, native="lora")
 def lora_project(x, a, b, adapters, base, *, scales=None, ranks=None, out=None):
     inputs = [x, a, b, adapters, base] + [t for t in (scales, ranks) if t is not None]
     given = inputs + ([out] if out is not None else [])

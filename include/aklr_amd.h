@@ -401,7 +401,7 @@ int aklr_kv_cache_update_pages(int32_t* page_refs, int64_t pages, const int32_t*
  * outside [0, vocab), or a parent that does not come before it, is passed over, and so are those past `most`.
  * out_tokens (draft_tokens' type) and path [batch, most]: the drafts that stand, then the next token; 0, then the numbers
  * of the drafts that stand; -1 behind counts[b] entries (0 of a sequence without query tokens). tokens: rows of the two
- * tensors, vocab <= 2^24, most <= 1024, batch <= 65536. Workspace: aklr_verify_drafts_workspace_bytes(...), any content.
+ * tensors, 8 <= vocab <= 2^24, most <= 1024, batch <= 65536. Workspace: aklr_verify_drafts_workspace_bytes(...), any content.
  */
 size_t aklr_verify_drafts_workspace_bytes(int64_t batch, int64_t vocab, int64_t most);
 int aklr_verify_drafts(const void* target_probs, int64_t target_stride, const void* draft_probs, int64_t draft_stride,
