@@ -3,6 +3,7 @@
 // The cache is kv_cache.hip's: e4m3fn codes [pages, kv heads, page, head_dim] and fp32 scales [pages, kv heads, page] for
 // keys and for values. Nothing here computes with what it holds; the operators move bytes and count holders.
 #include "common.h"
+#include "scan.h"
 
 AKLR_SCALAR_FP32_BEGIN
 
@@ -299,30 +300,9 @@ __global__ __launch_bounds__(kThreads) void update_hold_kernel(const UpdateArgs 
 
 constexpr int kJoin = 1024;
 
-// Exclusive sum over the workgroup; `total` to all. `sums`: kJoin / 64 words.
-__device__ __forceinline__ int block_before(int x, int* sums, int& total) {
-  int s = x;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int y = __shfl_up(s, d, 64);
-    if ((int)(threadIdx.x & 63) >= d) s += y;
-  }
-  const int wave = threadIdx.x >> 6;
-  __syncthreads();  // the last call's reads are done
-  if ((threadIdx.x & 63) == 63) sums[wave] = s;
-  __syncthreads();
-  int off = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kJoin / 64; ++w) {
-    off += w < wave ? sums[w] : 0;
-    total += sums[w];
-  }
-  return off + s - x;
-}
-
-constexpr int kLdsRows = 4096;  // sequences whose sums are searched in LDS; of more, in memory
+constexpr int kLdsRows = 2048;  // sequences whose sums are searched in LDS; of more, in memory
 constexpr int kScan = 8;        // pages a lane looks at in one round
+constexpr int kRound = kJoin * kScan;
 constexpr int32_t kClaim = INT32_MIN;
 
 // Every atomic before it has been performed, for all lanes of the workgroup.
@@ -334,13 +314,30 @@ __device__ __forceinline__ void settle() {
 // One workgroup for what hangs on an order. A partly kept page that nobody holds any more goes to the lowest of the
 // sequences that keep a part of it (each claims it by an atomic minimum); the others, and all that keep a part of a page
 // somebody still holds, copy it to a new one. New pages are then asked for in the order of sequences and columns, and the
-// k-th asked for is the k-th lowest free page: found by counting zeros in rounds of 8192 pages and, for each, searching
-// whose it is in the sums of what the sequences ask for. Bound by its chain of loads and atomics: a lane keeps what it knows
-// of its first sequence, so that up to 1024 are read once.
+// k-th asked for is the k-th lowest free page: rounds of 8192 pages are counted into a list of the free ones, and a lane
+// takes one that is asked for and searches whose it is in the sums of what the sequences ask for. Bound by its chain of
+// loads and atomics: a lane keeps what it knows of its first sequence, so that up to 1024 are read once, and the first
+// round's counts come beside that: all that changes among them is what this kernel claims, which LDS remembers.
 __global__ __launch_bounds__(kJoin) void update_grow_kernel(const UpdateArgs a) {
   __shared__ int sums[kJoin / 64];
-  __shared__ int32_t lds_before[kLdsRows], lds_begin[kLdsRows];
+  __shared__ int32_t lds_before[kLdsRows], lds_begin[kLdsRows], list[kRound];
+  __shared__ uint8_t claimed[kRound];
   const bool fits = a.batch <= kLdsRows;
+  const auto load_refs = [&](int64_t p0, i32x4 (&x)[2]) {  // past the last page: not 0
+    const int64_t p = p0 + (int)threadIdx.x * kScan;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (p + 4 * h + 4 <= a.pages) {
+        x[h] = *reinterpret_cast<const i32x4*>(a.refs + p + 4 * h);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[h][e] = p + 4 * h + e < a.pages ? a.refs[p + 4 * h + e] : 1;
+      }
+    }
+  };
+  i32x4 counts[2];
+  load_refs(0, counts);
+  *reinterpret_cast<uint64_t*>(claimed + threadIdx.x * kScan) = 0;
   struct Part {
     Row r;
     int page;  // of which a part is kept; -1: none, or one that the cache does not have
@@ -354,6 +351,7 @@ __global__ __launch_bounds__(kJoin) void update_grow_kernel(const UpdateArgs a) 
   Part own{};
   if ((int)threadIdx.x < a.batch) own = read(threadIdx.x);
   const auto part = [&](int b) { return b < kJoin ? own : read(b); };
+#pragma unroll 1
   for (int b = threadIdx.x; b < a.batch; b += kJoin) {
     const Part p = part(b);
     if (p.page < 0) continue;
@@ -362,6 +360,7 @@ __global__ __launch_bounds__(kJoin) void update_grow_kernel(const UpdateArgs a) 
   }
   settle();
   int asked = 0;
+#pragma unroll 1
   for (int b0 = 0; b0 < a.batch; b0 += kJoin) {
     const int b = b0 + threadIdx.x;
     int need = 0, begin = 0;
@@ -369,13 +368,16 @@ __global__ __launch_bounds__(kJoin) void update_grow_kernel(const UpdateArgs a) 
     if (b < a.batch) {
       const Part p = part(b);
       const bool takes = p.page >= 0 && ref_load(a.refs + p.page) == kClaim + b;
-      if (takes) a.out[(int64_t)b * a.cols + p.r.full] = p.page;
+      if (takes) {
+        a.out[(int64_t)b * a.cols + p.r.full] = p.page;
+        if (p.page < kRound) claimed[p.page] = 1;
+      }
       copies = p.page >= 0 && !takes;
       begin = p.r.full + (p.r.part && !copies ? 1 : 0);  // a part of no page stays one of none
       need = max((p.r.want + a.page - 1) / a.page - begin, 0);
     }
     int total;
-    const int off = asked + block_before(need, sums, total);
+    const int off = asked + block_before<kJoin>(need, sums, total);
     asked += total;
     if (b < a.batch) {
       a.begin[b] = begin;
@@ -385,38 +387,50 @@ __global__ __launch_bounds__(kJoin) void update_grow_kernel(const UpdateArgs a) 
     }
   }
   settle();
+#pragma unroll 1
   for (int b = threadIdx.x; b < a.batch; b += kJoin) {  // claims become holders, now that all have read them
     const Part p = part(b);
     if (p.page >= 0 && a.src[b] != -2) __hip_atomic_store(a.refs + p.page, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  settle();
+  if (a.pages > kRound) settle();
   const int32_t* const before = fits ? lds_before : a.before;
   const int32_t* const begin = fits ? lds_begin : a.begin;
   int found = 0;
-  for (int64_t p0 = 0; p0 < a.pages && found < asked; p0 += (int64_t)kJoin * kScan) {
-    const int64_t p = p0 + (int64_t)threadIdx.x * kScan;
+#pragma unroll 1
+  for (int64_t p0 = 0; p0 < a.pages && found < asked; p0 += kRound) {
+    if (p0 > 0) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");  // the claims among them
+      load_refs(p0, counts);
+    }
+    const int at = threadIdx.x * kScan;
     uint32_t free = 0;
 #pragma unroll
     for (int j = 0; j < kScan; ++j)
-      if (p + j < a.pages && ref_load(a.refs + p + j) == 0) free |= 1u << j;
+      if (counts[j / 4][j % 4] == 0 && (p0 > 0 || !claimed[at + j])) free |= 1u << j;
     int total;
-    int k = found + block_before(__popc(free), sums, total);
-    for (; free && k < asked; ++k, free &= free - 1) {
-      const int page = (int)(p + __ffs(free) - 1);
-      int lo = 0, hi = a.batch;  // the last sequence whose first new page is the k-th or before
+    int k = block_before<kJoin>(__popc(free), sums, total);
+#pragma unroll 1
+    for (; free; ++k, free &= free - 1) list[k] = at + __ffs(free) - 1;
+    __syncthreads();
+    const int taken = min(total, asked - found);
+#pragma unroll 1
+    for (int i = threadIdx.x; i < taken; i += kJoin) {
+      const int64_t page = p0 + list[i];
+      int lo = 0, hi = a.batch;  // the last sequence whose first new page is this one or before
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (before[mid] <= k)
+        if (before[mid] <= found + i)
           lo = mid;
         else
           hi = mid;
       }
-      a.out[(int64_t)lo * a.cols + begin[lo] + k - before[lo]] = page;
+      a.out[(int64_t)lo * a.cols + begin[lo] + found + i - before[lo]] = (int)page;
       __hip_atomic_store(a.refs + page, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     found += total;
   }
   settle();
+#pragma unroll 1
   for (int b = threadIdx.x; b < a.batch; b += kJoin) {
     const Part p = part(b);
     const int first = begin[b], got = found - before[b];

@@ -11,6 +11,7 @@
 //
 // Bound by memory: decode by the adapters' weights, prompts by x, base and out (figures at plan_lora).
 #include "common.h"
+#include "scan.h"
 
 AKLR_SCALAR_FP32_BEGIN
 
@@ -47,6 +48,8 @@ struct LoraArgs {
   const float* scales;
   const int32_t* ranks;
   float* part;  // [splits][tokens][rank rounded up to the products' rows]
+  uint16_t* joined;  // [2][tokens][..] pieces, and powers [tokens], of many tokens
+  int32_t* powers;
   int32_t* order;
   Tile* tiles;
   int tokens, k, n, rank, adapters, ids64, splits, k_split, n_group, copies;
@@ -143,15 +146,23 @@ __device__ __forceinline__ bool find_tile(const LoraArgs& a, int id, int (&rows)
 constexpr int kSort = 1024, kHeld = 8;
 __global__ __launch_bounds__(kSort) void sort_kernel(const LoraArgs a, const int tm, const int most) {
   extern __shared__ int32_t counts[];  // [adapters + 1], then where each one's next token goes
-  __shared__ int sums[kSort / 64], tile_sums[kSort / 64];
-  const int groups = a.adapters + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ int sums[kSort / 64];
+  const int groups = a.adapters + 1, lane = threadIdx.x & 63;
   int32_t* const next = counts + groups;
   int g[kHeld];
-  const auto read = [&](int t0) {
+  const auto read = [&](int t0) {  // -1 past the last token
+    const uint32_t* const p = static_cast<const uint32_t*>(a.ids);
+    uint32_t high[kHeld];
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
-      const int t = t0 + i * kSort + threadIdx.x;
-      g[i] = t < a.tokens ? adapter_of(a, t) : -1;
+      const int64_t t = min(t0 + i * kSort + (int)threadIdx.x, a.tokens - 1);
+      g[i] = (int)p[t << a.ids64];
+      high[i] = p[a.ids64 ? 2 * t + 1 : t];
+    }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const bool is = (uint32_t)g[i] < (uint32_t)a.adapters && !(a.ids64 && high[i]);
+      g[i] = t0 + i * kSort + (int)threadIdx.x >= a.tokens ? -1 : is ? g[i] : a.adapters;
     }
   };
   read(0);
@@ -169,27 +180,17 @@ __global__ __launch_bounds__(kSort) void sort_kernel(const LoraArgs a, const int
   }
   __syncthreads();
   int tokens_before = 0, tiles_before = 0;
+#pragma unroll 1
   for (int g0 = 0; g0 < groups; g0 += kSort) {
     const int id = g0 + threadIdx.x, c = id < groups ? counts[id] : 0, tiles = (c + tm - 1) / tm;
-    int s = c, u = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int y = __shfl_up(s, d, 64), z = __shfl_up(u, d, 64);
-      if (lane >= d) s += y, u += z;
-    }
-    __syncthreads();
-    if (lane == 63) sums[wave] = s, tile_sums[wave] = u;
-    __syncthreads();
-    int at = tokens_before + s - c, tile = tiles_before + u - tiles;
-#pragma unroll
-    for (int w = 0; w < kSort / 64; ++w) {
-      at += w < wave ? sums[w] : 0;
-      tile += w < wave ? tile_sums[w] : 0;
-      tokens_before += sums[w];
-      tiles_before += tile_sums[w];
-    }
+    int all, all_tiles;
+    const int at = tokens_before + block_before<kSort>(c, sums, all);
+    const int tile = tiles_before + block_before<kSort>(tiles, sums, all_tiles);
+    tokens_before += all;
+    tiles_before += all_tiles;
     if (id < groups) {
       next[id] = at;
+#pragma unroll 1
       for (int i = 0; i < tiles; ++i) a.tiles[tile + i] = {id, at + i * tm, min(tm, c - i * tm), 0};
     }
   }
@@ -210,11 +211,37 @@ __global__ __launch_bounds__(kSort) void sort_kernel(const LoraArgs a, const int
   }
 }
 
+// Sixteen rows of 64 columns, two 16-byte loads or stores a lane. An operand of the products wants columns 8 g .. + 7 and
+// 32 + 8 g .. + 7 of row li from a lane; half a line of a row an instruction, that is 4.3 TB/s of a copy. As they go to and
+// from memory a lane has the same columns of rows li % 8 and li % 8 + 8, 8 * (g + 4 * (li / 8)) .. + 7, whole lines of eight
+// rows: 4.9 TB/s. The lanes of one and the other trade places by a rotation of their sixteen.
+__device__ __forceinline__ u32x4 other_eight(const u32x4& x) {
+  u32x4 y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x[i], 0x128, 0xF, 0xF, true);  // row_ror:8
+  return y;
+}
+__device__ __forceinline__ u32x4 either(bool first, const u32x4& x, const u32x4& y) {
+  u32x4 z;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) z[i] = first ? x[i] : y[i];
+  return z;
+}
+__device__ __forceinline__ void to_operands(u32x4& x, u32x4& y) {  // from lines: rows li % 8, li % 8 + 8
+  const bool low = !(threadIdx.x & 8);
+  const u32x4 got = other_eight(either(low, y, x));
+  const u32x4 first = either(low, x, got);
+  y = either(low, got, y);
+  x = first;
+}
+__device__ __forceinline__ void to_lines(u32x4& x, u32x4& y) { to_operands(x, y); }  // its own inverse
+
 // v's part of a tile and a range of K. A wave takes 64 of K at a time (whole lines of x's and A's rows), every fourth such
-// piece; NR * 16 rows of A against MT * 16 tokens, both straight from memory: a lane's 16 bytes of a row are its share of an
-// operand. The four waves' sums meet in LDS, in a fixed order.
+// piece; NR * 16 rows of A against MT * 16 tokens, straight from memory into the products. The four waves' sums meet in LDS,
+// in a fixed order. Decode's waves have few pieces: the next one's loads are on their way during one's products; with more
+// tokens a tile the other waves' are (four workgroups a CU).
 template <int MT, int NR, bool F16>
-__global__ __launch_bounds__(kThreads) void shrink_kernel(const LoraArgs a) {
+__global__ __launch_bounds__(kThreads, MT == 1 ? 1 : MT * NR <= 8 ? 4 : MT * NR <= 16 ? 3 : 2) void shrink_kernel(const LoraArgs a) {
   constexpr int TM = 16 * MT;
   __shared__ int rows[TM];
   __shared__ f32x4 meet[2][NR][MT][64];
@@ -229,43 +256,63 @@ __global__ __launch_bounds__(kThreads) void shrink_kernel(const LoraArgs a) {
   if (rank == 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
   const int k0 = blockIdx.y * a.k_split, k1 = min(k0 + a.k_split, a.k);
-  const uint16_t* xr[MT];
-  const uint16_t* ar[NR];
+  const int own = 8 * (g + 4 * (li >> 3));  // the lane's columns of a line
+  const uint16_t *xr[MT][2], *ar[NR][2];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) xr[m] = a.x + rows[m * 16 + li] * a.x_row;
+  for (int h = 0; h < 2; ++h) {
 #pragma unroll
-  for (int r = 0; r < NR; ++r) ar[r] = a.a + adapter * a.a_adapter + min(r * 16 + li, rank - 1) * a.a_row;  // repeated rows are not used
+    for (int m = 0; m < MT; ++m) xr[m][h] = a.x + rows[m * 16 + (li & 7) + 8 * h] * a.x_row + own;
+#pragma unroll
+    for (int r = 0; r < NR; ++r)  // rows past the rank repeat its last; what they give is not used
+      ar[r][h] = a.a + adapter * a.a_adapter + min(r * 16 + (li & 7) + 8 * h, rank - 1) * a.a_row + own;
+  }
   const int used = (rank + 15) / 16;
   struct Piece {
-    u32x4 x[2][MT], w[2][NR];
+    u32x4 x[MT][2], w[NR][2];
   };
   const auto fetch = [&](int k, Piece& p) {
+    const bool on = k + own < k1;  // k % 8 == 0: eight values are inside or past the end
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int at = k + h * 32 + g * 8;
-      const bool on = at < k1;  // k % 8 == 0: eight values are inside or past the end
 #pragma unroll
-      for (int r = 0; r < NR; ++r) p.w[h][r] = on && r < used ? (MT == 1 ? ld16_nt(ar[r] + at) : ld16(ar[r] + at)) : u32x4{0, 0, 0, 0};
+      for (int r = 0; r < NR; ++r)
+        p.w[r][h] = on && r < used ? (MT == 1 ? ld16_nt(ar[r][h] + k) : ld16(ar[r][h] + k)) : u32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int m = 0; m < MT; ++m) p.x[h][m] = on ? ld16(xr[m] + at) : u32x4{0, 0, 0, 0};
+      for (int m = 0; m < MT; ++m) p.x[m][h] = on ? (MT == 1 ? ld16(xr[m][h] + k) : ld16_nt(xr[m][h] + k)) : u32x4{0, 0, 0, 0};
     }
   };
   f32x4 acc[NR][MT] = {};
-  Piece now;
+  const auto multiply = [&](Piece& p) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r) to_operands(p.w[r][0], p.w[r][1]);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      to_operands(p.x[m][0], p.x[m][1]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < NR; ++r) acc[r][m] = product<F16>(p.w[r][h], p.x[m][h], acc[r][m]);
+    }
+  };
   int k = k0 + wave * 64;
-  if (k < k1) fetch(k, now);
-  while (k < k1) {
-    Piece next;
-    const int after = k + 256;
-    if (after < k1) fetch(after, next);
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int r = 0; r < NR; ++r)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) acc[r][m] = product<F16>(now.w[h][r], now.x[h][m], acc[r][m]);
-    now = next;
-    k = after;
+  if constexpr (MT == 1) {
+    Piece now;
+    if (k < k1) fetch(k, now);
+    while (k < k1) {
+      Piece next;
+      const int after = k + 256;
+      if (after < k1) fetch(after, next);
+      multiply(now);
+      now = next;
+      k = after;
+    }
+  } else {
+#pragma unroll 1
+    for (; k < k1; k += 256) {
+      Piece p;
+      fetch(k, p);
+      multiply(p);
+    }
   }
   if (wave >= 2) {
 #pragma unroll
@@ -321,13 +368,66 @@ __device__ __forceinline__ float from16(uint32_t bits) {
     return bf16_lo(bits);
 }
 
+// Four values of v of a token from r on, their parts added in order, as pieces hi[0] | hi[1] << 16 ... fp16 has no room for
+// every v: the largest of a token's becomes 0.5 to 1, by a power of two. R / 4 lanes side by side have one token.
+template <int R, bool F16>
+__device__ __forceinline__ void join_four(const LoraArgs& a, int token, int r, int rank, u32x2& hi, u32x2& lo, int& power) {
+  f32x4 v = {0, 0, 0, 0};
+  if (r < rank) {
+    const float* from = a.part + (int64_t)token * R + r;
+    const int64_t step = (int64_t)a.tokens * R;
+    int s = 0;
+    for (; s + 4 <= a.splits; s += 4) {
+      f32x4 y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = *reinterpret_cast<const f32x4*>(from + (s + e) * step);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v += y[e];
+    }
+    for (; s < a.splits; ++s) v += *reinterpret_cast<const f32x4*>(from + s * step);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (r + e >= rank) v[e] = 0.0f;
+  }
+  power = 0;
+  if constexpr (F16) {
+    float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+    for (int d = 1; d < R / 4; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
+    power = top > 0.0f && top < __builtin_inff() ? __builtin_amdgcn_frexp_expf(top) : 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __builtin_amdgcn_ldexpf(v[j], -power);
+  }
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) pieces<F16>(v[e], h[e], l[e]);
+  hi = u32x2{h[0] | h[1] << 16, h[2] | h[3] << 16};
+  lo = u32x2{l[0] | l[1] << 16, l[2] | l[3] << 16};
+}
+
+// Many tokens: v joined once, not by every workgroup that needs it.
+template <int NR, bool F16>
+__global__ __launch_bounds__(kThreads) void join_kernel(const LoraArgs a) {
+  constexpr int R = 16 * NR;
+  const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int token = (int)min(id / (R / 4), (int64_t)a.tokens - 1), r = (int)(id % (R / 4)) * 4;
+  u32x2 hi, lo;
+  int power;
+  join_four<R, F16>(a, token, r, rank_of(a, adapter_of(a, token)), hi, lo, power);
+  if (id >= (int64_t)a.tokens * (R / 4)) return;
+  *reinterpret_cast<u32x2*>(a.joined + (int64_t)token * R + r) = hi;
+  *reinterpret_cast<u32x2*>(a.joined + ((int64_t)a.tokens + token) * R + r) = lo;
+  if (F16 && r == 0) a.powers[token] = power;
+}
+
 // The outputs of a tile for n_group columns. A wave takes 64 columns at a time, four products' rows: row i of the q-th is
 // column 32 (q / 2) + 8 (i / 4) + 4 (q % 2) + i % 4, so that a lane ends with twice eight columns side by side of one token,
-// and a token's four lanes with half a line of base and out an instruction. B's rows stay in registers for all the tile's
-// tokens; base comes sixteen tokens ahead, the first of it and of B before v's parts.
+// which go to memory as whole lines. B's rows stay in registers for all the tile's tokens; base comes sixteen tokens ahead,
+// the first of it and of B before v.
 template <int MT, int NR, bool F16>
 __global__ __launch_bounds__(kThreads) void expand_kernel(const LoraArgs a) {
   constexpr int TM = 16 * MT, R = 16 * NR, kSteps = (R + 31) / 32, kRow = kSteps * 32 + 8;  // a row of pieces: 16 bytes more
+  constexpr bool kStream = MT == 4;  // base and out pass the caches by
   __shared__ int rows[TM];
   __shared__ __align__(16) uint16_t piece[2][TM][kRow];
   __shared__ int power[TM];
@@ -343,7 +443,7 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(const LoraArgs a) {
         *reinterpret_cast<u32x4*>(a.out + rows[i] * a.out_row + c) = ld16(a.base + rows[i] * a.base_row + c);
     return;
   }
-  const int steps = (rank + 31) / 32;
+  const int steps = (rank + 31) / 32, own = 8 * (g + 4 * (li >> 3));  // the lane's columns of a line
   u32x4 w[kSteps][4], old[2];
   const auto load_w = [&](int c) {
 #pragma unroll
@@ -358,54 +458,45 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(const LoraArgs a) {
   };
   const auto load_old = [&](int c, int m, u32x4 (&o)[2]) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (m * 16 + li < count && c + g * 8 + 32 * h < c1) o[h] = ld16(a.base + rows[m * 16 + li] * a.base_row + c + g * 8 + 32 * h);
+    for (int h = 0; h < 2; ++h) {
+      const int t = m * 16 + (li & 7) + 8 * h;
+      o[h] = u32x4{0, 0, 0, 0};
+      if (t >= count || c + own >= c1) continue;
+      const uint16_t* const from = a.base + rows[t] * a.base_row + c + own;
+      o[h] = kStream ? ld16_nt(from) : ld16(from);
+    }
   };
   int c = c0 + wave * 64;
   if (c < c1) {
     load_w(c);
     load_old(c, 0, old);
   }
-  constexpr int kLanes = R / 4;  // of a token: four values each
+  if constexpr (MT == 1) {
+    constexpr int kLanes = R / 4;
 #pragma unroll
-  for (int i = 0; i < (TM * kLanes + kThreads - 1) / kThreads; ++i) {
-    const int id = i * kThreads + threadIdx.x, t = id / kLanes, r = id % kLanes * 4;
-    if (TM * kLanes % kThreads != 0 && t >= TM) break;
-    f32x4 v = {0, 0, 0, 0};
-    if (t < count && r < rank) {
-      const float* from = a.part + (int64_t)rows[t] * R + r;
-      const int64_t step = (int64_t)a.tokens * R;
-      int s = 0;
-      for (; s + 4 <= a.splits; s += 4) {
-        f32x4 y[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = *reinterpret_cast<const f32x4*>(from + (s + e) * step);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v += y[e];
-      }
-      for (; s < a.splits; ++s) v += *reinterpret_cast<const f32x4*>(from + s * step);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (r + e >= rank) v[e] = 0.0f;
-    }
-    if constexpr (F16) {  // fp16 has no room for every v: the largest of a token's becomes 0.5 to 1, by a power of two
-      float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-#pragma unroll
-      for (int d = 1; d < kLanes; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
-      const int e = top > 0.0f && top < __builtin_inff() ? __builtin_amdgcn_frexp_expf(top) : 0;
+    for (int i = 0; i < (TM * kLanes + kThreads - 1) / kThreads; ++i) {
+      const int id = i * kThreads + threadIdx.x, t = id / kLanes, r = id % kLanes * 4;
+      if (TM * kLanes % kThreads != 0 && t >= TM) break;
+      u32x2 hi, lo;
+      int e;
+      join_four<R, F16>(a, rows[t], r, t < count ? rank : 0, hi, lo, e);
+      *reinterpret_cast<u32x2*>(&piece[0][t][r]) = hi;
+      *reinterpret_cast<u32x2*>(&piece[1][t][r]) = lo;
       if (r == 0) power[t] = e;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = __builtin_amdgcn_ldexpf(v[j], -e);
     }
-    uint32_t hi[4], lo[4];
+  } else {
+    constexpr int kPieces = TM * R / 8;  // of 16 bytes
 #pragma unroll
-    for (int e = 0; e < 4; ++e) pieces<F16>(v[e], hi[e], lo[e]);
-    *reinterpret_cast<u32x2*>(&piece[0][t][r]) = u32x2{hi[0] | hi[1] << 16, hi[2] | hi[3] << 16};
-    *reinterpret_cast<u32x2*>(&piece[1][t][r]) = u32x2{lo[0] | lo[1] << 16, lo[2] | lo[3] << 16};
-    if (R < 32) {  // the products' K is 32
-      *reinterpret_cast<u32x2*>(&piece[0][t][r + R]) = u32x2{0, 0};
-      *reinterpret_cast<u32x2*>(&piece[1][t][r + R]) = u32x2{0, 0};
+    for (int i = 0; i < (2 * kPieces + kThreads - 1) / kThreads; ++i) {
+      const int id = i * kThreads + threadIdx.x, low = id / kPieces, t = id % kPieces / (R / 8), r = id % (R / 8) * 8;
+      if (2 * kPieces % kThreads != 0 && low >= 2) break;
+      *reinterpret_cast<u32x4*>(&piece[low][t][r]) = ld16(a.joined + ((int64_t)low * a.tokens + rows[t]) * R + r);
     }
+    if (F16 && (int)threadIdx.x < TM) power[threadIdx.x] = a.powers[rows[threadIdx.x]];
+  }
+  if (R < 32 && (int)threadIdx.x < TM) {  // the products' K is 32
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(&piece[i / 2][threadIdx.x][R + i % 2 * 8]) = u32x4{0, 0, 0, 0};
   }
   __syncthreads();
   const float scale = a.scales ? a.scales[adapter] : 1.0f;
@@ -440,27 +531,33 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(const LoraArgs a) {
         for (int q = 0; q < 4; ++q) acc[q] = product<F16>(w[s][q], hi, acc[q]);
       }
       if (m + 1 == MT && after < c1) load_w(after);
-      if (m * 16 + li < count) {
-        const int e = F16 ? power[m * 16 + li] : 0;
-        uint16_t* const to = a.out + rows[m * 16 + li] * a.out_row + c + g * 8;
+      const int e = F16 ? power[m * 16 + li] : 0;
+      to_operands(old[0], old[1]);
+      u32x4 word[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (c + g * 8 + 32 * h >= c1) continue;
-          u32x4 word;
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float y[2];
+        for (int j = 0; j < 4; ++j) {
+          float y[2];
 #pragma unroll
-            for (int z = 0; z < 2; ++z) {
-              const int at = 8 * h + 2 * j + z;
-              float d = acc[at / 4][at % 4];
-              if constexpr (F16) d = __builtin_amdgcn_ldexpf(d, e);
-              y[z] = fmaf(d, scale, from16<F16>(z ? old[h][j] >> 16 : old[h][j] & 0xFFFFu));
-            }
-            word[j] = pack_out2(y[0], y[1], F16 ? AKLR_OUT_F16 : AKLR_OUT_BF16);
+          for (int z = 0; z < 2; ++z) {
+            const int at = 8 * h + 2 * j + z;
+            float d = acc[at / 4][at % 4];
+            if constexpr (F16) d = __builtin_amdgcn_ldexpf(d, e);
+            y[z] = fmaf(d, scale, from16<F16>(z ? old[h][j] >> 16 : old[h][j] & 0xFFFFu));
           }
-          *reinterpret_cast<u32x4*>(to + 32 * h) = word;
+          word[h][j] = pack_out2(y[0], y[1], F16 ? AKLR_OUT_F16 : AKLR_OUT_BF16);
         }
+      to_lines(word[0], word[1]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int t = m * 16 + (li & 7) + 8 * h;
+        if (t >= count || c + own >= c1) continue;
+        u32x4* const to = reinterpret_cast<u32x4*>(a.out + rows[t] * a.out_row + c + own);
+        if (kStream)
+          __builtin_nontemporal_store(word[h], to);
+        else
+          *to = word[h];
       }
       old[0] = next[0];
       old[1] = next[1];
@@ -479,7 +576,7 @@ struct Plan {
   int mt, nr;         // tiles of 16 tokens, of 16 rank rows
   int64_t tiles;      // workgroups along x: the most tiles there can be
   int64_t splits, k_split, n_group;
-  size_t order, tile, part, bytes;  // offsets in the workspace
+  size_t order, tile, part, joined, powers, bytes;  // offsets in the workspace
 };
 
 constexpr int64_t kAtOnce = 1024;  // workgroups that run at once, about
@@ -500,7 +597,7 @@ Plan plan_lora(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapt
   p.k_split = up((k + splits - 1) / splits, 256);
   p.splits = (k + p.k_split - 1) / p.k_split;
   int64_t groups_n = (n + 255) / 256, loops = 1;
-  while (loops < 4 && p.tiles * ((groups_n + loops - 1) / loops) > 2 * kAtOnce) loops *= 2;
+  while (loops < 2 && p.tiles * ((groups_n + loops - 1) / loops) > 2 * kAtOnce) loops *= 2;
   p.n_group = 256 * loops;
   size_t at = 0;
   p.order = at;
@@ -508,7 +605,12 @@ Plan plan_lora(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapt
   p.tile = at;
   at += up(16 * p.tiles, 256);
   p.part = at;
-  p.bytes = at + 4 * (size_t)(p.splits * tokens * 16 * p.nr);
+  at += up(4 * p.splits * tokens * 16 * p.nr, 256);
+  p.joined = at;
+  if (sorts) at += up(4 * tokens * 16 * p.nr, 256);
+  p.powers = at;
+  if (sorts) at += up(4 * tokens, 256);
+  p.bytes = at;
   return p;
 }
 
@@ -557,6 +659,8 @@ extern "C" int aklr_lora_project(const void* x, int64_t x_stride, const void* a,
   g.scales = scales;
   g.ranks = ranks;
   g.part = reinterpret_cast<float*>(ws + p.part);
+  g.joined = reinterpret_cast<uint16_t*>(ws + p.joined);
+  g.powers = reinterpret_cast<int32_t*>(ws + p.powers);
   g.order = reinterpret_cast<int32_t*>(ws + p.order);
   g.tiles = reinterpret_cast<Tile*>(ws + p.tile);
   g.tokens = (int)tokens;
@@ -579,6 +683,10 @@ extern "C" int aklr_lora_project(const void* x, int64_t x_stride, const void* a,
     constexpr bool F16 = decltype(f16)::value;
     hipLaunchKernelGGL((shrink_kernel<MT, NR, F16>), shrink, dim3(kThreads), 0, stream, g);
     AKLR_LAUNCH_CHECK();
+    if constexpr (MT > 1) {
+      hipLaunchKernelGGL((join_kernel<NR, F16>), dim3((unsigned)((tokens * NR * 4 + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream, g);
+      AKLR_LAUNCH_CHECK();
+    }
     hipLaunchKernelGGL((expand_kernel<MT, NR, F16>), expand, dim3(kThreads), 0, stream, g);
     AKLR_LAUNCH_CHECK();
     return AKLR_OK;

@@ -13,6 +13,7 @@
 // over the vocabulary, and 32 bits would move some of its borders with the order of the additions. The sums are bound by the
 // loads all the same (figures at plan_verify).
 #include "common.h"
+#include "scan.h"
 
 AKLR_SCALAR_FP32_BEGIN
 
@@ -83,24 +84,6 @@ struct Eight {
     }
   }
 };
-
-// x plus what lane `CTRL` says holds, in the rows of 16 lanes that MASK names (0 from no lane).
-template <int CTRL, int MASK>
-__device__ __forceinline__ double plus_dpp(double x) {
-  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(x), CTRL, MASK, 0xF, true);
-  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(x), CTRL, MASK, 0xF, true);
-  return x + __hiloint2double(hi, lo);
-}
-// The sum of the lanes of a wave's half up to this one; the second half's has the first's with WHOLE.
-template <bool WHOLE>
-__device__ __forceinline__ double sum_upto(double x) {
-  x = plus_dpp<0x111, 0xF>(x);  // row_shr:1
-  x = plus_dpp<0x112, 0xF>(x);
-  x = plus_dpp<0x114, 0xF>(x);
-  x = plus_dpp<0x118, 0xF>(x);
-  x = plus_dpp<0x142, 0xA>(x);  // row_bcast:15 into rows 1 and 3
-  return WHOLE ? plus_dpp<0x143, 0xC>(x) : x;  // row_bcast:31 into rows 2 and 3
-}
 
 struct Drafts {  // a sequence's tokens, in LDS
   int parent[kMost], token[kMost];
