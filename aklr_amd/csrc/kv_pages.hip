@@ -169,74 +169,78 @@ __global__ __launch_bounds__(kThreads) void compact_short_kernel(const CompactAr
 // All items of a launch are independent, so it fills the chip whatever the path; what lies past the window's places, as
 // after a cut that drops more than it keeps, is read once. A workgroup takes kRows items of a sequence, for keys or values.
 constexpr int kRows = 32;
+constexpr int kSavers = 16;  // workgroups of a sequence that look for what to copy aside
 
 template <int D, bool SAVE>
 __global__ __launch_bounds__(kThreads) void compact_long_kernel(const CompactArgs a) {
   constexpr int U = D / 16;
   __shared__ Place from[kRows], to[kRows];
   __shared__ int aside[kRows], any;
-  const int tiles = (a.w1 - a.w0 + kRows - 1) / kRows;
-  const int seq = blockIdx.x / tiles, b = a.b0 + seq;
-  const int i0 = a.w0 + (blockIdx.x - seq * tiles) * kRows;
-  if (SAVE) {  // path ascends: where a tile's first item comes from behind the window, nothing of it is copied aside
-    if (i0 >= a.counts[b] || a.path[(int64_t)b * a.path_row + i0] >= a.w1) return;
-  }
-  if (threadIdx.x < 64) {
-    Place f = {-1, 0}, t = {-1, 0};
-    int source = -1;
-    const int i = i0 + threadIdx.x;
-    if (threadIdx.x < kRows && i < a.w1) item_of(a, b, i, f, t, source);
-    const bool kept = f.page >= 0 && source < a.w1;
-    if (SAVE && !kept) f.page = -1;
-    const uint64_t on = __ballot(f.page >= 0);
-    if (threadIdx.x < kRows) {
-      from[threadIdx.x] = f;
-      to[threadIdx.x] = t;
-      aside[threadIdx.x] = kept;
+  const int tiles = (a.w1 - a.w0 + kRows - 1) / kRows, groups = SAVE ? min(tiles, kSavers) : tiles;
+  const int seq = blockIdx.x / groups, b = a.b0 + seq;
+  for (int tile = blockIdx.x - seq * groups; tile < tiles; tile += groups) {
+    const int i0 = a.w0 + tile * kRows;
+    if (i0 >= a.counts[b]) return;
+    // path ascends: where a tile's first item comes from behind the window, nothing of it or of those behind is copied aside
+    if (SAVE && a.path[(int64_t)b * a.path_row + i0] >= a.w1) return;
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      Place f = {-1, 0}, t = {-1, 0};
+      int source = -1;
+      const int i = i0 + threadIdx.x;
+      if (threadIdx.x < kRows && i < a.w1) item_of(a, b, i, f, t, source);
+      const bool kept = f.page >= 0 && source < a.w1;
+      if (SAVE && !kept) f.page = -1;
+      const uint64_t on = __ballot(f.page >= 0);
+      if (threadIdx.x < kRows) {
+        from[threadIdx.x] = f;
+        to[threadIdx.x] = t;
+        aside[threadIdx.x] = kept;
+      }
+      if (threadIdx.x == 0) any = on != 0;
     }
-    if (threadIdx.x == 0) any = on != 0;
-  }
-  __syncthreads();
-  if (!any) return;
-  const Side& s = blockIdx.y ? a.v : a.k;
-  // the copies' rows: [keys or values][sequence][item of the window][head]
-  const int64_t row0 = ((int64_t)blockIdx.y * a.batch + seq) * (a.w1 - a.w0) + (i0 - a.w0);
-  const int total = kRows * a.heads * U;
-  const auto in_cache = [&](const Place& p, int head, int u) {
-    return s.codes + p.page * s.code_page + ((int64_t)head * a.page + p.off) * D + u * 16;
-  };
-  const auto unit = [&](int id, int& r, int& head, int& u) {  // items of one head side by side
-    u = id % U;
-    r = id / U % kRows;
-    head = id / (U * kRows);
-  };
-  for (int base = threadIdx.x; base < total; base += 4 * kThreads) {
-    u32x4 held[4];
+    __syncthreads();
+    if (!any) continue;
+    const Side& s = blockIdx.y ? a.v : a.k;
+    // the copies' rows: [keys or values][sequence][item of the window][head]
+    const int64_t row0 = ((int64_t)blockIdx.y * a.batch + seq) * (a.w1 - a.w0) + (i0 - a.w0);
+    const int total = kRows * a.heads * U;
+    const auto in_cache = [&](const Place& p, int head, int u) {
+      return s.codes + p.page * s.code_page + ((int64_t)head * a.page + p.off) * D + u * 16;
+    };
+    const auto unit = [&](int id, int& r, int& head, int& u) {  // items of one head side by side
+      u = id % U;
+      r = id / U % kRows;
+      head = id / (U * kRows);
+    };
+    for (int base = threadIdx.x; base < total; base += 4 * kThreads) {
+      u32x4 held[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      int r, head, u;
-      unit(base + j * kThreads, r, head, u);
-      if (base + j * kThreads >= total || from[r].page < 0) continue;
-      held[j] = ld16_nt(!SAVE && aside[r] ? a.saved + ((row0 + r) * a.heads + head) * D + u * 16 : in_cache(from[r], head, u));
-    }
+      for (int j = 0; j < 4; ++j) {
+        int r, head, u;
+        unit(base + j * kThreads, r, head, u);
+        if (base + j * kThreads >= total || from[r].page < 0) continue;
+        held[j] = ld16_nt(!SAVE && aside[r] ? a.saved + ((row0 + r) * a.heads + head) * D + u * 16 : in_cache(from[r], head, u));
+      }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      int r, head, u;
-      unit(base + j * kThreads, r, head, u);
-      if (base + j * kThreads >= total || from[r].page < 0) continue;
-      *reinterpret_cast<u32x4*>(SAVE ? a.saved + ((row0 + r) * a.heads + head) * D + u * 16 : in_cache(to[r], head, u)) = held[j];
+      for (int j = 0; j < 4; ++j) {
+        int r, head, u;
+        unit(base + j * kThreads, r, head, u);
+        if (base + j * kThreads >= total || from[r].page < 0) continue;
+        *reinterpret_cast<u32x4*>(SAVE ? a.saved + ((row0 + r) * a.heads + head) * D + u * 16 : in_cache(to[r], head, u)) = held[j];
+      }
     }
-  }
-  for (int id = threadIdx.x; id < kRows * a.heads; id += kThreads) {
-    const int r = id % kRows, head = id / kRows;
-    if (from[r].page < 0) continue;
-    float* const copy = a.saved_scales + (row0 + r) * a.heads + head;
-    float* const old = s.scales + from[r].page * s.scale_page + (int64_t)head * a.page + from[r].off;
-    float* const now = s.scales + to[r].page * s.scale_page + (int64_t)head * a.page + to[r].off;
-    if (SAVE)
-      *copy = *old;
-    else
-      *now = aside[r] ? *copy : *old;
+    for (int id = threadIdx.x; id < kRows * a.heads; id += kThreads) {
+      const int r = id % kRows, head = id / kRows;
+      if (from[r].page < 0) continue;
+      float* const copy = a.saved_scales + (row0 + r) * a.heads + head;
+      float* const old = s.scales + from[r].page * s.scale_page + (int64_t)head * a.page + from[r].off;
+      float* const now = s.scales + to[r].page * s.scale_page + (int64_t)head * a.page + to[r].off;
+      if (SAVE)
+        *copy = *old;
+      else
+        *now = aside[r] ? *copy : *old;
+    }
   }
 }
 
@@ -497,10 +501,10 @@ int compact(CompactArgs a, int64_t batch, uint8_t* ws, hipStream_t stream) {
       a.w1 = (int)(a.most - w0 < w.items ? a.most : w0 + w.items);
       a.saved = ws;
       a.saved_scales = reinterpret_cast<float*>(ws + 2ll * a.batch * (a.w1 - a.w0) * a.heads * D);
-      const dim3 grid((unsigned)((int64_t)a.batch * ((a.w1 - a.w0 + kRows - 1) / kRows)), 2);
-      hipLaunchKernelGGL((compact_long_kernel<D, true>), grid, dim3(kThreads), 0, stream, a);
+      const int tiles = (a.w1 - a.w0 + kRows - 1) / kRows, savers = tiles < kSavers ? tiles : kSavers;
+      hipLaunchKernelGGL((compact_long_kernel<D, true>), dim3((unsigned)(a.batch * savers), 2), dim3(kThreads), 0, stream, a);
       AKLR_LAUNCH_CHECK();
-      hipLaunchKernelGGL((compact_long_kernel<D, false>), grid, dim3(kThreads), 0, stream, a);
+      hipLaunchKernelGGL((compact_long_kernel<D, false>), dim3((unsigned)(a.batch * tiles), 2), dim3(kThreads), 0, stream, a);
       AKLR_LAUNCH_CHECK();
     }
   }

@@ -23,7 +23,6 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr int kThreads = 256;
 constexpr int kScan = 256;  // tokens that a workgroup looks through by itself
 constexpr int kMostAdapters = 4096;  // what the sort counts in LDS
-constexpr int kIdBits = 13;          // of a token's adapter, one behind them included
 
 template <bool F16>
 __device__ __forceinline__ f32x4 product(const u32x4& a, const u32x4& b, const f32x4& c) {
@@ -80,63 +79,69 @@ __device__ __forceinline__ bool read_tile(const LoraArgs& a, int id, int (&rows)
   return true;
 }
 
-struct Find {  // what looking for a tile takes of LDS
-  uint64_t bits[kThreads / 64][kIdBits];
-  int words[kThreads / 64], counts[kThreads / 64], leader, first;
-};
-
-// The same with few tokens, by the workgroup itself: which tokens have a lane's adapter follows from ballots over the bits of
-// all tokens' numbers. A tile begins at each token that has a whole number of tiles' tokens of its adapter before it, and the
-// tiles are counted in the order of where they begin. `writes`: puts it into the workspace, for the second launch.
+// The same with few tokens, by each wave for itself (no wave waits for another): which tokens have a lane's adapter follows
+// from ballots over the bits of all tokens' numbers. A tile begins at each token that has a whole number of tiles' tokens of
+// its adapter before it, and the tiles are counted in the order of where they begin. `writes`: puts it into the workspace, for
+// the second launch.
 template <int TM>
-__device__ __forceinline__ bool find_tile(const LoraArgs& a, int id, int (&rows)[TM], Find& f, int& adapter, int& count, bool writes) {
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int own = t < a.tokens ? adapter_of(a, t) : (1 << kIdBits) - 1;
+__device__ __forceinline__ bool find_tile(const LoraArgs& a, int id, int (&rows)[TM], int& adapter, int& count, bool writes) {
+  constexpr int kChunks = kScan / 64;
+  const int lane = threadIdx.x & 63, bits = 32 - __builtin_clz(a.adapters), chunks = (a.tokens + 63) / 64;
+  const uint64_t below = (1ull << lane) - 1;
+  int own[kChunks], before[kChunks];
+  uint64_t same[kChunks][kChunks];  // of a token of chunk c: the tokens of chunk d with its adapter
 #pragma unroll
-  for (int i = 0; i < kIdBits; ++i) {
-    const uint64_t on = __ballot(own >> i & 1);
-    if (lane == 0) f.bits[wave][i] = on;
-  }
-  if (t == 0) f.leader = -1;
-  __syncthreads();
-  int before = 0;
-  const int waves = (a.tokens + 63) / 64;
-  for (int w = 0; w < min(waves, wave + 1); ++w) {
-    uint64_t same = w < wave ? ~0ull : (1ull << lane) - 1;
+  for (int c = 0; c < kChunks; ++c) {
+    const int t = c * 64 + lane;
+    own[c] = t < a.tokens ? adapter_of(a, t) : a.adapters;
 #pragma unroll
-    for (int i = 0; i < kIdBits; ++i) same &= f.bits[w][i] ^ ((uint64_t)(own >> i & 1) - 1);
-    before += __popcll(same);
+    for (int d = 0; d <= c; ++d) same[c][d] = __ballot(d * 64 + lane < a.tokens);
   }
-  const bool begins = t < a.tokens && before % TM == 0;
-  const uint64_t on = __ballot(begins);
-  if (lane == 0) f.words[wave] = __popcll(on);
-  __syncthreads();
-  int number = __popcll(on & ((1ull << lane) - 1));
+#pragma unroll 1
+  for (int i = 0; i < bits; ++i) {
+    uint64_t b[kChunks];
 #pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) number += w < wave ? f.words[w] : 0;
-  if (begins && number == id) {
-    f.leader = own;
-    f.first = before;
+    for (int c = 0; c < kChunks; ++c) {
+      if (c >= chunks) break;
+      b[c] = __ballot(own[c] >> i & 1);
+      const uint64_t flip = (uint64_t)(own[c] >> i & 1) - 1;
+#pragma unroll
+      for (int d = 0; d <= c; ++d) same[c][d] &= b[d] ^ flip;
+    }
   }
-  __syncthreads();
-  adapter = f.leader;
+  int left = id, first = -1;
+  adapter = -1;
+#pragma unroll
+  for (int c = 0; c < kChunks; ++c) {
+    before[c] = __popcll(same[c][c] & below);
+#pragma unroll
+    for (int d = 0; d < c; ++d) before[c] += __popcll(same[c][d]);
+    const bool begins = c * 64 + lane < a.tokens && before[c] % TM == 0;
+    const uint64_t all = __ballot(begins), chosen = __ballot(begins && __popcll(all & below) == left);
+    left -= __popcll(all);
+    if (chosen) {
+      const int at = __ffsll((unsigned long long)chosen) - 1;
+      adapter = __builtin_amdgcn_readlane(own[c], at);
+      first = __builtin_amdgcn_readlane(before[c], at);
+    }
+  }
   if (adapter < 0) {
-    if (writes && t == 0) a.tiles[id] = {0, 0, 0, 0};
+    if (writes && threadIdx.x == 0) a.tiles[id] = {0, 0, 0, 0};
     return false;
   }
-  const int at = before - f.first;
-  const bool in = own == adapter && at >= 0 && at < TM;
-  const uint64_t ins = __ballot(in);
-  if (lane == 0) f.counts[wave] = __popcll(ins);
-  if (in) rows[at] = t;
-  __syncthreads();
-  count = f.counts[0] + f.counts[1] + f.counts[2] + f.counts[3];
-  if (t >= count && t < TM) rows[t] = rows[0];
-  __syncthreads();
-  if (writes) {
-    if (t < count) a.order[id * TM + t] = rows[t];
-    if (t == 0) a.tiles[id] = {adapter, id * TM, count, 0};
+  count = 0;
+#pragma unroll
+  for (int c = 0; c < kChunks; ++c) {
+    const int at = before[c] - first;
+    const bool in = c * 64 + lane < a.tokens && own[c] == adapter && at >= 0 && at < TM;
+    count += __popcll(__ballot(in));
+    if (in) rows[at] = c * 64 + lane;
   }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  if (lane >= count && lane < TM) rows[lane] = rows[0];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  if (writes && (int)threadIdx.x < count) a.order[id * TM + threadIdx.x] = rows[threadIdx.x];
+  if (writes && threadIdx.x == 0) a.tiles[id] = {adapter, id * TM, count, 0};
   return true;
 }
 
@@ -241,14 +246,14 @@ __device__ __forceinline__ void to_lines(u32x4& x, u32x4& y) { to_operands(x, y)
 // in a fixed order. Decode's waves have few pieces: the next one's loads are on their way during one's products; with more
 // tokens a tile the other waves' are (four workgroups a CU).
 template <int MT, int NR, bool F16>
-__global__ __launch_bounds__(kThreads, MT == 1 ? 1 : MT * NR <= 8 ? 4 : MT * NR <= 16 ? 3 : 2) void shrink_kernel(const LoraArgs a) {
+__global__ __launch_bounds__(kThreads, MT == 1 ? 1 : MT * NR <= 8 ? 4 : MT * NR <= 16 ? 2 : 1) void shrink_kernel(const LoraArgs a) {
   constexpr int TM = 16 * MT;
-  __shared__ int rows[TM];
+  __shared__ int all_rows[MT == 1 ? kThreads / 64 : 1][TM];
   __shared__ f32x4 meet[2][NR][MT][64];
   int adapter, count;
+  int(&rows)[TM] = all_rows[MT == 1 ? threadIdx.x >> 6 : 0];
   if constexpr (MT == 1) {
-    __shared__ Find find;
-    if (!find_tile<TM>(a, blockIdx.x, rows, find, adapter, count, blockIdx.y == 0)) return;
+    if (!find_tile<TM>(a, blockIdx.x, rows, adapter, count, blockIdx.y == 0)) return;
   } else {
     if (!read_tile<TM>(a, blockIdx.x, rows, adapter, count)) return;
   }
@@ -376,15 +381,15 @@ __device__ __forceinline__ void join_four(const LoraArgs& a, int token, int r, i
   if (r < rank) {
     const float* from = a.part + (int64_t)token * R + r;
     const int64_t step = (int64_t)a.tokens * R;
-    int s = 0;
-    for (; s + 4 <= a.splits; s += 4) {
-      f32x4 y[4];
+    constexpr int kAhead = 8;
+#pragma unroll 1
+    for (int s = 0; s < a.splits; s += kAhead) {
+      f32x4 y[kAhead];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = *reinterpret_cast<const f32x4*>(from + (s + e) * step);
+      for (int e = 0; e < kAhead; ++e) y[e] = *reinterpret_cast<const f32x4*>(from + min(s + e, a.splits - 1) * step);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v += y[e];
+      for (int e = 0; e < kAhead; ++e) v += s + e < a.splits ? y[e] : f32x4{0, 0, 0, 0};
     }
-    for (; s < a.splits; ++s) v += *reinterpret_cast<const f32x4*>(from + s * step);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (r + e >= rank) v[e] = 0.0f;
@@ -579,8 +584,6 @@ struct Plan {
   size_t order, tile, part, joined, powers, bytes;  // offsets in the workspace
 };
 
-constexpr int64_t kAtOnce = 1024;  // workgroups that run at once, about
-
 int64_t up(int64_t v, int64_t q) { return (v + q - 1) / q * q; }
 
 Plan plan_lora(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapters) {
@@ -591,13 +594,14 @@ Plan plan_lora(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapt
   const int64_t tm = 16 * p.mt, groups = adapters + 1 < tokens ? adapters + 1 : tokens;
   const int64_t most = (tokens + tm - 1) / tm + groups;  // sum of ceil(c / tm) over groups of c tokens
   p.tiles = most < tokens ? most : tokens;
-  int64_t splits = kAtOnce / p.tiles;
+  const int64_t at_once = 256 * (p.nr == 8 ? 2 : p.nr == 4 ? 3 : 4);  // as many as the registers leave room for
+  int64_t splits = at_once / p.tiles;
   if (splits > (k + 511) / 512) splits = (k + 511) / 512;
   if (splits < 1) splits = 1;
   p.k_split = up((k + splits - 1) / splits, 256);
   p.splits = (k + p.k_split - 1) / p.k_split;
   int64_t groups_n = (n + 255) / 256, loops = 1;
-  while (loops < 2 && p.tiles * ((groups_n + loops - 1) / loops) > 2 * kAtOnce) loops *= 2;
+  while (loops < 2 && p.tiles * ((groups_n + loops - 1) / loops) > 2048) loops *= 2;
   p.n_group = 256 * loops;
   size_t at = 0;
   p.order = at;
