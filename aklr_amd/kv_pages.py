@@ -8,8 +8,9 @@
   ``counts[b]`` with the numbers ``path[b]`` (int32 [batch, most], ascending) become the first ones: position
   ``seq_lens[b] - T + path[b, i]`` moves to ``seq_lens[b] - T + i``. That is what ``verify_drafts`` returns for the drafts of
   ``tree_attention_fp8``'s call; with T the whole length it cuts a context to the positions worth keeping. Returns the four
-  tensors. Positions in pages that the cache does not have stay, and so does what is not kept, behind. The pages written
-  belong to one sequence (``kv_cache_update_pages`` sees to it).
+  tensors. Positions in pages that the cache does not have stay, and so does what is not kept, behind. The pages that
+  positions move to belong to one sequence. Those behind what ``kv_cache_update_pages`` was last told to keep do; whoever cuts
+  a context whose first pages others hold too copies them before.
 - ``kv_cache_update_pages(page_refs, block_table, lens, new_lens, page_size, parents=None)`` says which pages each sequence
   holds next, for all layers that share a block table. ``page_refs`` (int32 [pages], zeros to begin with) counts the entries
   of block tables, and whoever else, that hold each page; a page with 0 is free. It is updated in place. Sequence b had
@@ -59,6 +60,11 @@ def _cache_ok(cache, *others):
     if not all(apart(cache[i], cache[j]) for i in range(4) for j in range(i)) or not all(apart(c, t) for c in cache for t in others):
         return None
     return strides
+
+
+def _rows_ok(t, batch) -> bool:
+    """An int32 table with a row for each sequence, one of no rows with any strides."""
+    return table_ok(t, batch) or (batch == 0 and t.dtype == torch.int32 and t.dim() == 2 and t.shape[0] == 0)
 
 
 # ---------------------------------------------------------------------------------------------
@@ -135,11 +141,11 @@ def kv_cache_compact_fp8(k_cache, v_cache, k_scale, v_scale, block_table, seq_le
     if not tensors_ok(*cache, block_table, seq_lens, starts, path, counts) or seq_lens.dim() != 1:
         return _OOC
     batch = seq_lens.numel()
-    if batch > _MAX_BATCH or not starts_ok(starts) or starts.numel() != batch + 1 or not table_ok(block_table, batch):
+    if batch > _MAX_BATCH or not starts_ok(starts) or starts.numel() != batch + 1 or not _rows_ok(block_table, batch):
         return _OOC
     if not vector_ok(seq_lens, batch, torch.int32) or not vector_ok(counts, batch, torch.int32):
         return _OOC
-    if not table_ok(path, batch) or path.shape[1] >= 2**31:
+    if not _rows_ok(path, batch) or path.shape[1] >= 2**31:
         return _OOC
     strides = _cache_ok(cache, block_table, seq_lens, starts, path, counts)
     if strides is None or block_table.shape[1] * k_cache.shape[2] > 2**28:
@@ -187,7 +193,7 @@ def kv_cache_update_pages(page_refs, block_table, lens, new_lens, page_size, par
     if isinstance(page_size, bool) or not isinstance(page_size, int) or page_size < 1:
         return _OOC
     batch, pages = lens.numel(), page_refs.numel()
-    if batch > _MAX_BATCH or pages < 1 or pages * page_size >= 2**31 or not table_ok(block_table, batch):
+    if batch > _MAX_BATCH or pages < 1 or pages * page_size >= 2**31 or not _rows_ok(block_table, batch):
         return _OOC
     cols = block_table.shape[1]
     if cols * page_size > 2**28 or batch * cols >= 2**31 or not vector_ok(page_refs, pages, torch.int32) or not aligned(page_refs):

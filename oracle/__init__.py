@@ -11,6 +11,7 @@ This package restates, in numpy, the arithmetic the reference (AMD-AGI/AKLR) def
                rounding;
 - ``layouts``: Preshuffle / ColumnMajor / E8M0Scales (aklr/core/contract/semantics/_layouts.py:20-156);
 - ``moe``:     the grouped DeepSeek FP8 MoE (aklr/plugins/sglang/models/deepseek_v2/reference.py:121-183).
+- ``requests``: verification of drafted tokens, pages of the cache and low-rank adapters, from their definitions;
 - ``cache``:   rotary positions, the FP8 key/value cache and the attention over it, from their definitions (they have
                no counterpart in the reference's scope here).
 
