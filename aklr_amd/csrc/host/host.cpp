@@ -871,7 +871,7 @@ PyObject* kv_compact(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
   const int64_t batch = lens->numel();
   if (batch < 1 || batch > 65536 || !starts_ok(*starts) || starts->numel() != batch + 1 || !table_ok(*table, batch) ||
       table->size(1) < 1 || !vector_ok(*lens, batch, at::kInt) || !vector_ok(*counts, batch, at::kInt) || !table_ok(*path, batch) ||
-      path->size(1) < 1 || path->size(1) >= (int64_t{1} << 31))
+      path->size(1) < 1 || path->size(1) > (int64_t{1} << 28))
     Py_RETURN_NONE;
   if (!c.read(p) || !cache_apart(c, {table, lens, starts, path, counts}) || table->size(1) * c.page > (int64_t{1} << 28)) Py_RETURN_NONE;
   const int64_t most = path->size(1);

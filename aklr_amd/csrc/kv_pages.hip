@@ -548,7 +548,7 @@ extern "C" int aklr_kv_cache_compact_fp8(void* k_codes, void* v_codes, float* k_
                                          const int32_t* counts, int64_t batch, int64_t kv_heads, int64_t head_dim,
                                          int64_t pages, int64_t page_size, void* workspace, size_t workspace_bytes,
                                          hipStream_t stream) {
-  if (!shape_ok(pages, page_size, kv_heads, head_dim) || batch < 0 || batch > 65536 || most < 0 || most > 0x7FFFFFFF ||
+  if (!shape_ok(pages, page_size, kv_heads, head_dim) || batch < 0 || batch > 65536 || most < 0 || most > (1 << 28) ||
       table_cols < 0 || table_cols * page_size > (1 << 28) || table_stride < table_cols || path_stride < most)
     return AKLR_ERR_INVALID_ARGUMENT;
   if (!side_ok(k_codes, k_scales, k_page, ks_page, kv_heads, head_dim, page_size) ||

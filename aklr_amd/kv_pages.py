@@ -145,7 +145,7 @@ def kv_cache_compact_fp8(k_cache, v_cache, k_scale, v_scale, block_table, seq_le
         return _OOC
     if not vector_ok(seq_lens, batch, torch.int32) or not vector_ok(counts, batch, torch.int32):
         return _OOC
-    if not _rows_ok(path, batch) or path.shape[1] >= 2**31:
+    if not _rows_ok(path, batch) or path.shape[1] > 2**28:
         return _OOC
     strides = _cache_ok(cache, block_table, seq_lens, starts, path, counts)
     if strides is None or block_table.shape[1] * k_cache.shape[2] > 2**28:

@@ -159,6 +159,22 @@ def test_rows_of_no_probabilities():
     check(p)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_probabilities_below_the_normal_range(dtype):
+    say(f"verify subnormal {dtype}")
+    tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    p = torch.zeros((3, 2000), dtype=dtype, device=DEV)
+    p[:, [3, 700, 1999]] = torch.tensor([1.0, 2.0, 5.0], device=DEV).mul(tiny).to(dtype)
+    q = torch.zeros_like(p)
+    q[:, 700] = 3 * tiny
+    for v in (0.0, 0.125, 0.374, 0.375, 0.5, 0.99):
+        for u in (0.0, 0.66, 0.67):
+            case = {"target": p, "draft": q, "tokens": torch.tensor([0, 700, 700], device=DEV), "parents": None, "most": 3, "v": torch.tensor([v], device=DEV),
+                    "u": torch.full((3,), u, device=DEV), "starts": torch.tensor([0, 3], dtype=torch.int32, device=DEV)}
+            check(case, (u, v))
+            check({**case, "draft": None}, (u, v))
+
+
 def test_drafts_that_are_passed_over():
     say("verify: tokens outside the vocabulary, parents that do not come before, more tokens than most, numbers that are none")
     for form in ("tree", "certain"):

@@ -259,6 +259,7 @@ def test_entry_points_reject_before_any_launch(native_lib):
     size = L.aklr_kv_cache_compact_fp8_workspace_bytes
     assert size(7, 64, 8, 128) == 0 and size(1, 65, 1, 64) == 2 * 65 * 68
     assert compact(batch=1, most=65, path_stride=65) == 3 and compact(batch=1, most=65, path_stride=65, ws=p, nbytes=2 * 65 * 68 - 1) == 3
+    assert compact(batch=1, most=(1 << 28) + 1, path_stride=1 << 30) == 1
     for b, most, h, d in ((1, 1 << 20, 1, 64), (65536, 100, 1, 64), (64, 8192, 8, 128), (3, 1 << 30, 1024, 256), (1, 65, 1024, 256)):
         assert 0 < size(b, most, h, d) <= 128 << 20 and size(b, most, h, d) % (2 * h * (d + 4)) == 0
 
