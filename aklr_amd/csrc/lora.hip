@@ -51,7 +51,7 @@ struct LoraArgs {
   int32_t* powers;
   int32_t* order;
   Tile* tiles;
-  int tokens, k, n, rank, adapters, ids64, splits, k_split, n_group, copies;
+  int tokens, k, n, rank, adapters, ids64, splits, k_split, n_group, copies, part_row;
 };
 
 // A token's adapter, `adapters` where it has none.
@@ -151,7 +151,7 @@ __device__ __forceinline__ bool find_tile(const LoraArgs& a, int id, int (&rows)
 constexpr int kSort = 1024, kHeld = 8;
 __global__ __launch_bounds__(kSort) void sort_kernel(const LoraArgs a, const int tm, const int most) {
   extern __shared__ int32_t counts[];  // [adapters + 1], then where each one's next token goes
-  __shared__ int sums[kSort / 64];
+  __shared__ int2 sums[kSort / 64];  // tokens, tiles
   const int groups = a.adapters + 1, lane = threadIdx.x & 63;
   int32_t* const next = counts + groups;
   int g[kHeld];
@@ -188,11 +188,19 @@ __global__ __launch_bounds__(kSort) void sort_kernel(const LoraArgs a, const int
 #pragma unroll 1
   for (int g0 = 0; g0 < groups; g0 += kSort) {
     const int id = g0 + threadIdx.x, c = id < groups ? counts[id] : 0, tiles = (c + tm - 1) / tm;
-    int all, all_tiles;
-    const int at = tokens_before + block_before<kSort>(c, sums, all);
-    const int tile = tiles_before + block_before<kSort>(tiles, sums, all_tiles);
-    tokens_before += all;
-    tiles_before += all_tiles;
+    const int c_upto = sum_upto<true>(c), tiles_upto = sum_upto<true>(tiles), wave = threadIdx.x >> 6;
+    __syncthreads();  // the last round's reads are done
+    if (lane == 63) sums[wave] = int2{c_upto, tiles_upto};
+    __syncthreads();
+    int at = tokens_before + c_upto - c, tile = tiles_before + tiles_upto - tiles;
+#pragma unroll
+    for (int w = 0; w < kSort / 64; ++w) {
+      const int2 x = sums[w];
+      at += w < wave ? x.x : 0;
+      tile += w < wave ? x.y : 0;
+      tokens_before += x.x;
+      tiles_before += x.y;
+    }
     if (id < groups) {
       next[id] = at;
 #pragma unroll 1
@@ -241,12 +249,12 @@ __device__ __forceinline__ void to_operands(u32x4& x, u32x4& y) {  // from lines
 }
 __device__ __forceinline__ void to_lines(u32x4& x, u32x4& y) { to_operands(x, y); }  // its own inverse
 
-// v's part of a tile and a range of K. A wave takes 64 of K at a time (whole lines of x's and A's rows), every fourth such
-// piece; NR * 16 rows of A against MT * 16 tokens, straight from memory into the products. The four waves' sums meet in LDS,
-// in a fixed order. Decode's waves have few pieces: the next one's loads are on their way during one's products; with more
-// tokens a tile the other waves' are (four workgroups a CU).
+// v's part of a tile, a range of K and up to 64 rows of A (ranges of K first along blockIdx.y). A wave takes 64 of K at a time (whole lines of x's and
+// A's rows), every fourth such piece; NR * 16 rows of A against MT * 16 tokens, straight from memory into the products. The
+// four waves' sums meet in LDS, in a fixed order. Where a SIMD has few waves, or a wave few pieces (decode), the next one's
+// loads are on their way during one's products; else the other waves' are.
 template <int MT, int NR, bool F16>
-__global__ __launch_bounds__(kThreads, MT == 1 ? 1 : MT * NR <= 8 ? 4 : MT * NR <= 16 ? 2 : 1) void shrink_kernel(const LoraArgs a) {
+__global__ __launch_bounds__(kThreads, MT == 1 ? 1 : MT * NR <= 8 ? 4 : 2) void shrink_kernel(const LoraArgs a) {
   constexpr int TM = 16 * MT;
   __shared__ int all_rows[MT == 1 ? kThreads / 64 : 1][TM];
   __shared__ f32x4 meet[2][NR][MT][64];
@@ -257,10 +265,11 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 1 : MT * NR <= 8 ? 4 : MT * NR 
   } else {
     if (!read_tile<TM>(a, blockIdx.x, rows, adapter, count)) return;
   }
-  const int rank = rank_of(a, adapter);
-  if (rank == 0) return;
+  const int rank_group = NR == 4 ? blockIdx.y / a.splits : 0, split = blockIdx.y - rank_group * a.splits;
+  const int r0 = rank_group * 16 * NR, rank = rank_of(a, adapter) - r0;
+  if (rank <= 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
-  const int k0 = blockIdx.y * a.k_split, k1 = min(k0 + a.k_split, a.k);
+  const int k0 = split * a.k_split, k1 = min(k0 + a.k_split, a.k);
   const int own = 8 * (g + 4 * (li >> 3));  // the lane's columns of a line
   const uint16_t *xr[MT][2], *ar[NR][2];
 #pragma unroll
@@ -269,7 +278,7 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 1 : MT * NR <= 8 ? 4 : MT * NR 
     for (int m = 0; m < MT; ++m) xr[m][h] = a.x + rows[m * 16 + (li & 7) + 8 * h] * a.x_row + own;
 #pragma unroll
     for (int r = 0; r < NR; ++r)  // rows past the rank repeat its last; what they give is not used
-      ar[r][h] = a.a + adapter * a.a_adapter + min(r * 16 + (li & 7) + 8 * h, rank - 1) * a.a_row + own;
+      ar[r][h] = a.a + adapter * a.a_adapter + (r0 + min(r * 16 + (li & 7) + 8 * h, rank - 1)) * a.a_row + own;
   }
   const int used = (rank + 15) / 16;
   struct Piece {
@@ -300,7 +309,7 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 1 : MT * NR <= 8 ? 4 : MT * NR 
     }
   };
   int k = k0 + wave * 64;
-  if constexpr (MT == 1) {
+  if constexpr (MT == 1 || MT * NR > 8) {
     Piece now;
     if (k < k1) fetch(k, now);
     while (k < k1) {
@@ -341,11 +350,11 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 1 : MT * NR <= 8 ? 4 : MT * NR 
   }
   __syncthreads();
   if (wave == 0) {  // a lane has rows 16 r + 4 g .. + 3 of token li
-    float* const to = a.part + (int64_t)blockIdx.y * a.tokens * (NR * 16);
+    float* const to = a.part + (int64_t)split * a.tokens * a.part_row + r0;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       if (m * 16 + li >= count) continue;
-      const int64_t row = (int64_t)rows[m * 16 + li] * (NR * 16) + 4 * g;
+      const int64_t row = (int64_t)rows[m * 16 + li] * a.part_row + 4 * g;
 #pragma unroll
       for (int r = 0; r < NR; ++r) *reinterpret_cast<f32x4*>(to + row + 16 * r) = acc[r][m] + meet[0][r][m][lane];
     }
@@ -410,7 +419,7 @@ __device__ __forceinline__ void join_four(const LoraArgs& a, int token, int r, i
   lo = u32x2{l[0] | l[1] << 16, l[2] | l[3] << 16};
 }
 
-// Many tokens: v joined once, not by every workgroup that needs it.
+// Where many workgroups need the same parts of v: joined once, not by each of them.
 template <int NR, bool F16>
 __global__ __launch_bounds__(kThreads) void join_kernel(const LoraArgs a) {
   constexpr int R = 16 * NR;
@@ -429,10 +438,12 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const LoraArgs a) {
 // column 32 (q / 2) + 8 (i / 4) + 4 (q % 2) + i % 4, so that a lane ends with twice eight columns side by side of one token,
 // which go to memory as whole lines. B's rows stay in registers for all the tile's tokens; base comes sixteen tokens ahead,
 // the first of it and of B before v.
-template <int MT, int NR, bool F16>
+enum Mode : int { kParts, kJoined, kStreamed };  // v from its parts, joined, and with base and out passing the caches by
+
+template <int MT, int NR, bool F16, Mode MODE>
 __global__ __launch_bounds__(kThreads) void expand_kernel(const LoraArgs a) {
   constexpr int TM = 16 * MT, R = 16 * NR, kSteps = (R + 31) / 32, kRow = kSteps * 32 + 8;  // a row of pieces: 16 bytes more
-  constexpr bool kStream = MT == 4;  // base and out pass the caches by
+  constexpr bool kStream = MODE == kStreamed;
   __shared__ int rows[TM];
   __shared__ __align__(16) uint16_t piece[2][TM][kRow];
   __shared__ int power[TM];
@@ -443,9 +454,21 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(const LoraArgs a) {
   const int c0 = blockIdx.y * a.n_group, c1 = min(c0 + a.n_group, a.n);
   if (rank == 0) {
     if (!a.copies) return;
-    for (int i = 0; i < count; ++i)
-      for (int c = c0 + 8 * threadIdx.x; c < c1; c += 8 * kThreads)
-        *reinterpret_cast<u32x4*>(a.out + rows[i] * a.out_row + c) = ld16(a.base + rows[i] * a.base_row + c);
+    constexpr int kAhead = 4;
+    const int units = (c1 - c0) / 8, all = count * units;  // n % 8 == 0
+    for (int u0 = threadIdx.x; u0 < all; u0 += kAhead * kThreads) {
+      u32x4 held[kAhead];
+      uint16_t* to[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int u = min(u0 + i * kThreads, all - 1), t = rows[u / units], c = c0 + u % units * 8;
+        held[i] = ld16(a.base + t * a.base_row + c);
+        to[i] = a.out + t * a.out_row + c;
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (u0 + i * kThreads < all) *reinterpret_cast<u32x4*>(to[i]) = held[i];
+    }
     return;
   }
   const int steps = (rank + 31) / 32, own = 8 * (g + 4 * (li >> 3));  // the lane's columns of a line
@@ -476,7 +499,7 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(const LoraArgs a) {
     load_w(c);
     load_old(c, 0, old);
   }
-  if constexpr (MT == 1) {
+  if constexpr (MODE == kParts) {
     constexpr int kLanes = R / 4;
 #pragma unroll
     for (int i = 0; i < (TM * kLanes + kThreads - 1) / kThreads; ++i) {
@@ -580,9 +603,14 @@ namespace {
 struct Plan {
   int mt, nr;         // tiles of 16 tokens, of 16 rank rows
   int64_t tiles;      // workgroups along x: the most tiles there can be
-  int64_t splits, k_split, n_group;
+  int64_t splits, k_split, n_group, rank_groups;
+  bool joins;         // v's parts by a launch of their own
   size_t order, tile, part, joined, powers, bytes;  // offsets in the workspace
 };
+
+// What reading v's parts in every workgroup that needs them may cost: the launch that joins them takes 3 to 5 us, in which the
+// caches give some 20 MB.
+constexpr int64_t kJoinBytes = 20 << 20;
 
 int64_t up(int64_t v, int64_t q) { return (v + q - 1) / q * q; }
 
@@ -594,8 +622,8 @@ Plan plan_lora(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapt
   const int64_t tm = 16 * p.mt, groups = adapters + 1 < tokens ? adapters + 1 : tokens;
   const int64_t most = (tokens + tm - 1) / tm + groups;  // sum of ceil(c / tm) over groups of c tokens
   p.tiles = most < tokens ? most : tokens;
-  const int64_t at_once = 256 * (p.nr == 8 ? 2 : p.nr == 4 ? 3 : 4);  // as many as the registers leave room for
-  int64_t splits = at_once / p.tiles;
+  p.rank_groups = p.nr == 8 ? 2 : 1;
+  int64_t splits = 256 * (p.nr < 4 ? 4 : p.mt < 4 ? 3 : 2) / (p.tiles * p.rank_groups);  // as many workgroups as the registers leave room for
   if (splits > (k + 511) / 512) splits = (k + 511) / 512;
   if (splits < 1) splits = 1;
   p.k_split = up((k + splits - 1) / splits, 256);
@@ -603,6 +631,7 @@ Plan plan_lora(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapt
   int64_t groups_n = (n + 255) / 256, loops = 1;
   while (loops < 2 && p.tiles * ((groups_n + loops - 1) / loops) > 2048) loops *= 2;
   p.n_group = 256 * loops;
+  p.joins = sorts && p.splits * tokens * 64 * p.nr * ((n + p.n_group - 1) / p.n_group) > kJoinBytes;
   size_t at = 0;
   p.order = at;
   at += up(4 * (sorts ? tokens : p.tiles * tm), 256);
@@ -611,9 +640,9 @@ Plan plan_lora(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapt
   p.part = at;
   at += up(4 * p.splits * tokens * 16 * p.nr, 256);
   p.joined = at;
-  if (sorts) at += up(4 * tokens * 16 * p.nr, 256);
+  if (p.joins) at += up(4 * tokens * 16 * p.nr, 256);
   p.powers = at;
-  if (sorts) at += up(4 * tokens, 256);
+  if (p.joins) at += up(4 * tokens, 256);
   p.bytes = at;
   return p;
 }
@@ -677,21 +706,32 @@ extern "C" int aklr_lora_project(const void* x, int64_t x_stride, const void* a,
   g.k_split = (int)p.k_split;
   g.n_group = (int)p.n_group;
   g.copies = base != out;
+  g.part_row = 16 * p.nr;
+  const auto whole_lines = [](const void* q, int64_t stride) { return reinterpret_cast<uintptr_t>(q) % 128 == 0 && stride % 64 == 0; };
+  const bool streams = whole_lines(base, base_stride) && whole_lines(out, out_stride);
   if (tokens > kScan) {
     hipLaunchKernelGGL(sort_kernel, dim3(1), dim3(kSort), 8 * (adapter_count + 1), stream, g, 16 * p.mt, (int)p.tiles);
     AKLR_LAUNCH_CHECK();
   }
-  const dim3 shrink((unsigned)p.tiles, (unsigned)p.splits), expand((unsigned)p.tiles, (unsigned)((n + p.n_group - 1) / p.n_group));
+  const dim3 shrink((unsigned)p.tiles, (unsigned)(p.splits * p.rank_groups)), expand((unsigned)p.tiles, (unsigned)((n + p.n_group - 1) / p.n_group));
   const auto go = [&](auto mt, auto nr, auto f16) -> int {
     constexpr int MT = decltype(mt)::value, NR = decltype(nr)::value;
     constexpr bool F16 = decltype(f16)::value;
-    hipLaunchKernelGGL((shrink_kernel<MT, NR, F16>), shrink, dim3(kThreads), 0, stream, g);
+    hipLaunchKernelGGL((shrink_kernel<MT, NR == 8 ? 4 : NR, F16>), shrink, dim3(kThreads), 0, stream, g);
     AKLR_LAUNCH_CHECK();
     if constexpr (MT > 1) {
-      hipLaunchKernelGGL((join_kernel<NR, F16>), dim3((unsigned)((tokens * NR * 4 + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream, g);
-      AKLR_LAUNCH_CHECK();
+      if (p.joins) {
+        hipLaunchKernelGGL((join_kernel<NR, F16>), dim3((unsigned)((tokens * NR * 4 + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream, g);
+        AKLR_LAUNCH_CHECK();
+        if (MT == 4 && streams)
+          hipLaunchKernelGGL((expand_kernel<MT, NR, F16, MT == 4 ? kStreamed : kJoined>), expand, dim3(kThreads), 0, stream, g);
+        else
+          hipLaunchKernelGGL((expand_kernel<MT, NR, F16, kJoined>), expand, dim3(kThreads), 0, stream, g);
+        AKLR_LAUNCH_CHECK();
+        return AKLR_OK;
+      }
     }
-    hipLaunchKernelGGL((expand_kernel<MT, NR, F16>), expand, dim3(kThreads), 0, stream, g);
+    hipLaunchKernelGGL((expand_kernel<MT, NR, F16, kParts>), expand, dim3(kThreads), 0, stream, g);
     AKLR_LAUNCH_CHECK();
     return AKLR_OK;
   };
