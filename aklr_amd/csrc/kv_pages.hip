@@ -316,7 +316,7 @@ __device__ __forceinline__ void settle() {
 }
 
 // One workgroup for what hangs on an order. A partly kept page that nobody holds any more goes to the lowest of the
-// sequences that keep a part of it (each claims it by an atomic minimum); the others, and all that keep a part of a page
+// sequences that keep a part of it (each claims it, by an atomic minimum where another has); the others, and all that keep a part of a page
 // somebody still holds, copy it to a new one. New pages are then asked for in the order of sequences and columns, and the
 // k-th asked for is the k-th lowest free page: rounds of 8192 pages are counted into a list of the free ones, and a lane
 // takes one that is asked for and searches whose it is in the sums of what the sequences ask for. Bound by its chain of
@@ -359,8 +359,8 @@ __global__ __launch_bounds__(kJoin) void update_grow_kernel(const UpdateArgs a) 
   for (int b = threadIdx.x; b < a.batch; b += kJoin) {
     const Part p = part(b);
     if (p.page < 0) continue;
-    const int32_t n = ref_load(a.refs + p.page);
-    if (n == 0 || (n < 0 && n < kClaim + a.batch)) atomicMin(a.refs + p.page, kClaim + b);
+    const int32_t n = atomicCAS(a.refs + p.page, 0, kClaim + b);
+    if (n < 0 && n < kClaim + a.batch) atomicMin(a.refs + p.page, kClaim + b);
   }
   settle();
   int asked = 0;

@@ -149,7 +149,6 @@ __global__ __launch_bounds__(kThreads, 4) void verify_kernel(const VerifyArgs a,
   };
   // The first draft from `i` on that follows `node`, or n. One wave.
   const auto child = [&](int node, int i) {
-    if (CHAIN) return i == node + 1 && i < n && d.parent[i] == node ? i : n;
 #pragma unroll 1
     for (int base = i & ~63; base < n; base += 64) {
       const int j = base + lane;
@@ -212,7 +211,39 @@ __global__ __launch_bounds__(kThreads, 4) void verify_kernel(const VerifyArgs a,
   for (;;) {
     bool sums = true;  // whether the row has to be added up
     if (searches) {
-      if (wave == 0) {  // goes on until a row has to be, for a rejection or for the token that follows
+      if (CHAIN && wave == 0) {  // every draft is its node's only one: all are tried at once, up to the first that falls
+        int last = n - 1;  // the node at which the chain ends, and whether a draft after it was refused
+        bool falls = false;
+#pragma unroll 1
+        for (int base = 0; base < n; base += 64) {
+          const int j = base + lane;
+          const bool on = j > 0 && j < n, tried = on && d.parent[j] >= 0;
+          const double u = on ? unit_number(d.u[j]) : 0.0, p = on ? d.p[j] : 0.0, q = SURE || !on ? 1.0 : d.q[j];
+          const bool stands = tried && __dmul_rn(u, q) < p;
+          const uint64_t ends = __ballot(on && !stands), refused = __ballot(tried);
+          const int end = ends ? base + __ffsll((unsigned long long)ends) - 1 : n;
+          if (writes && on && j < end) {
+            a.path[(int64_t)seq * a.most + j] = j;
+            put_token(j - 1, d.token[j]);
+          }
+          if (ends) {
+            last = end - 1;
+            falls = refused >> (end - base) & 1;
+            break;
+          }
+        }
+        if (lane == 0) {
+          st.node = last;
+          st.count = last + 1;
+          st.a = !SURE && falls ? 1.0 : 0.0;
+          if (SURE && falls) {
+            d.gone[0] = d.token[last + 1];
+            gones = 1;
+          }
+          again = true;
+        }
+      }
+      if (!CHAIN && wave == 0) {  // goes on until a row has to be added up, for a rejection or for the token that follows
         State s = st;
         int refused = gones;
         bool moved = round == 0 && !alone;
@@ -316,7 +347,7 @@ __global__ __launch_bounds__(kThreads, 4) void verify_kernel(const VerifyArgs a,
         total += wave_total[w];
       }
     }
-    searches = st.status == kRefused;
+    searches = !CHAIN && !SURE && st.status == kRefused;
     const bool nothing = !(total > 0.0) && st.status == kEnd;
     __syncthreads();
     if (!searches && !nothing) break;
