@@ -608,30 +608,35 @@ struct Plan {
   size_t order, tile, part, joined, powers, bytes;  // offsets in the workspace
 };
 
-// What reading v's parts in every workgroup that needs them may cost: the launch that joins them takes 3 to 5 us, in which the
-// caches give some 20 MB.
-constexpr int64_t kJoinBytes = 20 << 20;
-
 int64_t up(int64_t v, int64_t q) { return (v + q - 1) / q * q; }
 
+// The plan of a call, from its sizes alone. Measured on 8 adapters, bf16, us (both sides of each choice):
+// - up to 256 tokens each wave looks for its tile: 120 tokens of 4096 x 4096, rank 16: 9.6 (sorted: 14.8), 250: 11.0 (15.7).
+// - 64 tokens a tile from 7168 tokens on, 32 below: 8191 of 8192 x 10240, rank 32: 120 (32 a tile: 131), rank 64: 142 (163); 6000
+//   of 4096 x 4096, rank 16: 46 (64 a tile: 53), 6269 of 840 x 5512: 55 (57), 3000 and fewer the same.
+// - as many ranges of K as make the workgroups that run at once, of at least 512: 192 tokens of 48 adapters, 8192 x 10240, rank 64:
+//   29.2 (11 ranges), 29.4 (8), 30.9 (16). That call is bound by the adapters' weights, 66 MB in 14.5 + 15.5 us.
+// - 256 columns a workgroup, 512 where that makes more than 2048: the same call 29.2 (256: 30.4, 1024: 31.5), 8191 of 8192 x
+//   10240 120 (256: 123, 1024: 122).
+// - v joined by a launch of its own (3 to 5 us) where workgroups would read and convert much of it again and again, a conversion
+//   about as much as eight parts' reads: 8191 of 8192 x 10240, rank 32: 120 (from its parts 129), of 4096 x 4096, rank 128: 107 (114),
+//   3000 of 4096 x 4096, rank 64: 42.5 (joined 43.9), rank 16: 30.9 (34.4).
 Plan plan_lora(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapters) {
   Plan p{};
   p.nr = rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8;
+  p.rank_groups = p.nr == 8 ? 2 : 1;
   const bool sorts = tokens > kScan;
-  p.mt = !sorts ? 1 : tokens < 2048 ? 2 : 4;
+  p.mt = !sorts ? 1 : tokens < 7168 ? 2 : 4;
   const int64_t tm = 16 * p.mt, groups = adapters + 1 < tokens ? adapters + 1 : tokens;
   const int64_t most = (tokens + tm - 1) / tm + groups;  // sum of ceil(c / tm) over groups of c tokens
   p.tiles = most < tokens ? most : tokens;
-  p.rank_groups = p.nr == 8 ? 2 : 1;
-  int64_t splits = 256 * (p.nr < 4 ? 4 : p.mt < 4 ? 3 : 2) / (p.tiles * p.rank_groups);  // as many workgroups as the registers leave room for
+  int64_t splits = 256 * (p.nr < 4 ? 4 : p.mt < 4 ? 3 : 2) / (p.tiles * p.rank_groups);  // by what registers leave room for
   if (splits > (k + 511) / 512) splits = (k + 511) / 512;
   if (splits < 1) splits = 1;
   p.k_split = up((k + splits - 1) / splits, 256);
   p.splits = (k + p.k_split - 1) / p.k_split;
-  int64_t groups_n = (n + 255) / 256, loops = 1;
-  while (loops < 2 && p.tiles * ((groups_n + loops - 1) / loops) > 2048) loops *= 2;
-  p.n_group = 256 * loops;
-  p.joins = sorts && p.splits * tokens * 64 * p.nr * ((n + p.n_group - 1) / p.n_group) > kJoinBytes;
+  p.n_group = p.tiles * ((n + 255) / 256) > 2048 ? 512 : 256;
+  p.joins = sorts && tokens * 16 * p.nr * ((n + p.n_group - 1) / p.n_group) * (p.splits + 8) > 70000000;
   size_t at = 0;
   p.order = at;
   at += up(4 * (sorts ? tokens : p.tiles * tm), 256);

@@ -69,6 +69,24 @@ def test_sizes(t, k, n, r, count, dtype):
         check(call(p), p, kind)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("t,k,n,r,count", [(7168, 72, 40, 16, 3), (7301, 136, 2056, 128, 5), (7200, 264, 2048, 128, 9), (9000, 1032, 4104, 64, 2),
+                                           (4000, 512, 4096, 128, 3), (8000, 136, 72, 24, 4000), (7999, 2056, 520, 8, 1), (16400, 72, 4096, 32, 7)])
+def test_many_tokens(t, k, n, r, count, dtype):
+    # the oracle on some of the rows; all rows of tokens without an adapter
+    say(f"lora many {t} {k} {n} {r} {count} {dtype}")
+    for kind in ("mixed", "runs"):
+        p = problem(t, k, n, r, count, dtype, t + k, kind)
+        p["ranks"] = torch.arange(count, dtype=torch.int32, device=DEV) % (r + 1)
+        p["ranks"][-1] = r
+        got = call(p)
+        none = (p["ids"] < 0) | (p["ranks"][p["ids"].clamp(min=0)] == 0)
+        assert torch.equal(got[none], p["base"][none])
+        rows = torch.from_numpy(np.r_[0, t - 1, np.random.RandomState(1).choice(t, 250, replace=False)]).to(DEV)
+        check(got[rows], {**p, "x": p["x"][rows], "ids": p["ids"][rows], "base": p["base"][rows]}, kind)
+        assert bool(got.isfinite().all()) and torch.equal(call({**p, "base": p["base"].clone()}, out=p["base"]), got)
+
+
 @pytest.mark.parametrize("t", [3, 40, 250, 600, 2300])
 def test_who_has_which(t):
     say(f"lora adapters {t}")
@@ -88,7 +106,7 @@ def test_who_has_which(t):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("t,r", [(9, 8), (70, 24), (200, 128), (400, 64), (2300, 16), (2100, 128)])
+@pytest.mark.parametrize("t,r", [(9, 8), (70, 24), (200, 128), (400, 64), (2300, 16), (2100, 128), (7200, 64)])
 def test_ranks_and_what_lies_behind_them(t, r, dtype):
     say(f"lora ranks {t} {r} {dtype}")
     p = problem(t, 264, 136, r, 12, dtype, 7)
@@ -104,7 +122,7 @@ def test_ranks_and_what_lies_behind_them(t, r, dtype):
     assert torch.equal(call({**p, "ranks": odd}), want)
 
 
-@pytest.mark.parametrize("t", [20, 200, 500, 2100])
+@pytest.mark.parametrize("t", [20, 200, 500, 2100, 7300])
 def test_views_and_places(t):
     say(f"lora views {t}")
     k, n, r, count = 136, 72, 16, 4
@@ -132,7 +150,7 @@ def test_views_and_places(t):
 
 def test_a_result_does_not_hang_on_its_place():
     say("lora: tokens in another order, among others, twice")
-    for t in (60, 250, 700, 2600):
+    for t in (60, 250, 700, 2600, 7400):
         p = problem(t, 520, 264, 32, 6, BF16, 10)
         want = call(p)
         assert torch.equal(call(p), want)
@@ -141,7 +159,7 @@ def test_a_result_does_not_hang_on_its_place():
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("t", [20, 300, 2100])
+@pytest.mark.parametrize("t", [20, 300, 7300])
 def test_values_that_are_not_finite_stay_with_their_token(t, dtype):
     say(f"lora values {t} {dtype}")
     p = problem(t, 136, 72, 24, 3, dtype, 11, "one")
@@ -206,7 +224,7 @@ def test_offsets_past_32_bits():
 
 def test_captured_and_on_streams():
     say("lora: captured, replayed with other values between eager calls; two streams at once")
-    for t in (40, 250, 700, 2100):
+    for t in (40, 250, 700, 7200):
         ps = [problem(t, 264, 136, 32, 5, BF16, s) for s in range(30, 33)]
         p = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in ps[0].items()}
         torch.cuda.synchronize()
