@@ -1,7 +1,8 @@
 // Low-rank adapters of many requests beside a projection that all share: out[t] = base[t] + s_a (x[t] A_a^T) B_a^T with
 // a = adapters[t], A_a [rank, K], B_a [N, rank]. gfx950 only.
 //
-// Two launches over tiles of up to 16 * MT tokens of one adapter, so that its weights are read once a tile:
+// Two launches over tiles of up to 16 * MT tokens of one adapter, so that its weights are read once a tile (what many
+// workgroups of the second would convert again is joined by one between them):
 //   shrink  v[t, r] = sum_k x[t, k] A[r, k], K split over workgroups (fp32 parts in the workspace) and over a workgroup's
 //           four waves, on 16x16x32 products with the adapter's rows as one operand and tokens as the other;
 //   expand  the parts added in their order, v as two 16-bit pieces (hi + lo: what is left of v's rounding is 2^-17 of it
@@ -249,10 +250,11 @@ __device__ __forceinline__ void to_operands(u32x4& x, u32x4& y) {  // from lines
 }
 __device__ __forceinline__ void to_lines(u32x4& x, u32x4& y) { to_operands(x, y); }  // its own inverse
 
-// v's part of a tile, a range of K and up to 64 rows of A (ranges of K first along blockIdx.y). A wave takes 64 of K at a time (whole lines of x's and
-// A's rows), every fourth such piece; NR * 16 rows of A against MT * 16 tokens, straight from memory into the products. The
-// four waves' sums meet in LDS, in a fixed order. Where a SIMD has few waves, or a wave few pieces (decode), the next one's
-// loads are on their way during one's products; else the other waves' are.
+// v's part of a tile, a range of K and up to 64 rows of A (ranges of K first along blockIdx.y). A wave takes 64 of K at a
+// time (whole lines of x's and A's rows), every fourth such piece; NR * 16 rows of A against MT * 16 tokens, straight from
+// memory into the products. The four waves' sums meet in LDS, in a fixed order. Where a SIMD has few waves, or a wave few
+// pieces (decode), the next one's loads are on their way during one's products; else the other waves' are. Bound by memory:
+// 8191 tokens of 8192, 134 MB of x, in 33 us, 4.1 TB/s; 192 tokens of 48 adapters, 50 MB of A, in 14.7 us, 3.4 TB/s.
 template <int MT, int NR, bool F16>
 __global__ __launch_bounds__(kThreads, MT == 1 ? 1 : MT * NR <= 8 ? 4 : 2) void shrink_kernel(const LoraArgs a) {
   constexpr int TM = 16 * MT;
@@ -405,10 +407,12 @@ __device__ __forceinline__ void join_four(const LoraArgs& a, int token, int r, i
   }
   power = 0;
   if constexpr (F16) {
-    float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+    float top = 0.0f;  // of the finite ones
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = fmaxf(top, __builtin_isfinite(v[j]) ? fabsf(v[j]) : 0.0f);
 #pragma unroll
     for (int d = 1; d < R / 4; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
-    power = top > 0.0f && top < __builtin_inff() ? __builtin_amdgcn_frexp_expf(top) : 0;
+    power = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = __builtin_amdgcn_ldexpf(v[j], -power);
   }
@@ -437,7 +441,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const LoraArgs a) {
 // The outputs of a tile for n_group columns. A wave takes 64 columns at a time, four products' rows: row i of the q-th is
 // column 32 (q / 2) + 8 (i / 4) + 4 (q % 2) + i % 4, so that a lane ends with twice eight columns side by side of one token,
 // which go to memory as whole lines. B's rows stay in registers for all the tile's tokens; base comes sixteen tokens ahead,
-// the first of it and of B before v.
+// the first of it and of B before v. Bound by memory: 8191 tokens of 10240, 336 MB of base and out, in 76 us, 4.4 TB/s.
 enum Mode : int { kParts, kJoined, kStreamed };  // v from its parts, joined, and with base and out passing the caches by
 
 template <int MT, int NR, bool F16, Mode MODE>
@@ -479,7 +483,8 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(const LoraArgs a) {
       const int r0 = s * 32 + g * 8;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int n = min(c + (q >> 1) * 32 + (li >> 2) * 8 + (q & 1) * 4 + (li & 3), a.n - 1);  // those past the end are not stored
+        // those past the end are not stored
+        const int n = min(c + (q >> 1) * 32 + (li >> 2) * 8 + (q & 1) * 4 + (li & 3), a.n - 1);
         w[s][q] = r0 < rank ? ld16(a.b + adapter * a.b_adapter + n * a.b_row + r0) : u32x4{0, 0, 0, 0};
       }
     }
@@ -612,15 +617,15 @@ int64_t up(int64_t v, int64_t q) { return (v + q - 1) / q * q; }
 
 // The plan of a call, from its sizes alone. Measured on 8 adapters, bf16, us (both sides of each choice):
 // - up to 256 tokens each wave looks for its tile: 120 tokens of 4096 x 4096, rank 16: 9.6 (sorted: 14.8), 250: 11.0 (15.7).
-// - 64 tokens a tile from 7168 tokens on, 32 below: 8191 of 8192 x 10240, rank 32: 120 (32 a tile: 131), rank 64: 142 (163); 6000
-//   of 4096 x 4096, rank 16: 46 (64 a tile: 53), 6269 of 840 x 5512: 55 (57), 3000 and fewer the same.
-// - as many ranges of K as make the workgroups that run at once, of at least 512: 192 tokens of 48 adapters, 8192 x 10240, rank 64:
-//   29.2 (11 ranges), 29.4 (8), 30.9 (16). That call is bound by the adapters' weights, 66 MB in 14.5 + 15.5 us.
+// - 64 tokens a tile from 7168 tokens on, 32 below: 8191 of 8192 x 10240, rank 32: 120 (32 a tile: 131), rank 64: 142
+//   (163); 6000 of 4096 x 4096, rank 16: 46 (64 a tile: 53), 6269 of 840 x 5512: 55 (57), 3000 and fewer the same.
+// - as many ranges of K as make the workgroups that run at once, of at least 512: 192 tokens of 48 adapters, 8192 x 10240,
+//   rank 64: 29.2 (11 ranges), 29.4 (8), 30.9 (16). That call is bound by the adapters' weights, 66 MB in 14.5 + 15.5 us.
 // - 256 columns a workgroup, 512 where that makes more than 2048: the same call 29.2 (256: 30.4, 1024: 31.5), 8191 of 8192 x
 //   10240 120 (256: 123, 1024: 122).
-// - v joined by a launch of its own (3 to 5 us) where workgroups would read and convert much of it again and again, a conversion
-//   about as much as eight parts' reads: 8191 of 8192 x 10240, rank 32: 120 (from its parts 129), of 4096 x 4096, rank 128: 107 (114),
-//   3000 of 4096 x 4096, rank 64: 42.5 (joined 43.9), rank 16: 30.9 (34.4).
+// - v joined by a launch of its own (3 to 5 us) where workgroups would read and convert much of it again and again, a
+//   conversion about as much as eight parts' reads: 8191 of 8192 x 10240, rank 32: 120 (from its parts 129), of 4096 x
+//   4096, rank 128: 107 (114), 3000 of 4096 x 4096, rank 64: 42.5 (joined 43.9), rank 16: 30.9 (34.4).
 Plan plan_lora(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapters) {
   Plan p{};
   p.nr = rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8;
@@ -657,7 +662,9 @@ bool sizes_ok(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapte
          rank >= 8 && rank <= 128 && rank % 8 == 0 && adapters >= 1 && adapters <= kMostAdapters;
 }
 
-bool row_ok(const void* p, int64_t stride, int64_t least) { return p && aklr_aligned16(p) && stride % 8 == 0 && stride >= least; }
+bool row_ok(const void* p, int64_t stride, int64_t least) {
+  return p && aklr_aligned16(p) && stride % 8 == 0 && stride >= least;
+}
 
 }  // namespace
 
@@ -712,13 +719,16 @@ extern "C" int aklr_lora_project(const void* x, int64_t x_stride, const void* a,
   g.n_group = (int)p.n_group;
   g.copies = base != out;
   g.part_row = 16 * p.nr;
-  const auto whole_lines = [](const void* q, int64_t stride) { return reinterpret_cast<uintptr_t>(q) % 128 == 0 && stride % 64 == 0; };
+  const auto whole_lines = [](const void* q, int64_t stride) {
+    return reinterpret_cast<uintptr_t>(q) % 128 == 0 && stride % 64 == 0;
+  };
   const bool streams = whole_lines(base, base_stride) && whole_lines(out, out_stride);
   if (tokens > kScan) {
     hipLaunchKernelGGL(sort_kernel, dim3(1), dim3(kSort), 8 * (adapter_count + 1), stream, g, 16 * p.mt, (int)p.tiles);
     AKLR_LAUNCH_CHECK();
   }
-  const dim3 shrink((unsigned)p.tiles, (unsigned)(p.splits * p.rank_groups)), expand((unsigned)p.tiles, (unsigned)((n + p.n_group - 1) / p.n_group));
+  const dim3 shrink((unsigned)p.tiles, (unsigned)(p.splits * p.rank_groups));
+  const dim3 expand((unsigned)p.tiles, (unsigned)((n + p.n_group - 1) / p.n_group));
   const auto go = [&](auto mt, auto nr, auto f16) -> int {
     constexpr int MT = decltype(mt)::value, NR = decltype(nr)::value;
     constexpr bool F16 = decltype(f16)::value;
@@ -726,7 +736,8 @@ extern "C" int aklr_lora_project(const void* x, int64_t x_stride, const void* a,
     AKLR_LAUNCH_CHECK();
     if constexpr (MT > 1) {
       if (p.joins) {
-        hipLaunchKernelGGL((join_kernel<NR, F16>), dim3((unsigned)((tokens * NR * 4 + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream, g);
+        const dim3 grid((unsigned)((tokens * NR * 4 + kThreads - 1) / kThreads));
+        hipLaunchKernelGGL((join_kernel<NR, F16>), grid, dim3(kThreads), 0, stream, g);
         AKLR_LAUNCH_CHECK();
         if (MT == 4 && streams)
           hipLaunchKernelGGL((expand_kernel<MT, NR, F16, MT == 4 ? kStreamed : kJoined>), expand, dim3(kThreads), 0, stream, g);
@@ -741,7 +752,10 @@ extern "C" int aklr_lora_project(const void* x, int64_t x_stride, const void* a,
     return AKLR_OK;
   };
   const auto by_rank = [&](auto mt, auto f16) -> int {
-    return p.nr == 1 ? go(mt, IC<1>{}, f16) : p.nr == 2 ? go(mt, IC<2>{}, f16) : p.nr == 4 ? go(mt, IC<4>{}, f16) : go(mt, IC<8>{}, f16);
+    return p.nr == 1   ? go(mt, IC<1>{}, f16)
+           : p.nr == 2 ? go(mt, IC<2>{}, f16)
+           : p.nr == 4 ? go(mt, IC<4>{}, f16)
+                       : go(mt, IC<8>{}, f16);
   };
   const auto by_rows = [&](auto f16) -> int {
     return p.mt == 1 ? by_rank(IC<1>{}, f16) : p.mt == 2 ? by_rank(IC<2>{}, f16) : by_rank(IC<4>{}, f16);

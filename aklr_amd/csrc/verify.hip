@@ -422,7 +422,8 @@ __global__ __launch_bounds__(kThreads, 4) void verify_kernel(const VerifyArgs a,
         }
       }
       const uint64_t passed = __ballot(pick != kNone), weighs = __ballot(final >= 0);
-      pick = passed ? __shfl(pick, __ffsll((unsigned long long)passed) - 1, 64) : __shfl(final, 63 - __clzll((long long)weighs), 64);
+      pick = passed ? __shfl(pick, __ffsll((unsigned long long)passed) - 1, 64)
+                    : __shfl(final, 63 - __clzll((long long)weighs), 64);
       if (lane == 0) put_token(count - 1, pick);
     }
   } else if (threadIdx.x == 0) {
@@ -453,8 +454,16 @@ struct Plan {
 };
 
 // How many workgroups share a row: one unit a wave while that makes no more workgroups than run at once (two of 512 lanes a
-// CU), and at most 255, what an arrival word counts. Only trees whose drafts have rows need more than one sum of a row a sequence;
-// they get `rounds` launches for it, and what is left after those the last workgroup does alone.
+// CU), and at most 16: they arrive by atomics on one word, which wait for each other. Only trees whose drafts have rows need
+// more than one sum of a row a sequence; they get up to four launches for it, and what is left after those the last workgroup
+// does alone, at the rate of one CU (15 us for two rows of 128003 floats). Measured, fp32, us (both sides of each choice):
+// - 16 trees of 33 tokens, vocabulary 128003: 33 with 16 workgroups a row; 44 with 4, 38 with 8, 76 with 32. 64 chains of
+//   8, vocabulary 131072: 18.2 with any of them, 67 MB of rows at 3.7 TB/s. 4 chains of 5, vocabulary 32000: 8.1.
+// - the same trees in 3 launches 42, 4: 30 to 33, 5: 36, 8: 36. A sequence adds up 1.6 rows at the mean, 3 or 4 at the most; a
+//   launch that finds its sequences done takes 1.3.
+// - four units' loads in flight a wave instead of two no longer fit the registers.
+// What bounds a call of few sequences is its chain of dependent loads, starts, then parents and tokens, then what the rows hold
+// for them, then the rows, at 0.8 to 2 us each, and the 64-bit tail: a lone wave issues a vector instruction every five cycles.
 Plan plan_verify(int64_t batch, int64_t vocab, bool chain, bool sure, int64_t most) {
   Plan p;
   p.units = (int)((vocab + kUnit - 1) / kUnit);

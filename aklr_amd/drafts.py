@@ -4,9 +4,9 @@
 parents=None)`` comes after a pass of ``tree_attention_fp8`` over the same query tokens: ``starts[b]`` to
 ``starts[b + 1] - 1`` (int32 [batch + 1], ascending) are sequence b's, the first its last token that stands, the others
 drafts. Drafted token i follows ``parents[i]`` (int32 [tokens], counted within the sequence and before i), or without
-``parents`` the token before it: a chain. ``target_probs`` [tokens, vocabulary] (8 to 2^24 tokens) holds the target model's probabilities
-after each query token, ``draft_probs`` (the same shape and type, bf16, fp16 or fp32) those that the drafts after it were
-drawn from, independently of each other; without it the drafts were certain (a greedy draft, the likeliest tokens).
+``parents`` the token before it: a chain. ``target_probs`` [tokens, vocabulary] (8 to 2^24 tokens) holds the target model's
+probabilities after each query token, ``draft_probs`` (the same shape and type, bf16, fp16 or fp32) those that the drafts
+after it were drawn from, independently of each other; without it the drafts were certain (a greedy draft, the likeliest tokens).
 
   At a node with rows p and q its drafts are tried in their order, from W = p, S = 1. Draft i with token x stands if
   ``accept_uniforms[i]`` * S * q(x) < W(x) (without q: < W(x) alone), and the search goes on at it; else

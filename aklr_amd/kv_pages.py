@@ -57,7 +57,9 @@ def _cache_ok(cache, *others):
     strides = cache_strides(*cache)
     if strides is None or not on_gpu(*cache, *others):
         return None
-    if not all(apart(cache[i], cache[j]) for i in range(4) for j in range(i)) or not all(apart(c, t) for c in cache for t in others):
+    if not all(apart(cache[i], cache[j]) for i in range(4) for j in range(i)):
+        return None
+    if not all(apart(c, t) for c in cache for t in others):
         return None
     return strides
 
@@ -196,7 +198,9 @@ def kv_cache_update_pages(page_refs, block_table, lens, new_lens, page_size, par
     if batch > _MAX_BATCH or pages < 1 or pages * page_size >= 2**31 or not _rows_ok(block_table, batch):
         return _OOC
     cols = block_table.shape[1]
-    if cols * page_size > 2**28 or batch * cols >= 2**31 or not vector_ok(page_refs, pages, torch.int32) or not aligned(page_refs):
+    if cols * page_size > 2**28 or batch * cols >= 2**31:
+        return _OOC
+    if not vector_ok(page_refs, pages, torch.int32) or not aligned(page_refs):
         return _OOC
     if not all(vector_ok(t, batch, torch.int32) for t in (lens, new_lens, parents) if t is not None):
         return _OOC

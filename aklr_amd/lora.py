@@ -12,7 +12,8 @@
   contiguous and everything else lies on 16 bytes. ``out``: where the result goes, base itself for in place.
 
   x a^T is held in 32 bits and enters the second product as two 16-bit pieces, which keep 2^-17 (bf16) or 2^-23 (fp16, of the
-  token's largest) of it; base is added in fp32, and the sum rounded once.
+  token's largest) of it; base is added in fp32, and the sum rounded once. What is not finite in a token or in its adapter
+  comes out not finite, an infinity perhaps as NaN, and no other token sees it.
 
 Nothing waits for the GPU, and a captured call serves other adapters of the same shapes. Calls it does not serve return a
 ``FallbackReason``; so does a call that wants gradients or tangents. The reference has no such op in this library's scope.
@@ -83,11 +84,15 @@ def lora_project(x, a, b, adapters, base, *, scales=None, ranks=None, out=None):
         return _OOC
     if tokens > 2**20 or not 1 <= count <= 4096:
         return _OOC
-    if not _pieces_ok(x, x.dtype, tokens, k) or not _pieces_ok(a, x.dtype, count, rank, k) or not _pieces_ok(b, x.dtype, count, n, rank):
+    if not _pieces_ok(x, x.dtype, tokens, k) or not _pieces_ok(a, x.dtype, count, rank, k):
+        return _OOC
+    if not _pieces_ok(b, x.dtype, count, n, rank):
         return _OOC
     if not _pieces_ok(base, x.dtype, tokens, n) or not vector_ok(adapters, tokens, torch.int32, torch.int64):
         return _OOC
-    if scales is not None and not vector_ok(scales, count, torch.float32) or ranks is not None and not vector_ok(ranks, count, torch.int32):
+    if scales is not None and not vector_ok(scales, count, torch.float32):
+        return _OOC
+    if ranks is not None and not vector_ok(ranks, count, torch.int32):
         return _OOC
     if not on_gpu(*given) or wants_grad(x, a, b, base, scales, out):
         return _OOC

@@ -178,6 +178,21 @@ def test_values_that_are_not_finite_stay_with_their_token(t, dtype):
     assert torch.equal(got, want2)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("t", [20, 300, 7300])
+def test_an_infinite_weight_beside_large_values(t, dtype):
+    say(f"lora infinite weight {t} {dtype}")
+    p = problem(t, 136, 72, 24, 3, dtype, 15)
+    p["x"], p["a"][1] = p["x"] * 2.0**12, p["a"][1] * 2.0**12  # v of 2^24, past fp16
+    p["x"][p["x"] == 0], p["b"][p["b"] == 0], p["scales"][1] = 1, 1, 0.5
+    want = call(p)
+    hit = p["ids"] == 1
+    p["a"][1, 7, 5] = float("inf")
+    got = call(p)
+    assert hit.any() and torch.equal(got[~hit], want[~hit])
+    assert torch.equal(got[hit], (p["x"][hit][:, 5:6].sign() * p["b"][1, :, 7].sign() * float("inf")).to(dtype))
+
+
 @pytest.mark.parametrize("t", [20, 300])
 def test_large_and_small_values(t):
     # products of 2^15 and more in a row: v of 2^36, past fp16; weights of fp16's subnormals
