@@ -254,7 +254,7 @@ __device__ __forceinline__ void to_lines(u32x4& x, u32x4& y) { to_operands(x, y)
 // time (whole lines of x's and A's rows), every fourth such piece; NR * 16 rows of A against MT * 16 tokens, straight from
 // memory into the products. The four waves' sums meet in LDS, in a fixed order. Where a SIMD has few waves, or a wave few
 // pieces (decode), the next one's loads are on their way during one's products; else the other waves' are. Bound by memory:
-// 8191 tokens of 8192, 134 MB of x, in 33 us, 4.1 TB/s; 192 tokens of 48 adapters, 50 MB of A, in 14.7 us, 3.4 TB/s.
+// 8191 tokens of 8192, 134 MB of x, in 33 us, 4.1 TB/s.
 template <int MT, int NR, bool F16>
 __global__ __launch_bounds__(kThreads, MT == 1 ? 1 : MT * NR <= 8 ? 4 : 2) void shrink_kernel(const LoraArgs a) {
   constexpr int TM = 16 * MT;
@@ -267,7 +267,8 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 1 : MT * NR <= 8 ? 4 : 2) void 
   } else {
     if (!read_tile<TM>(a, blockIdx.x, rows, adapter, count)) return;
   }
-  const int rank_group = NR == 4 ? blockIdx.y / a.splits : 0, split = blockIdx.y - rank_group * a.splits;
+  constexpr bool kGroups = MT == 1 ? NR == 2 : NR == 4;  // of rows of A there may be more than one
+  const int rank_group = kGroups ? blockIdx.y / a.splits : 0, split = blockIdx.y - rank_group * a.splits;
   const int r0 = rank_group * 16 * NR, rank = rank_of(a, adapter) - r0;
   if (rank <= 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
@@ -605,6 +606,9 @@ using namespace aklr;
 
 namespace {
 
+// Rows of A, in sixteens, that a workgroup of the first product takes: others take the rest of a larger rank.
+constexpr int shrink_nr(int mt, int nr) { return mt == 1 && nr > 2 ? 2 : nr > 4 ? 4 : nr; }
+
 struct Plan {
   int mt, nr;         // tiles of 16 tokens, of 16 rank rows
   int64_t tiles;      // workgroups along x: the most tiles there can be
@@ -618,24 +622,29 @@ int64_t up(int64_t v, int64_t q) { return (v + q - 1) / q * q; }
 // The plan of a call, from its sizes alone. Measured on 8 adapters, bf16, us (both sides of each choice):
 // - up to 256 tokens each wave looks for its tile: 120 tokens of 4096 x 4096, rank 16: 9.6 (sorted: 14.8), 250: 11.0 (15.7).
 // - 64 tokens a tile from 7168 tokens on, 32 below: 8191 of 8192 x 10240, rank 32: 120 (32 a tile: 131), rank 64: 142
-//   (163); 6000 of 4096 x 4096, rank 16: 46 (64 a tile: 53), 6269 of 840 x 5512: 55 (57), 3000 and fewer the same.
-// - as many ranges of K as make the workgroups that run at once, of at least 512: 192 tokens of 48 adapters, 8192 x 10240,
-//   rank 64: 29.2 (11 ranges), 29.4 (8), 30.9 (16). That call is bound by the adapters' weights, 66 MB in 14.5 + 15.5 us.
-// - 256 columns a workgroup, 512 where that makes more than 2048: the same call 29.2 (256: 30.4, 1024: 31.5), 8191 of 8192 x
-//   10240 120 (256: 123, 1024: 122).
+//   (163); 6000 of 4096 x 4096, rank 16: 46 (64 a tile: 53), 6269 of 840 x 5512: 55 (57), 3000 and fewer the same. Above
+//   rank 32, where a tile's weights are more than its tokens, from 2560 on: 5000 of 8192 x 2048, rank 64: 52.9 (60.9), rank
+//   128: 78 (101), 2600 of 4096 x 4096, rank 128: 51 (56); 2000 of 8192 x 2048, rank 64: 36.5 (64 a tile: 40.7).
+// - up to 256 tokens 32 rows of A a workgroup: 4 tokens of 7168 x 2112, rank 64: 10.2 (64 rows: 12.3, 16: 9.9), 64 of 7168
+//   x 4608, rank 128: 17.7 (19.3, 18.6), 200 of 2048 x 8192, rank 64: 15.6 (17.7, 15.9).
+// - as many ranges of K as make the workgroups that run at once, of at least 512; up to 256 tokens six workgroups a CU: 192
+//   tokens of 48 adapters, 8192 x 10240, rank 64: 27.6 (four a CU: 28.4, eight: 30.1).
+// - 256 columns a workgroup, 512 where that makes more than 2048: the same call 27.6 (256: 1.2 more, 1024: 2.3), 8191 of
+//   8192 x 10240 120 (256: 123, 1024: 122).
 // - v joined by a launch of its own (3 to 5 us) where workgroups would read and convert much of it again and again, a
 //   conversion about as much as eight parts' reads: 8191 of 8192 x 10240, rank 32: 120 (from its parts 129), of 4096 x
 //   4096, rank 128: 107 (114), 3000 of 4096 x 4096, rank 64: 42.5 (joined 43.9), rank 16: 30.9 (34.4).
 Plan plan_lora(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapters) {
   Plan p{};
   p.nr = rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8;
-  p.rank_groups = p.nr == 8 ? 2 : 1;
   const bool sorts = tokens > kScan;
-  p.mt = !sorts ? 1 : tokens < 7168 ? 2 : 4;
+  p.mt = !sorts ? 1 : tokens < (p.nr < 4 ? 7168 : 2560) ? 2 : 4;
+  p.rank_groups = p.nr / shrink_nr(p.mt, p.nr);
   const int64_t tm = 16 * p.mt, groups = adapters + 1 < tokens ? adapters + 1 : tokens;
   const int64_t most = (tokens + tm - 1) / tm + groups;  // sum of ceil(c / tm) over groups of c tokens
   p.tiles = most < tokens ? most : tokens;
-  int64_t splits = 256 * (p.nr < 4 ? 4 : p.mt < 4 ? 3 : 2) / (p.tiles * p.rank_groups);  // by what registers leave room for
+  // what registers leave room for, and for one token a tile more, since their work is uneven
+  int64_t splits = 256 * (p.mt == 1 ? 6 : p.nr < 4 ? 4 : p.mt < 4 ? 3 : 2) / (p.tiles * p.rank_groups);
   if (splits > (k + 511) / 512) splits = (k + 511) / 512;
   if (splits < 1) splits = 1;
   p.k_split = up((k + splits - 1) / splits, 256);
@@ -732,7 +741,7 @@ extern "C" int aklr_lora_project(const void* x, int64_t x_stride, const void* a,
   const auto go = [&](auto mt, auto nr, auto f16) -> int {
     constexpr int MT = decltype(mt)::value, NR = decltype(nr)::value;
     constexpr bool F16 = decltype(f16)::value;
-    hipLaunchKernelGGL((shrink_kernel<MT, NR == 8 ? 4 : NR, F16>), shrink, dim3(kThreads), 0, stream, g);
+    hipLaunchKernelGGL((shrink_kernel<MT, shrink_nr(MT, NR), F16>), shrink, dim3(kThreads), 0, stream, g);
     AKLR_LAUNCH_CHECK();
     if constexpr (MT > 1) {
       if (p.joins) {
