@@ -250,6 +250,21 @@ __device__ __forceinline__ void to_operands(u32x4& x, u32x4& y) {  // from lines
 }
 __device__ __forceinline__ void to_lines(u32x4& x, u32x4& y) { to_operands(x, y); }  // its own inverse
 
+// Which tile and which part of it a workgroup takes. Above rank 32, where weights are much of what is read, the tiles of one
+// part follow each other on one XCD, whose L2 then has their adapters' weights: 1000 tokens of 4096 x 4096, rank 64: 25.8 us
+// (29.7 as workgroups come), rank 128: 34.0 (39.4), 600 of 8192 x 8192 and 16 adapters, rank 128: 41.0 (47.8). With fewer
+// parts (LEAST) XCDs would share them unevenly: 5000 of 8192 x 2048, rank 64: 54.4 (52.9). 1500 of 8192 x 8192,
+// rank 64, lose: 48.0 (45.9). Of rank 16 and 32 it gave nothing.
+struct Spot {
+  int tile, part;
+};
+template <bool WEIGHTS, int LEAST>
+__device__ __forceinline__ Spot spot() {
+  if (!WEIGHTS || gridDim.y < LEAST) return {(int)blockIdx.x, (int)blockIdx.y};
+  const uint32_t id = xcd_remap_any(blockIdx.x + gridDim.x * blockIdx.y, gridDim.x * gridDim.y), part = id / gridDim.x;
+  return {(int)(id - part * gridDim.x), (int)part};
+}
+
 // v's part of a tile, a range of K and up to 64 rows of A (ranges of K first along blockIdx.y). A wave takes 64 of K at a
 // time (whole lines of x's and A's rows), every fourth such piece; NR * 16 rows of A against MT * 16 tokens, straight from
 // memory into the products. The four waves' sums meet in LDS, in a fixed order. Where a SIMD has few waves, or a wave few
@@ -257,18 +272,19 @@ __device__ __forceinline__ void to_lines(u32x4& x, u32x4& y) { to_operands(x, y)
 // 8191 tokens of 8192, 134 MB of x, in 33 us, 4.1 TB/s.
 template <int MT, int NR, bool F16>
 __global__ __launch_bounds__(kThreads, MT == 1 ? 1 : MT * NR <= 8 ? 4 : 2) void shrink_kernel(const LoraArgs a) {
+  const Spot at = spot<(MT > 1 && NR == 4), 8>();
   constexpr int TM = 16 * MT;
   __shared__ int all_rows[MT == 1 ? kThreads / 64 : 1][TM];
   __shared__ f32x4 meet[2][NR][MT][64];
   int adapter, count;
   int(&rows)[TM] = all_rows[MT == 1 ? threadIdx.x >> 6 : 0];
   if constexpr (MT == 1) {
-    if (!find_tile<TM>(a, blockIdx.x, rows, adapter, count, blockIdx.y == 0)) return;
+    if (!find_tile<TM>(a, at.tile, rows, adapter, count, at.part == 0)) return;
   } else {
-    if (!read_tile<TM>(a, blockIdx.x, rows, adapter, count)) return;
+    if (!read_tile<TM>(a, at.tile, rows, adapter, count)) return;
   }
   constexpr bool kGroups = MT == 1 ? NR == 2 : NR == 4;  // of rows of A there may be more than one
-  const int rank_group = kGroups ? blockIdx.y / a.splits : 0, split = blockIdx.y - rank_group * a.splits;
+  const int rank_group = kGroups ? at.part / a.splits : 0, split = at.part - rank_group * a.splits;
   const int r0 = rank_group * 16 * NR, rank = rank_of(a, adapter) - r0;
   if (rank <= 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
@@ -447,16 +463,17 @@ enum Mode : int { kParts, kJoined, kStreamed };  // v from its parts, joined, an
 
 template <int MT, int NR, bool F16, Mode MODE>
 __global__ __launch_bounds__(kThreads) void expand_kernel(const LoraArgs a) {
+  const Spot at = spot<(MT > 1 && NR >= 4), 16>();
   constexpr int TM = 16 * MT, R = 16 * NR, kSteps = (R + 31) / 32, kRow = kSteps * 32 + 8;  // a row of pieces: 16 bytes more
   constexpr bool kStream = MODE == kStreamed;
   __shared__ int rows[TM];
   __shared__ __align__(16) uint16_t piece[2][TM][kRow];
   __shared__ int power[TM];
   int adapter, count;
-  if (!read_tile<TM>(a, blockIdx.x, rows, adapter, count)) return;
+  if (!read_tile<TM>(a, at.tile, rows, adapter, count)) return;
   const int rank = rank_of(a, adapter);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
-  const int c0 = blockIdx.y * a.n_group, c1 = min(c0 + a.n_group, a.n);
+  const int c0 = at.part * a.n_group, c1 = min(c0 + a.n_group, a.n);
   if (rank == 0) {
     if (!a.copies) return;
     constexpr int kAhead = 4;
