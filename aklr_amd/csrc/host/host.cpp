@@ -4,7 +4,8 @@
 // outputs, or None where the general Python path has to decide: a call outside the contract, a disabled or
 // traced op, out=, trans_b=False, a tensor subclass, an active torch mode, a missing or unknown argument.
 // It serves exactly what that path would serve, in the same way: the checks of aklr_amd/gemm.py, quant.py, rotary.py,
-// kv_cache.py, attention.py, drafts.py, kv_pages.py and lora.py, then torch's allocator for outputs and scratch and the C ABI on the current stream.
+// kv_cache.py, attention.py, drafts.py, kv_pages.py and lora.py, then torch's allocator for outputs and scratch and the C ABI
+// on the current stream.
 // Nothing is kept between calls, and the GIL is released around allocation and launch.
 //
 // Why: a decode GEMM takes 3 to 20 us on the GPU, and its call took 12 to 17 us on the host (argument
