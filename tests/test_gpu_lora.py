@@ -106,6 +106,17 @@ def test_who_has_which(t):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("t,k,n,r,count", [(300, 4104, 4104, 64, 3), (700, 2056, 4360, 128, 6), (2600, 4096, 4096, 40, 2), (257, 4360, 8200, 104, 40)])
+def test_many_ranges_of_columns(t, k, n, r, count, dtype):
+    say(f"lora ranges {t} {k} {n} {r} {count} {dtype}")
+    for kind in ("mixed", "runs"):
+        p = problem(t, k, n, r, count, dtype, t + n, kind)
+        got = call(p)
+        check(got, p, kind)
+        assert torch.equal(call(p), got)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("t,r", [(9, 8), (70, 24), (200, 128), (400, 64), (2300, 16), (2100, 128), (7200, 64)])
 def test_ranks_and_what_lies_behind_them(t, r, dtype):
     say(f"lora ranks {t} {r} {dtype}")
