@@ -5,8 +5,8 @@
 // workgroups of the second would convert again is joined by one between them):
 //   shrink  v[t, r] = sum_k x[t, k] A[r, k], K split over workgroups (fp32 parts in the workspace) and over a workgroup's
 //           four waves, on 16x16x32 products with the adapter's rows as one operand and tokens as the other;
-//   expand  the parts added in their order, v as two 16-bit pieces (hi + lo: what is left of v's rounding is 2^-17 of it
-//           for bf16, 2^-23 for fp16), products with B's rows, base added in fp32, one rounding.
+//   expand  the parts added in their order, v in 16-bit pieces (three for bf16, which hold all 24 bits of it; two for fp16,
+//           off by 2^-23 of the token's largest), products with B's rows, base added in fp32, one rounding.
 // Up to 256 tokens a workgroup finds its tile by itself, from all tokens' adapters; more are put in the adapters' order by a
 // launch before. A token's row of a tile changes no result: the products' columns do not meet.
 //
@@ -48,7 +48,7 @@ struct LoraArgs {
   const float* scales;
   const int32_t* ranks;
   float* part;  // [splits][tokens][rank rounded up to the products' rows]
-  uint16_t* joined;  // [2][tokens][..] pieces, and powers [tokens], of many tokens
+  uint16_t* joined;  // [pieces][tokens][..], and powers [tokens], of many tokens
   int32_t* powers;
   int32_t* order;
   Tile* tiles;
@@ -380,16 +380,25 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 1 : MT * NR <= 8 ? 4 : 2) void 
   }
 }
 
-// Two 16-bit pieces of x: hi, and what hi's rounding left.
+// x as a sum of 16-bit pieces, the largest first. bf16 holds 8 bits: three pieces, each what is left cut to its first 8 bits,
+// are x itself (down to bf16's least subnormal), and a finite x has none that is not. fp16 holds 11: x is at most 1 here, and
+// two pieces leave 2^-24. What is not finite is the first piece, with nothing behind it.
+constexpr int pieces_of(bool f16) { return f16 ? 2 : 3; }
+
 template <bool F16>
-__device__ __forceinline__ void pieces(float x, uint32_t& hi, uint32_t& lo) {
+__device__ __forceinline__ void pieces(float x, uint32_t (&to)[pieces_of(F16)]) {
+  const bool finite = __builtin_isfinite(x);
   if constexpr (F16) {
     const _Float16 h = (_Float16)x;
-    hi = __builtin_bit_cast(uint16_t, h);
-    lo = f32_to_f16_bits(__builtin_isfinite(x) ? x - (float)h : 0.0f);
+    to[0] = __builtin_bit_cast(uint16_t, h);
+    to[1] = f32_to_f16_bits(finite ? x - (float)h : 0.0f);
   } else {
-    hi = f32_to_bf16_bits(x);
-    lo = f32_to_bf16_bits((hi & 0x7F80u) != 0x7F80u ? x - bf16_lo(hi) : 0.0f);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const uint32_t first = __float_as_uint(x) & 0xFFFF0000u;
+      to[i] = first >> 16;
+      x = finite ? x - __uint_as_float(first) : 0.0f;
+    }
   }
 }
 
@@ -401,10 +410,11 @@ __device__ __forceinline__ float from16(uint32_t bits) {
     return bf16_lo(bits);
 }
 
-// Four values of v of a token from r on, their parts added in order, as pieces hi[0] | hi[1] << 16 ... fp16 has no room for
+// Four values of v of a token from r on, their parts added in order, each piece of the four side by side. fp16 has no room for
 // every v: the largest of a token's becomes 0.5 to 1, by a power of two. R / 4 lanes side by side have one token.
 template <int R, bool F16>
-__device__ __forceinline__ void join_four(const LoraArgs& a, int token, int r, int rank, u32x2& hi, u32x2& lo, int& power) {
+__device__ __forceinline__ void join_four(const LoraArgs& a, int token, int r, int rank, u32x2 (&to)[pieces_of(F16)],
+                                          int& power) {
   f32x4 v = {0, 0, 0, 0};
   if (r < rank) {
     const float* from = a.part + (int64_t)token * R + r;
@@ -433,11 +443,11 @@ __device__ __forceinline__ void join_four(const LoraArgs& a, int token, int r, i
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = __builtin_amdgcn_ldexpf(v[j], -power);
   }
-  uint32_t h[4], l[4];
+  uint32_t w[4][pieces_of(F16)];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) pieces<F16>(v[e], h[e], l[e]);
-  hi = u32x2{h[0] | h[1] << 16, h[2] | h[3] << 16};
-  lo = u32x2{l[0] | l[1] << 16, l[2] | l[3] << 16};
+  for (int e = 0; e < 4; ++e) pieces<F16>(v[e], w[e]);
+#pragma unroll
+  for (int i = 0; i < pieces_of(F16); ++i) to[i] = u32x2{w[0][i] | w[1][i] << 16, w[2][i] | w[3][i] << 16};
 }
 
 // Where many workgroups need the same parts of v: joined once, not by each of them.
@@ -446,12 +456,13 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const LoraArgs a) {
   constexpr int R = 16 * NR;
   const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   const int token = (int)min(id / (R / 4), (int64_t)a.tokens - 1), r = (int)(id % (R / 4)) * 4;
-  u32x2 hi, lo;
+  u32x2 v[pieces_of(F16)];
   int power;
-  join_four<R, F16>(a, token, r, rank_of(a, adapter_of(a, token)), hi, lo, power);
+  join_four<R, F16>(a, token, r, rank_of(a, adapter_of(a, token)), v, power);
   if (id >= (int64_t)a.tokens * (R / 4)) return;
-  *reinterpret_cast<u32x2*>(a.joined + (int64_t)token * R + r) = hi;
-  *reinterpret_cast<u32x2*>(a.joined + ((int64_t)a.tokens + token) * R + r) = lo;
+#pragma unroll
+  for (int i = 0; i < pieces_of(F16); ++i)
+    *reinterpret_cast<u32x2*>(a.joined + ((int64_t)i * a.tokens + token) * R + r) = v[i];
   if (F16 && r == 0) a.powers[token] = power;
 }
 
@@ -465,9 +476,10 @@ template <int MT, int NR, bool F16, Mode MODE>
 __global__ __launch_bounds__(kThreads) void expand_kernel(const LoraArgs a) {
   const Spot at = spot<(MT > 1 && NR >= 4), 16>();
   constexpr int TM = 16 * MT, R = 16 * NR, kSteps = (R + 31) / 32, kRow = kSteps * 32 + 8;  // a row of pieces: 16 bytes more
+  constexpr int kPieces = pieces_of(F16);
   constexpr bool kStream = MODE == kStreamed;
   __shared__ int rows[TM];
-  __shared__ __align__(16) uint16_t piece[2][TM][kRow];
+  __shared__ __align__(16) uint16_t piece[kPieces][TM][kRow];
   __shared__ int power[TM];
   int adapter, count;
   if (!read_tile<TM>(a, at.tile, rows, adapter, count)) return;
@@ -528,26 +540,26 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(const LoraArgs a) {
     for (int i = 0; i < (TM * kLanes + kThreads - 1) / kThreads; ++i) {
       const int id = i * kThreads + threadIdx.x, t = id / kLanes, r = id % kLanes * 4;
       if (TM * kLanes % kThreads != 0 && t >= TM) break;
-      u32x2 hi, lo;
+      u32x2 v[kPieces];
       int e;
-      join_four<R, F16>(a, rows[t], r, t < count ? rank : 0, hi, lo, e);
-      *reinterpret_cast<u32x2*>(&piece[0][t][r]) = hi;
-      *reinterpret_cast<u32x2*>(&piece[1][t][r]) = lo;
+      join_four<R, F16>(a, rows[t], r, t < count ? rank : 0, v, e);
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) *reinterpret_cast<u32x2*>(&piece[p][t][r]) = v[p];
       if (r == 0) power[t] = e;
     }
   } else {
-    constexpr int kPieces = TM * R / 8;  // of 16 bytes
+    constexpr int kEach = TM * R / 8;  // 16 bytes each
 #pragma unroll
-    for (int i = 0; i < (2 * kPieces + kThreads - 1) / kThreads; ++i) {
-      const int id = i * kThreads + threadIdx.x, low = id / kPieces, t = id % kPieces / (R / 8), r = id % (R / 8) * 8;
-      if (2 * kPieces % kThreads != 0 && low >= 2) break;
-      *reinterpret_cast<u32x4*>(&piece[low][t][r]) = ld16(a.joined + ((int64_t)low * a.tokens + rows[t]) * R + r);
+    for (int i = 0; i < (kPieces * kEach + kThreads - 1) / kThreads; ++i) {
+      const int id = i * kThreads + threadIdx.x, p = id / kEach, t = id % kEach / (R / 8), r = id % (R / 8) * 8;
+      if (kPieces * kEach % kThreads != 0 && p >= kPieces) break;
+      *reinterpret_cast<u32x4*>(&piece[p][t][r]) = ld16(a.joined + ((int64_t)p * a.tokens + rows[t]) * R + r);
     }
     if (F16 && (int)threadIdx.x < TM) power[threadIdx.x] = a.powers[rows[threadIdx.x]];
   }
   if (R < 32 && (int)threadIdx.x < TM) {  // the products' K is 32
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(&piece[i / 2][threadIdx.x][R + i % 2 * 8]) = u32x4{0, 0, 0, 0};
+    for (int i = 0; i < 2 * kPieces; ++i) *reinterpret_cast<u32x4*>(&piece[i / 2][threadIdx.x][R + i % 2 * 8]) = u32x4{0, 0, 0, 0};
   }
   __syncthreads();
   const float scale = a.scales ? a.scales[adapter] : 1.0f;
@@ -574,12 +586,12 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(const LoraArgs a) {
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         if (s >= steps) break;
-        const u32x4 hi = *reinterpret_cast<const u32x4*>(&piece[0][m * 16 + li][s * 32 + g * 8]);
-        const u32x4 lo = *reinterpret_cast<const u32x4*>(&piece[1][m * 16 + li][s * 32 + g * 8]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) acc[q] = product<F16>(w[s][q], lo, acc[q]);
+        for (int p = kPieces - 1; p >= 0; --p) {
+          const u32x4 v = *reinterpret_cast<const u32x4*>(&piece[p][m * 16 + li][s * 32 + g * 8]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) acc[q] = product<F16>(w[s][q], hi, acc[q]);
+          for (int q = 0; q < 4; ++q) acc[q] = product<F16>(w[s][q], v, acc[q]);
+        }
       }
       if (m + 1 == MT && after < c1) load_w(after);
       const int e = F16 ? power[m * 16 + li] : 0;
@@ -676,7 +688,7 @@ Plan plan_lora(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapt
   p.part = at;
   at += up(4 * p.splits * tokens * 16 * p.nr, 256);
   p.joined = at;
-  if (p.joins) at += up(4 * tokens * 16 * p.nr, 256);
+  if (p.joins) at += up(2 * pieces_of(false) * tokens * 16 * p.nr, 256);
   p.powers = at;
   if (p.joins) at += up(4 * tokens, 256);
   p.bytes = at;

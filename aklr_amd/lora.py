@@ -11,8 +11,8 @@
   x, base and out may be rows of something wider, a and b slices of what several projections stack: the last dimension is
   contiguous and everything else lies on 16 bytes. ``out``: where the result goes, base itself for in place.
 
-  x a^T is held in 32 bits and enters the second product as two 16-bit pieces, which keep 2^-17 (bf16) or 2^-23 (fp16, of the
-  token's largest) of it; base is added in fp32, and the sum rounded once. What is not finite in a token or in its adapter
+  x a^T is held in 32 bits and enters the second product as 16-bit pieces: whole (bf16, three pieces) or off by 2^-23 of the
+  token's largest (fp16, two); base is added in fp32, and the sum rounded once. What is not finite in a token or in its adapter
   comes out not finite, an infinity perhaps as NaN, and no other token sees it.
 
 Nothing waits for the GPU, and a captured call serves other adapters of the same shapes. Calls it does not serve return a
