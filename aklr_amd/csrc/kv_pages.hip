@@ -67,8 +67,8 @@ __global__ __launch_bounds__(kThreads) void copy_kernel(const Side k, const Side
 
 // ---------------------------------------------------------------------------------------------------------------
 // Compaction: position first + path[b, i] onto first + i, first = seq_lens[b] - T, T = starts[b + 1] - starts[b], for
-// i < counts[b]. path ascends, so an item's place lies at or before its source, and a place may be the source of an
-// earlier item, never of a later one.
+// i < counts[b]. Entries outside [0, T) are passed over wherever they stand; the others ascend. An item's place lies at or before
+// its source, and a place may be the source of an earlier item, never of a later one.
 struct CompactArgs {
   Side k, v;
   const int32_t *table, *lens, *starts, *path, *counts;
@@ -176,25 +176,29 @@ __global__ __launch_bounds__(kThreads) void compact_short_kernel(const CompactAr
 constexpr int kRows = 32;
 constexpr int kSavers = 16;  // workgroups of a sequence that look for what to copy aside
 
+// Whether anything of a tile may be copied aside, by its first entry alone, for both launches: path ascends, so not if that is
+// a position behind the window. An entry that is no position says nothing of those behind it.
+__device__ __forceinline__ bool looked_at(const CompactArgs& a, int b, int i0) {
+  const int32_t x = a.path[(int64_t)b * a.path_row + i0];
+  return x < a.w1 || x >= (int64_t)a.starts[b + 1] - a.starts[b];
+}
+
 template <int D, bool SAVE>
 __global__ __launch_bounds__(kThreads) void compact_long_kernel(const CompactArgs a) {
   constexpr int U = D / 16;
   __shared__ Place from[kRows], to[kRows];
   __shared__ int aside[kRows], any;
+  __shared__ uint64_t ahead[kThreads / 64];
   const int tiles = (a.w1 - a.w0 + kRows - 1) / kRows, groups = SAVE ? min(tiles, kSavers) : tiles;
-  const int seq = blockIdx.x / groups, b = a.b0 + seq;
-  for (int tile = blockIdx.x - seq * groups; tile < tiles; tile += groups) {
-    const int i0 = a.w0 + tile * kRows;
-    if (i0 >= a.counts[b]) return;
-    // path ascends: where a tile's first item comes from behind the window, nothing of it or of those behind is copied aside
-    if (SAVE && a.path[(int64_t)b * a.path_row + i0] >= a.w1) return;
+  const int seq = blockIdx.x / groups, b = a.b0 + seq, items = min(a.counts[b], a.w1);
+  const auto move = [&](int i0, bool looked) {  // the tile that begins with item i0
     __syncthreads();
     if (threadIdx.x < 64) {
       Place f = {-1, 0}, t = {-1, 0};
       int source = -1;
       const int i = i0 + threadIdx.x;
       if (threadIdx.x < kRows && i < a.w1) item_of(a, b, i, f, t, source);
-      const bool kept = f.page >= 0 && source < a.w1;
+      const bool kept = f.page >= 0 && looked && source < a.w1;
       if (SAVE && !kept) f.page = -1;
       const uint64_t on = __ballot(f.page >= 0);
       if (threadIdx.x < kRows) {
@@ -205,7 +209,7 @@ __global__ __launch_bounds__(kThreads) void compact_long_kernel(const CompactArg
       if (threadIdx.x == 0) any = on != 0;
     }
     __syncthreads();
-    if (!any) continue;
+    if (!any) return;
     const Side& s = blockIdx.y ? a.v : a.k;
     // the copies' rows: [keys or values][sequence][item of the window][head]
     const int64_t row0 = ((int64_t)blockIdx.y * a.batch + seq) * (a.w1 - a.w0) + (i0 - a.w0);
@@ -246,6 +250,24 @@ __global__ __launch_bounds__(kThreads) void compact_long_kernel(const CompactArg
         *copy = *old;
       else
         *now = aside[r] ? *copy : *old;
+    }
+  };
+  const int first = blockIdx.x - seq * groups;
+  if constexpr (!SAVE) {
+    const int i0 = a.w0 + first * kRows;
+    if (i0 < items) move(i0, looked_at(a, b, i0));
+  } else {  // a lane a tile looks which there are, then those one after the other
+    for (int tile0 = first; tile0 < tiles; tile0 += groups * kThreads) {
+      const int tile = tile0 + (int)threadIdx.x * groups, i0 = a.w0 + tile * kRows;
+      const uint64_t on = __ballot(tile < tiles && i0 < items && looked_at(a, b, i0));
+      __syncthreads();  // the last round's reads are done
+      if ((threadIdx.x & 63) == 0) ahead[threadIdx.x >> 6] = on;
+      __syncthreads();
+#pragma unroll 1
+      for (int w = 0; w < kThreads / 64; ++w)
+#pragma unroll 1
+        for (uint64_t left = ahead[w]; left; left &= left - 1)
+          move(a.w0 + (tile0 + (w * 64 + __ffsll((unsigned long long)left) - 1) * groups) * kRows, true);
     }
   }
 }

@@ -359,8 +359,9 @@ int aklr_kv_cache_copy_pages_fp8(void* k_codes, void* v_codes, float* k_scales, 
 
 /*
  * Kept positions of a paged cache moved together: of the last T = starts[b + 1] - starts[b] of seq_lens[b] positions, number
- * path[b * path_stride + i] becomes number i, for i < min(counts[b], most). path ascends. Entries outside [0, T), and those of
- * which the source or the place lies in a page that the cache does not have, are skipped. batch <= 65536, most <= 2^28,
+ * path[b * path_stride + i] becomes number i, for i < min(counts[b], most). Entries outside [0, T) are skipped, wherever they
+ * stand, the others ascend; skipped too are those of which the source or the place lies in a page that the cache does not have.
+ * Of a path that does not ascend, what the places hold is not defined. batch <= 65536, most <= 2^28,
  * table_cols * page_size <= 2^28. The pages moved to belong to one sequence. Workspace:
  * aklr_kv_cache_compact_fp8_workspace_bytes(batch, most, kv_heads, head_dim), any content, up to 128 MiB; none for most <= 64.
  */
