@@ -67,8 +67,11 @@ __global__ __launch_bounds__(kThreads) void copy_kernel(const Side k, const Side
 
 // ---------------------------------------------------------------------------------------------------------------
 // Compaction: position first + path[b, i] onto first + i, first = seq_lens[b] - T, T = starts[b + 1] - starts[b], for
-// i < counts[b]. Entries outside [0, T) are passed over wherever they stand; the others ascend. An item's place lies at or before
-// its source, and a place may be the source of an earlier item, never of a later one.
+// i < counts[b]. Entries outside [0, T) are passed over wherever they stand; the others, the items, ascend. Without such entries
+// each item moves down (i < path[i]) or stays; behind some it may move up. A place of an item that moves down may be the source
+// of an earlier one that does, never of a later one; of one that moves up, of a later one, never of an earlier one. And none of
+// one kind is a source of the other: of items i < j one has path[i] < path[j], so i < path[i] gives i < path[j], and j > path[j]
+// gives j > path[i].
 struct CompactArgs {
   Side k, v;
   const int32_t *table, *lens, *starts, *path, *counts;
@@ -79,6 +82,7 @@ struct CompactArgs {
   int w0, w1;         // its items
   uint8_t* saved;     // [2][sequences of the launch][w1 - w0][heads][D] codes, then the scales
   float* saved_scales;
+  int32_t* up;        // with several windows: whether there are items that move up, which these leave alone
 };
 
 struct Place {  // of a position: its page, -1 where the cache has none, and the token's place in it
@@ -106,70 +110,80 @@ __device__ __forceinline__ void item_of(const CompactArgs& a, int b, int i, Plac
   source = x;
 }
 
-// Short paths: the accepted ones of drafted tokens. A lane owns 16 bytes of one head (or its scale) for every item of a
-// sequence and goes through them in order, kHeld at a time: it reads what it will move before it writes, and nothing that a
-// later round reads has been written. A workgroup takes a sequence's units kThreads at a time; the items' places are
-// worked out once, a lane an item. Bound by its chain of loads (lengths and path, table, rows): 64 sequences of 5 kept tokens,
-// 8 heads of 128, 4.4 us; two launches of the long form's kind would take 9.
-constexpr int kShort = 64, kHeld = 8;
+// Items in an order in which nothing is read that has been written: those that move down from the first, those that move up
+// from the last. A lane owns 16 bytes of one head (or its scale) for every item of a sequence, kHeld at a time: it reads what it
+// will move before it writes. A workgroup takes a sequence's units kThreads at a time; the items' places are worked out
+// once, a lane an item, kShort in a round.
+// Short paths, the accepted ones of drafted tokens, are one round. Bound by its chain of loads (lengths and path, table, rows):
+// 64 sequences of 5 kept tokens, 8 heads of 128, 4.4 us; two launches of the long form's kind would take 9. UP: of paths in
+// several windows, the items that move up, rounds from the last, one after the other: 90000 of them, 8 heads of 128, 15 ms.
+// Where there are none, as in every path without entries that are passed over, it ends at once.
+constexpr int kShort = 64;
 
-template <int D>
+template <int D, bool UP>
 __global__ __launch_bounds__(kThreads) void compact_short_kernel(const CompactArgs a) {
-  constexpr int U = D / 16;
+  constexpr int U = D / 16, kHeld = UP ? 32 : 8;
   __shared__ Place from[kShort], to[kShort];
   __shared__ int moved;
-  const int b = a.b0 + blockIdx.x;
-  if (threadIdx.x < 64) {
-    Place f = {-1, 0}, t = {-1, 0};
-    int source;
-    if ((int)threadIdx.x < a.most) item_of(a, b, threadIdx.x, f, t, source);
-    const uint64_t on = __ballot(f.page >= 0);
-    if (f.page >= 0) {  // items in order, those that stay left out
-      const int at = __popcll(on & ((1ull << threadIdx.x) - 1));
-      from[at] = f;
-      to[at] = t;
+  if (UP && !*a.up) return;
+  const int b = a.b0 + blockIdx.x, units = a.heads * U;
+  const int last = UP ? max(min(a.counts[b], a.most) - 1, 0) / kShort * kShort : 0;
+  for (int first = last; first >= 0; first -= kShort) {
+    if (UP) __syncthreads();  // the last round's reads are done
+    if (threadIdx.x < 64) {
+      Place f = {-1, 0}, t = {-1, 0};
+      int source = -1;
+      const int i = first + (int)threadIdx.x;
+      if (i < a.most) item_of(a, b, i, f, t, source);
+      const bool on = f.page >= 0, rises = source < i;
+      const uint64_t down = __ballot(on && !rises), up = __ballot(on && rises), below = (1ull << threadIdx.x) - 1;
+      if (on && (rises || !UP)) {
+        const int at = rises ? (UP ? 0 : __popcll(down)) + __popcll(up & ~below) - 1 : __popcll(down & below);
+        from[at] = f;
+        to[at] = t;
+      }
+      if (threadIdx.x == 0) moved = __popcll(UP ? up : up | down);
     }
-    if (threadIdx.x == 0) moved = __popcll(on);
-  }
-  __syncthreads();
-  const int n = moved, units = a.heads * U;
-  if (n == 0) return;
-  for (int id = blockIdx.y * kThreads + threadIdx.x; id < 2 * (units + a.heads); id += gridDim.y * kThreads) {
-    const bool scale = id >= 2 * units;
-    const int r = scale ? id - 2 * units : id;
-    const bool second = r >= (scale ? a.heads : units);
-    const int x = r - (second ? (scale ? a.heads : units) : 0);
-    const Side& s = second ? a.v : a.k;
-    const int head = scale ? x : x / U, u = scale ? 0 : x % U;
-    const auto locate = [&](const Place& p) -> int64_t {
-      const int64_t token = (int64_t)head * a.page + p.off;
-      return scale ? p.page * s.scale_page + token : p.page * s.code_page + token * D + u * 16;
-    };
-    for (int i0 = 0; i0 < n; i0 += kHeld) {
-      u32x4 held[kHeld];
-      if (scale) {
+    __syncthreads();
+    const int n = moved;
+    for (int id = blockIdx.y * kThreads + threadIdx.x; id < 2 * (units + a.heads); id += gridDim.y * kThreads) {
+      const bool scale = id >= 2 * units;
+      const int r = scale ? id - 2 * units : id;
+      const bool second = r >= (scale ? a.heads : units);
+      const int x = r - (second ? (scale ? a.heads : units) : 0);
+      const Side& s = second ? a.v : a.k;
+      const int head = scale ? x : x / U, u = scale ? 0 : x % U;
+      const auto locate = [&](const Place& p) -> int64_t {
+        const int64_t token = (int64_t)head * a.page + p.off;
+        return scale ? p.page * s.scale_page + token : p.page * s.code_page + token * D + u * 16;
+      };
+      for (int i0 = 0; i0 < n; i0 += kHeld) {
+        u32x4 held[kHeld];
+        if (scale) {
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j)
-          if (i0 + j < n) held[j][0] = __float_as_uint(s.scales[locate(from[i0 + j])]);
+          for (int j = 0; j < kHeld; ++j)
+            if (i0 + j < n) held[j][0] = __float_as_uint(s.scales[locate(from[i0 + j])]);
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j)
-          if (i0 + j < n) s.scales[locate(to[i0 + j])] = __uint_as_float(held[j][0]);
-      } else {
+          for (int j = 0; j < kHeld; ++j)
+            if (i0 + j < n) s.scales[locate(to[i0 + j])] = __uint_as_float(held[j][0]);
+        } else {
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j)
-          if (i0 + j < n) held[j] = ld16(s.codes + locate(from[i0 + j]));
+          for (int j = 0; j < kHeld; ++j)
+            if (i0 + j < n) held[j] = ld16(s.codes + locate(from[i0 + j]));
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j)
-          if (i0 + j < n) *reinterpret_cast<u32x4*>(s.codes + locate(to[i0 + j])) = held[j];
+          for (int j = 0; j < kHeld; ++j)
+            if (i0 + j < n) *reinterpret_cast<u32x4*>(s.codes + locate(to[i0 + j])) = held[j];
+        }
       }
     }
   }
 }
 
 // Long paths (contexts cut to the positions worth keeping) in windows of items, each in two launches: SAVE copies the items
-// whose source is a place of the window (i < path[i] < w1) aside, then every item of the window moves, those from the copy.
-// All items of a launch are independent, so it fills the chip whatever the path; what lies past the window's places, as
-// after a cut that drops more than it keeps, is read once. A workgroup takes kRows items of a sequence, for keys or values.
+// whose source is a place of the window (path[i] < w1) aside, then every item of the window moves, those from the copy. With
+// several windows an item that moves up may have its source in one before: those are left to compact_short_kernel. All items
+// of a launch are independent, so it fills the chip whatever the path; what lies past the window's places, as after a cut that
+// drops more than it keeps, is read once. A workgroup takes kRows items of a sequence, for keys or values.
 // Bound by memory: 8 contexts cut from 16384 to 4095 positions, 8 heads of 128, 85 MB moved, 24.8 us with 4.5 us of SAVE;
 // the move is 4.1 TB/s, of rows of 128 bytes at a head's distance from each other. Eight loads a lane in flight instead of four
 // take 29 to 31, non-temporal stores the same.
@@ -198,6 +212,11 @@ __global__ __launch_bounds__(kThreads) void compact_long_kernel(const CompactArg
       int source = -1;
       const int i = i0 + threadIdx.x;
       if (threadIdx.x < kRows && i < a.w1) item_of(a, b, i, f, t, source);
+      if (a.up) {
+        if (!SAVE && __ballot(f.page >= 0 && source < i) && threadIdx.x == 0)
+          __hip_atomic_store(a.up, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (source < i) f.page = -1;
+      }
       const bool kept = f.page >= 0 && looked && source < a.w1;
       if (SAVE && !kept) f.page = -1;
       const uint64_t on = __ballot(f.page >= 0);
@@ -253,6 +272,7 @@ __global__ __launch_bounds__(kThreads) void compact_long_kernel(const CompactArg
     }
   };
   const int first = blockIdx.x - seq * groups;
+  if (SAVE && a.up && a.w0 == 0 && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.up = 0;
   if constexpr (!SAVE) {
     const int i0 = a.w0 + first * kRows;
     if (i0 < items) move(i0, looked_at(a, b, i0));
@@ -502,7 +522,11 @@ Windows windows_of(int64_t batch, int64_t most, int64_t kv_heads, int64_t head_d
   if (most <= kShort || batch < 1) return {most, batch, 0};
   const int64_t item = 2 * kv_heads * (head_dim + 4);  // at most 520 KiB
   const int64_t fit = kSaveBytes / item;               // at least 252
-  int64_t items = most < fit ? most : fit / kRows * kRows;
+  if (most > fit) {  // several windows, and behind their copies whether items move up
+    const int64_t items = (fit - 1) / kRows * kRows;
+    return {items, 1, (items + 1) * item};
+  }
+  const int64_t items = most;
   int64_t sequences = fit / items;
   const int64_t tiles = (items + kRows - 1) / kRows;
   if (sequences > kMostGroups / 2 / tiles) sequences = kMostGroups / 2 / tiles;
@@ -513,15 +537,15 @@ Windows windows_of(int64_t batch, int64_t most, int64_t kv_heads, int64_t head_d
 template <int D>
 int compact(CompactArgs a, int64_t batch, uint8_t* ws, hipStream_t stream) {
   const Windows w = windows_of(batch, a.most, a.heads, D);
+  const unsigned in_order = (unsigned)((2ll * a.heads * (D / 16 + 1) + kThreads - 1) / kThreads);
   if (a.most <= kShort) {
-    const int64_t lanes = 2ll * a.heads * (D / 16 + 1);
     a.b0 = 0;
     a.batch = (int)batch;
-    const dim3 grid((unsigned)batch, (unsigned)((lanes + kThreads - 1) / kThreads));
-    hipLaunchKernelGGL(compact_short_kernel<D>, grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((compact_short_kernel<D, false>), dim3((unsigned)batch, in_order), dim3(kThreads), 0, stream, a);
     AKLR_LAUNCH_CHECK();
     return AKLR_OK;
   }
+  if (w.items < a.most) a.up = reinterpret_cast<int32_t*>(ws + w.items * 2 * a.heads * (D + 4));
   for (int64_t b0 = 0; b0 < batch; b0 += w.sequences) {
     a.b0 = (int)b0;
     a.batch = (int)(batch - b0 < w.sequences ? batch - b0 : w.sequences);
@@ -534,6 +558,10 @@ int compact(CompactArgs a, int64_t batch, uint8_t* ws, hipStream_t stream) {
       hipLaunchKernelGGL((compact_long_kernel<D, true>), dim3((unsigned)(a.batch * savers), 2), dim3(kThreads), 0, stream, a);
       AKLR_LAUNCH_CHECK();
       hipLaunchKernelGGL((compact_long_kernel<D, false>), dim3((unsigned)(a.batch * tiles), 2), dim3(kThreads), 0, stream, a);
+      AKLR_LAUNCH_CHECK();
+    }
+    if (a.up) {
+      hipLaunchKernelGGL((compact_short_kernel<D, true>), dim3((unsigned)a.batch, in_order), dim3(kThreads), 0, stream, a);
       AKLR_LAUNCH_CHECK();
     }
   }

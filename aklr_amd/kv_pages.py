@@ -8,7 +8,8 @@
   ``counts[b]`` with the numbers ``path[b]`` (int32 [batch, most], ascending) become the first ones: position
   ``seq_lens[b] - T + path[b, i]`` moves to ``seq_lens[b] - T + i``. That is what ``verify_drafts`` returns for the drafts of
   ``tree_attention_fp8``'s call; with T the whole length it cuts a context to the positions worth keeping. Returns the four
-  tensors. Positions in pages that the cache does not have stay, and so does what is not kept, behind. The pages that
+  tensors. Positions in pages that the cache does not have stay, and so does what is not kept, behind. Entries of a path that
+  are none of the T positions, wherever they stand, are passed over; the others ascend. The pages that
   positions move to belong to one sequence. Those behind what ``kv_cache_update_pages`` was last told to keep do; whoever cuts
   a context whose first pages others hold too copies them before.
 - ``kv_cache_update_pages(page_refs, block_table, lens, new_lens, page_size, parents=None)`` says which pages each sequence
