@@ -958,7 +958,8 @@ PyObject* lora(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
   for (const Tensor* t : {x, a, b, base, scales, out})
     if (wants_grad(t)) Py_RETURN_NONE;
   if (out && (!pieces_ok(*out, type, {tokens, n}) || !no_inner_overlap(*out) || !(same_place(*out, *base) || apart(out, base)) ||
-              !apart_all(out, {x, a, b, ids, scales, ranks})))
+              !(apart(out, x) || (same_place(*out, *x) && same_place(*out, *base))) ||
+              !apart_all(out, {a, b, ids, scales, ranks})))
     Py_RETURN_NONE;
   Tensor o, ws;
   int st;

@@ -7,6 +7,7 @@
 //           four waves, on 16x16x32 products with the adapter's rows as one operand and tokens as the other;
 //   expand  the parts added in their order, v in 16-bit pieces (three for bf16, which hold all 24 bits of it; two for fp16,
 //           off by 2^-23 of the token's largest), products with B's rows, base added in fp32, one rounding.
+// Only the first reads x, so out may lie where x and base do.
 // Up to 256 tokens a workgroup finds its tile by itself, from all tokens' adapters; more are put in the adapters' order by a
 // launch before. A token's row of a tile changes no result: the products' columns do not meet.
 //

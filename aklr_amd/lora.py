@@ -9,7 +9,8 @@
   given. ``ranks``: int32 [adapters], 0 to R: the rows of a[i] and columns of b[i] from there on are not read (they may hold
   anything). K, N and R are multiples of 8, K up to 65536, N up to 262144, R up to 128; up to 2^20 tokens and 4096 adapters.
   x, base and out may be rows of something wider, a and b slices of what several projections stack: the last dimension is
-  contiguous and everything else lies on 16 bytes. ``out``: where the result goes, base itself for in place.
+  contiguous and everything else lies on 16 bytes. ``out``: where the result goes, base itself for in place (x may then be
+  base too), else apart from all that is read.
 
   x a^T is held in 32 bits and enters the second product as 16-bit pieces: whole (bf16, three pieces) or off by 2^-23 of the
   token's largest (fp16, two); base is added in fp32, and the sum rounded once. What is not finite in a token or in its adapter
@@ -75,8 +76,7 @@ def _run_lora(p: _LoraPlan):
 
 @api("lora_project@1.0", _run_lora, native="lora")
 def lora_project(x, a, b, adapters, base, *, scales=None, ranks=None, out=None):
-    inputs = [x, a, b, adapters, base] + [t for t in (scales, ranks) if t is not None]
-    given = inputs + ([out] if out is not None else [])
+    given = [x, a, b, adapters, base] + [t for t in (scales, ranks, out) if t is not None]
     if not tensors_ok(*given) or x.dim() != 2 or b.dim() != 3 or x.dtype not in _OUT:
         return _OOC
     (tokens, k), (count, n, rank) = x.shape, b.shape
@@ -99,6 +99,8 @@ def lora_project(x, a, b, adapters, base, *, scales=None, ranks=None, out=None):
     if out is not None:
         if not _pieces_ok(out, x.dtype, tokens, n) or not no_inner_overlap(out):
             return _OOC
-        if not (same_place(out, base) or apart(out, base)) or not all(apart(out, t) for t in inputs if t is not base):
+        if not (same_place(out, base) or apart(out, base)) or not all(apart(out, t) for t in (a, b, adapters, scales, ranks)):
+            return _OOC
+        if not (apart(out, x) or (same_place(out, x) and same_place(out, base))):
             return _OOC
     return _LoraPlan(x, a, b, adapters, base, scales, ranks, out, "decode" if tokens <= 256 else "sorted")

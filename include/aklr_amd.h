@@ -415,7 +415,8 @@ int aklr_verify_drafts(const void* target_probs, int64_t target_stride, const vo
  * Low-rank adapters beside a shared projection: out[t] = base[t] + scales[i] * (x[t] a[i]^T) b[i]^T, i = adapters[t] (int32, or
  * int64 with adapters_64); out[t] = base[t] where i is outside [0, adapter_count). x [tokens, k], a [adapter_count, rank, k],
  * b [adapter_count, n, rank], base and out [tokens, n] of dtype (bf16, fp16), the last dimension contiguous, other strides in
- * elements, multiples of 8, pointers aligned to 16 bytes; out is base (same pointer and stride) or apart from all inputs.
+ * elements, multiples of 8, pointers aligned to 16 bytes; out is base (same pointer and stride; x may be there too) and apart
+ * from the other inputs, or apart from all.
  * scales fp32 (NULL: 1), ranks int32 (NULL: rank): of adapter i only the first ranks[i] rows of a and columns of b are used.
  * k, n, rank multiples of 8; k <= 65536, n <= 262144, rank <= 128, tokens <= 2^20, adapter_count <= 4096.
  * Workspace: aklr_lora_project_workspace_bytes(...), any content.
