@@ -67,11 +67,11 @@ __global__ __launch_bounds__(kThreads) void copy_kernel(const Side k, const Side
 
 // ---------------------------------------------------------------------------------------------------------------
 // Compaction: position first + path[b, i] onto first + i, first = seq_lens[b] - T, T = starts[b + 1] - starts[b], for
-// i < counts[b]. Entries outside [0, T) are passed over wherever they stand; the others, the items, ascend. Without such entries
-// each item moves down (i < path[i]) or stays; behind some it may move up. A place of an item that moves down may be the source
-// of an earlier one that does, never of a later one; of one that moves up, of a later one, never of an earlier one. And none of
-// one kind is a source of the other: of items i < j one has path[i] < path[j], so i < path[i] gives i < path[j], and j > path[j]
-// gives j > path[i].
+// i < counts[b]. Entries outside [0, T) are passed over wherever they stand; the others, the items, ascend. Without such
+// entries each item moves down (i < path[i]) or stays; behind some it may move up. A place of an item that moves down may be
+// the source of an earlier one that does, never of a later one; of one that moves up, of a later one, never of an earlier
+// one. And no place of one kind is a source of the other: of items i < j one has path[i] < path[j], so i < path[i] gives
+// i < path[j], and j > path[j] gives j > path[i].
 struct CompactArgs {
   Side k, v;
   const int32_t *table, *lens, *starts, *path, *counts;
@@ -111,8 +111,8 @@ __device__ __forceinline__ void item_of(const CompactArgs& a, int b, int i, Plac
 }
 
 // Items in an order in which nothing is read that has been written: those that move down from the first, those that move up
-// from the last. A lane owns 16 bytes of one head (or its scale) for every item of a sequence, kHeld at a time: it reads what it
-// will move before it writes. A workgroup takes a sequence's units kThreads at a time; the items' places are worked out
+// from the last. A lane owns 16 bytes of one head (or its scale) for every item of a sequence, kHeld at a time: it reads what
+// it will move before it writes. A workgroup takes a sequence's units kThreads at a time; the items' places are worked out
 // once, a lane an item, kShort in a round.
 // Short paths, the accepted ones of drafted tokens, are one round. Bound by its chain of loads (lengths and path, table, rows):
 // 64 sequences of 5 kept tokens, 8 heads of 128, 4.4 us; two launches of the long form's kind would take 9. UP: of paths in
@@ -184,9 +184,10 @@ __global__ __launch_bounds__(kThreads) void compact_short_kernel(const CompactAr
 // several windows an item that moves up may have its source in one before: those are left to compact_short_kernel. All items
 // of a launch are independent, so it fills the chip whatever the path; what lies past the window's places, as after a cut that
 // drops more than it keeps, is read once. A workgroup takes kRows items of a sequence, for keys or values.
-// Bound by memory: 8 contexts cut from 16384 to 4095 positions, 8 heads of 128, 85 MB moved, 24.8 us with 4.5 us of SAVE;
+// Bound by memory: 8 contexts cut from 16384 to 4095 positions, 8 heads of 128, 85 MB moved, 25.0 us with 4.6 us of SAVE;
 // the move is 4.1 TB/s, of rows of 128 bytes at a head's distance from each other. Eight loads a lane in flight instead of four
-// take 29 to 31, non-temporal stores the same.
+// take 29 to 31, non-temporal stores the same. Where most is copied aside its bytes move twice: as many positions of the same
+// contexts, scattered, 51; all but 7 early ones 64, all but 1000 early ones 59.
 constexpr int kRows = 32;
 constexpr int kSavers = 16;  // workgroups of a sequence that look for what to copy aside
 
@@ -371,6 +372,8 @@ __device__ __forceinline__ void settle() {
 // its chain of loads and atomics, 7 to 9 us: a lane keeps what it knows of its first sequence, so that up to 1024 are read
 // once, and the first round's counts come beside that: all that changes among them is what this kernel claims, which LDS
 // remembers. Spread over workgroups it would wait for each of three steps by words in memory, about as long.
+// That is with free pages among the first 8192. The search begins at page 0 and ends with the last page asked for, or with the
+// pool: 2.8 us a round, so a pool whose low pages are all held costs its length: of 2^18 pages 93 us, of 2^20 358.
 __global__ __launch_bounds__(kJoin) void update_grow_kernel(const UpdateArgs a) {
   __shared__ int sums[kJoin / 64];
   __shared__ int32_t lds_before[kLdsRows], lds_begin[kLdsRows], list[kRound];

@@ -11,7 +11,8 @@
 // Up to 256 tokens a workgroup finds its tile by itself, from all tokens' adapters; more are put in the adapters' order by a
 // launch before. A token's row of a tile changes no result: the products' columns do not meet.
 //
-// Bound by memory: decode by the adapters' weights, prompts by x, base and out (figures at plan_lora).
+// Bound by memory in long prompts, by x, base and out, and in the second product of batches, by B; the first of batches up to
+// 256 tokens has 2.5 TB/s of A behind its search for a tile, and a few tokens are two chains of loads (figures at plan_lora).
 #include "common.h"
 #include "scan.h"
 
@@ -560,7 +561,8 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(const LoraArgs a) {
   }
   if (R < 32 && (int)threadIdx.x < TM) {  // the products' K is 32
 #pragma unroll
-    for (int i = 0; i < 2 * kPieces; ++i) *reinterpret_cast<u32x4*>(&piece[i / 2][threadIdx.x][R + i % 2 * 8]) = u32x4{0, 0, 0, 0};
+    for (int i = 0; i < 2 * kPieces; ++i)
+      *reinterpret_cast<u32x4*>(&piece[i / 2][threadIdx.x][R + i % 2 * 8]) = u32x4{0, 0, 0, 0};
   }
   __syncthreads();
   const float scale = a.scales ? a.scales[adapter] : 1.0f;
@@ -649,7 +651,8 @@ struct Plan {
 
 int64_t up(int64_t v, int64_t q) { return (v + q - 1) / q * q; }
 
-// The plan of a call, from its sizes alone. Measured on 8 adapters, bf16, us (both sides of each choice):
+// The plan of a call, from its sizes alone. Measured on 8 adapters, bf16, us (both sides of each choice, with two pieces of v;
+// the third takes 0.5 to 2 % more, 3 at rank 128 and 8191 tokens):
 // - up to 256 tokens each wave looks for its tile: 120 tokens of 4096 x 4096, rank 16: 9.6 (sorted: 14.8), 250: 11.0 (15.7).
 // - 64 tokens a tile from 7168 tokens on, 32 below: 8191 of 8192 x 10240, rank 32: 120 (32 a tile: 131), rank 64: 142
 //   (163); 6000 of 4096 x 4096, rank 16: 46 (64 a tile: 53), 6269 of 840 x 5512: 55 (57), 3000 and fewer the same. Above

@@ -10,8 +10,9 @@
 //
 // Bound by memory and, for few sequences, by its chain of loads: the whole rows p and q of one node a sequence, and once
 // more for each rejection that another child follows. Everything is in 64 bits: which token is drawn hangs on a running sum
-// over the vocabulary, and 32 bits would move some of its borders with the order of the additions. The sums are bound by the
-// loads all the same (figures at plan_verify).
+// over the vocabulary, and 32 bits would move some of its borders with the order of the additions; in 64 they move by some
+// 2^-50 of the row's sum. The order is set by the sizes, not by who arrives when. The sums are bound by the loads all the same
+// (figures at plan_verify).
 #include "common.h"
 #include "scan.h"
 
@@ -460,7 +461,9 @@ struct Plan {
 // - 16 trees of 33 tokens, vocabulary 128003: 33 with 16 workgroups a row; 44 with 4, 38 with 8, 76 with 32. 64 chains of
 //   8, vocabulary 131072: 18.2 with any of them, 67 MB of rows at 3.7 TB/s. 4 chains of 5, vocabulary 32000: 8.1.
 // - the same trees in 3 launches 42, 4: 30 to 33, 5: 36, 8: 36. A sequence adds up 1.6 rows at the mean, 3 or 4 at the most; a
-//   launch that finds its sequences done takes 1.3.
+//   launch that finds its sequences done takes 1.3. Chosen for trees like these; where many siblings fall one after the other,
+//   each past the fourth takes 15 to 20: 16 roots of 4 siblings 33 to 37, of 8 (all fall in some) 82 to 119, of 20 142 to 375.
+// - drafts without rows take one launch whatever falls: the same trees 12, 64 chains of 8 15.8, 4 chains of 5 8.4.
 // - four units' loads in flight a wave instead of two no longer fit the registers.
 // What bounds a call of few sequences is its chain of dependent loads, starts, then parents and tokens, then what the rows hold
 // for them, then the rows, at 0.8 to 2 us each, and the 64-bit tail: a lone wave issues a vector instruction every five cycles.

@@ -9,11 +9,12 @@ probabilities after each query token, ``draft_probs`` (the same shape and type, 
 after it were drawn from, independently of each other; without it the drafts were certain (a greedy draft, the likeliest tokens).
 
   At a node with rows p and q its drafts are tried in their order, from W = p, S = 1. Draft i with token x stands if
-  ``accept_uniforms[i]`` * S * q(x) < W(x) (without q: < W(x) alone), and the search goes on at it; else
+  ``accept_uniforms[i]`` * S * q(x) < W(x) (without q: ``accept_uniforms[i]`` * S < W(x)), and the search goes on at it; else
   W = max(W - S q, 0) and S = sum(W) (without q: S -= W(x), then W(x) = 0). Where none stands, the next token is the
   least v for which W(0) + ... + W(v) > ``sample_uniforms[b]`` * sum(W). Drafts drawn from q and uniform numbers make the
   tokens that come out the target's own samples. Where nothing is left of W, p itself is sampled; a row without any
-  probability gives -1. All of it is computed in 64 bits: the result does not hang on the order of a sum.
+  probability gives -1. All of it is computed in 64 bits, the sums in an order that the sizes alone set, so a call repeats
+  itself; another order of the same sums may decide otherwise where a number is within some 2^-50 of a row's sum of a border.
 
   uniforms: fp32 [tokens] and [batch], in [0, 1); others count as the nearest that is, NaN as 0. Entries of the rows that
   are negative, infinite or NaN count as 0; rows need not add up to 1. Rows may lie apart, each is contiguous. A draft whose

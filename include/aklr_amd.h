@@ -396,7 +396,8 @@ int aklr_kv_cache_update_pages(int32_t* page_refs, int64_t pages, const int32_t*
  * before). At a node with target row p and draft row q its drafts are tried in order, from W = p, S = 1: token x stands if
  * accept_uniforms[i] * S * q(x) < W(x), else W = max(W - S q, 0), S = sum(W); with draft_probs NULL if
  * accept_uniforms[i] * S < W(x), else S -= W(x), W(x) = 0. Where none stands, the next token is the least v with
- * W(0) + ... + W(v) > sample_uniforms[b] * sum(W); p itself where sum(W) is 0, -1 where p's is too. In 64 bits.
+ * W(0) + ... + W(v) > sample_uniforms[b] * sum(W); p itself where sum(W) is 0, -1 where p's is too. In 64 bits, sums in an
+ * order of the kernel's own.
  * target_probs, draft_probs: rows of vocab values of dtype (AKLR_OUT_BF16, AKLR_OUT_F16, AKLR_F32), rows *_stride elements
  * apart; what is negative, infinite or NaN counts as 0. Uniforms are cut to [0, 1 - 2^-24], NaN to 0. A draft with a token
  * outside [0, vocab), or a parent that does not come before it, is passed over, and so are those past `most`.
@@ -419,7 +420,8 @@ int aklr_verify_drafts(const void* target_probs, int64_t target_stride, const vo
  * from the other inputs, or apart from all.
  * scales fp32 (NULL: 1), ranks int32 (NULL: rank): of adapter i only the first ranks[i] rows of a and columns of b are used.
  * k, n, rank multiples of 8; k <= 65536, n <= 262144, rank <= 128, tokens <= 2^20, adapter_count <= 4096.
- * Workspace: aklr_lora_project_workspace_bytes(...), any content.
+ * Workspace: aklr_lora_project_workspace_bytes(...), any content: at most 14 MiB up to 8192 tokens, of many some 10 bytes for
+ * each token and each of the rank rounded up to a power of two, 1.3 GiB for 2^20 tokens of rank 128.
  */
 size_t aklr_lora_project_workspace_bytes(int64_t tokens, int64_t k, int64_t n, int64_t rank, int64_t adapter_count);
 int aklr_lora_project(const void* x, int64_t x_stride, const void* a, int64_t a_adapter_stride, int64_t a_row_stride,
