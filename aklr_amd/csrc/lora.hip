@@ -6,7 +6,7 @@
 //   shrink  v[t, r] = sum_k x[t, k] A[r, k], K split over workgroups (fp32 parts in the workspace) and over a workgroup's
 //           four waves, on 16x16x32 products with the adapter's rows as one operand and tokens as the other;
 //   expand  the parts added in their order, v in 16-bit pieces (three for bf16, which hold all 24 bits of it; two for fp16,
-//           off by 2^-23 of the token's largest), products with B's rows, base added in fp32, one rounding.
+//           off by 2^-23 of it or 2^-39 of the token's largest), products with B's rows, base added in fp32, one rounding.
 // Only the first reads x, so out may lie where x and base do.
 // Up to 256 tokens a workgroup finds its tile by itself, from all tokens' adapters; more are put in the adapters' order by a
 // launch before. A token's row of a tile changes no result: the products' columns do not meet.
@@ -383,8 +383,8 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 1 : MT * NR <= 8 ? 4 : 2) void 
 }
 
 // x as a sum of 16-bit pieces, the largest first. bf16 holds 8 bits: three pieces, each what is left cut to its first 8 bits,
-// are x itself (down to bf16's least subnormal), and a finite x has none that is not. fp16 holds 11: x is at most 1 here, and
-// two pieces leave 2^-24. What is not finite is the first piece, with nothing behind it.
+// are x itself (down to bf16's least subnormal), and a finite x has none that is not. fp16 holds 11: two pieces leave 2^-23 of
+// x, or half its least subnormal, 2^-25. What is not finite is the first piece, with nothing behind it.
 constexpr int pieces_of(bool f16) { return f16 ? 2 : 3; }
 
 template <bool F16>
@@ -413,7 +413,8 @@ __device__ __forceinline__ float from16(uint32_t bits) {
 }
 
 // Four values of v of a token from r on, their parts added in order, each piece of the four side by side. fp16 has no room for
-// every v: the largest of a token's becomes 0.5 to 1, by a power of two. R / 4 lanes side by side have one token.
+// every v: the largest of a token's becomes 2^14 to 2^15, by a power of two, so that 2^-25 is 2^-39 of it and the small ones keep
+// their bits too. R / 4 lanes side by side have one token.
 template <int R, bool F16>
 __device__ __forceinline__ void join_four(const LoraArgs& a, int token, int r, int rank, u32x2 (&to)[pieces_of(F16)],
                                           int& power) {
@@ -441,7 +442,7 @@ __device__ __forceinline__ void join_four(const LoraArgs& a, int token, int r, i
     for (int j = 0; j < 4; ++j) top = fmaxf(top, __builtin_isfinite(v[j]) ? fabsf(v[j]) : 0.0f);
 #pragma unroll
     for (int d = 1; d < R / 4; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
-    power = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) : 0;
+    power = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = __builtin_amdgcn_ldexpf(v[j], -power);
   }

@@ -12,8 +12,8 @@
   contiguous and everything else lies on 16 bytes. ``out``: where the result goes, base itself for in place (x may then be
   base too), else apart from all that is read.
 
-  x a^T is held in 32 bits and enters the second product as 16-bit pieces: whole (bf16, three pieces) or off by 2^-23 of the
-  token's largest (fp16, two); base is added in fp32, and the sum rounded once. What is not finite in a token or in its adapter
+  x a^T is held in 32 bits and enters the second product as 16-bit pieces: whole (bf16, three pieces) or off by 2^-23 of it
+  or 2^-39 of the token's largest (fp16, two); base is added in fp32, and the sum rounded once. What is not finite in a token or in its adapter
   comes out not finite, an infinity perhaps as NaN, and no other token sees it.
 
 Nothing waits for the GPU, and a captured call serves other adapters of the same shapes. Calls it does not serve return a
