@@ -413,8 +413,8 @@ __device__ __forceinline__ float from16(uint32_t bits) {
 }
 
 // Four values of v of a token from r on, their parts added in order, each piece of the four side by side. fp16 has no room for
-// every v: the largest of a token's becomes 2^14 to 2^15, by a power of two, so that 2^-25 is 2^-39 of it and the small ones keep
-// their bits too. R / 4 lanes side by side have one token.
+// every v: the largest of a token's becomes 2^14 to 2^15, by a power of two, so that 2^-25 is 2^-39 of it and the small ones
+// keep their bits too. R / 4 lanes side by side have one token.
 template <int R, bool F16>
 __device__ __forceinline__ void join_four(const LoraArgs& a, int token, int r, int rank, u32x2 (&to)[pieces_of(F16)],
                                           int& power) {
